@@ -9,7 +9,8 @@ id; a state always belongs to one run, also when the run reads another run's pag
 model's embedding (`embedding_need`), which may look back at a request's tokens.
 
 `CacheStorage` allocates one pool per group, [planes, pages, parts (K, V; or one), kv heads,
-page_size, head size] in the compute dtype, the state arrays, and the native `CacheManager` that owns
+page_size, head size] in the compute dtype (a group whose needs are `packed`: uint8 [planes, pages, kv heads, page_size / 16,
+bytes of a block of 16 positions in 4 bits]), the state arrays, and the native `CacheManager` that owns
 the page and slot numbers.  Page size and page counts are parameters (the pool is sized for
 the tokens the caller wants resident, or for a fraction of the free HBM).
 """
@@ -21,13 +22,15 @@ from typing import List, Optional
 import torch
 
 from .. import host
+from ..errors import ConfigError
+from ..ops import lib as ops
 
 
 @dataclass
 class LayerCache:
     """What one run of a layer may touch."""
     group: Optional[int]            # index into ctx.block_tables, None when the mixer keeps no pages
-    plane: Optional[torch.Tensor]   # [pages, 2, Hkv, page_size, D]
+    plane: Optional[torch.Tensor]   # [pages, 2, Hkv, page_size, D]; in 4 bits: uint8 [pages, Hkv, page_size / 16, block bytes]
     page_stride: int                # elements from one page to the next
     page_size: int
     writes: bool                    # False: reads the plane another run wrote
@@ -40,6 +43,7 @@ class CacheLayout:
         self.schedule = model.schedule
         self.group_keys: List[tuple] = []
         self.group_keep_first: List[int] = []
+        self.group_packed: List[bool] = []       # per group: held in 4 bits
         self.group_planes: List[int] = []
         self.run_group: List[Optional[int]] = []
         self.run_plane: List[Optional[int]] = []
@@ -54,8 +58,8 @@ class CacheLayout:
             if run.cache_of is not None:
                 j = run.cache_of
                 a, b = need.paged, self.needs[j].paged
-                if (a is None) != (b is None) or (a is not None and (a.n_kv_heads, a.head_dim, a.parts) !=
-                                                  (b.n_kv_heads, b.head_dim, b.parts)):
+                if (a is None) != (b is None) or (a is not None and (a.n_kv_heads, a.head_dim, a.parts, a.packed) !=
+                                                  (b.n_kv_heads, b.head_dim, b.parts, b.packed)):
                     raise ValueError(f"run {k} cannot read the cache of run {j}: their needs differ")
                 if a is not None:
                     keep[j].append(a.window)
@@ -69,11 +73,15 @@ class CacheLayout:
                 window = 0 if min(keep[k]) <= 0 else max(keep[k])
                 key = (need.paged.n_kv_heads, need.paged.head_dim, window, need.paged.parts)
                 kept = first[k] if window else 0
-                if (key, kept) not in zip(self.group_keys, self.group_keep_first):
+                if need.paged.packed and need.paged.parts != 2:
+                    raise ValueError("a cache in 4 bits holds keys and values")
+                own = (key, kept, need.paged.packed)
+                if own not in zip(self.group_keys, self.group_keep_first, self.group_packed):
                     self.group_keys.append(key)
                     self.group_keep_first.append(kept)
+                    self.group_packed.append(need.paged.packed)
                     self.group_planes.append(0)
-                g = list(zip(self.group_keys, self.group_keep_first)).index((key, kept))
+                g = list(zip(self.group_keys, self.group_keep_first, self.group_packed)).index(own)
                 self.run_group.append(g)
                 self.run_plane.append(self.group_planes[g])
                 self.group_planes[g] += 1
@@ -94,7 +102,8 @@ class CacheLayout:
 
     def bytes_per_token(self, dtype) -> int:
         size = torch.empty((), dtype=dtype).element_size()
-        return sum(parts * h * d * planes * size for (h, d, _, parts), planes in zip(self.group_keys, self.group_planes))
+        return sum((h * ops.packed_block_bytes(d) // 16 if packed else parts * h * d * size) * planes
+                   for (h, d, _, parts), planes, packed in zip(self.group_keys, self.group_planes, self.group_packed))
 
 
 class CacheStorage:
@@ -123,7 +132,13 @@ class CacheStorage:
         self.manager = host.module().CacheManager(specs, int(max_requests))
         self.max_requests = int(max_requests)
         self.pools = []
+        if any(self.layout.group_packed) and self.page_size % 16:
+            raise ConfigError(f"a cache in 4 bits has pages of a multiple of 16 positions, found {self.page_size}")
         for g, (hkv, d, _w, parts) in enumerate(self.layout.group_keys):
+            if self.layout.group_packed[g]:
+                self.pools.append(torch.empty((self.layout.group_planes[g], pages[g], hkv, self.page_size // 16, ops.packed_block_bytes(d)),
+                                              dtype=torch.uint8, device=device))
+                continue
             self.pools.append(torch.empty((self.layout.group_planes[g], pages[g], parts, hkv, self.page_size, d),
                                           dtype=dtype, device=device))
         self.states = [torch.zeros((self.max_requests,) + tuple(n.shape), dtype=n.dtype, device=device)

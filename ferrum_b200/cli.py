@@ -8,13 +8,13 @@ errors, exit code 2 for usage errors and 1 for runtime errors, messages prefixed
 `SubmitRequest` and `SamplingParams` (crates/core-types/src/schedule.rs:16-49).
 
     ferrum generate --model DIR|FILE.gguf --prompt-tokens 1,2,3 [--prompt-tokens ...]
-                    [--dtype bfloat16|float16|float32] [--max-new-tokens N] [--temperature T] [--top-p 1]
-                    [--seed S] [--stop-tokens a,b] [--max-batch-tokens N] [--max-batch-seqs N]
+                    [--dtype bfloat16|float16|float32] [--max-new-tokens N] [--temperature T] [--top-k K] [--top-p P]
+                    [--min-p P] [--cache-bits 4|16] [--seed S] [--stop-tokens a,b] [--max-batch-tokens N] [--max-batch-seqs N]
                     [--chunk-size N] [--page-size N] [--num-pages N] [--max-model-len N]
                     [--random-weights] [--weights-seed S] [--stats] [--profile]
     ferrum random-weights --config CONFIG.json --out DIR [--seed S] [--dtype float32|bfloat16|float16] [--gguf]
     ferrum bench --model DIR|CONFIG.json [--random-weights] [--dtype D] [--batch B] [--prompt-len P] [--new-tokens N]
-                 [--layers L] [--page-size N] [--chunk-size N] [--seed S]
+                 [--layers L] [--page-size N] [--chunk-size N] [--cache-bits 4|16] [--seed S]
     ferrum replay --model DIR --dtype D --out DIR --max-tokens N        (steps on standard input)
     ferrum dump FILE.gguf|FILE.safetensors|DIR
     ferrum serve                                                          (not part of this engine)
@@ -30,13 +30,13 @@ USAGE = "usage: ferrum generate|random-weights|bench|replay|dump|serve [options]
 # option -> (kind, repeatable)
 OPTIONS = {
     "generate": {"--model": "str", "--prompt-tokens": "tokens+", "--prompt-file": "str", "--dtype": "str",
-                 "--max-new-tokens": "int", "--temperature": "float", "--top-p": "float", "--seed": "int",
-                 "--stop-tokens": "tokens", "--max-batch-tokens": "int", "--max-batch-seqs": "int",
+                 "--max-new-tokens": "int", "--temperature": "float", "--top-p": "float", "--top-k": "int", "--min-p": "float",
+                 "--cache-bits": "int", "--seed": "int", "--stop-tokens": "tokens", "--max-batch-tokens": "int", "--max-batch-seqs": "int",
                  "--chunk-size": "int", "--page-size": "int", "--num-pages": "int", "--max-model-len": "int",
                  "--random-weights": "flag", "--weights-seed": "int", "--stats": "flag", "--profile": "flag"},
     "random-weights": {"--config": "str", "--out": "str", "--seed": "int", "--dtype": "str", "--gguf": "flag"},
     "bench": {"--model": "str", "--random-weights": "flag", "--dtype": "str", "--batch": "int", "--prompt-len": "int",
-              "--new-tokens": "int", "--layers": "int", "--page-size": "int", "--chunk-size": "int", "--seed": "int"},
+              "--new-tokens": "int", "--layers": "int", "--page-size": "int", "--chunk-size": "int", "--cache-bits": "int", "--seed": "int"},
     "replay": {"--model": "str", "--dtype": "str", "--out": "str", "--max-tokens": "int", "--page-size": "int",
                "--max-requests": "int"},
     "dump": {},
@@ -126,12 +126,12 @@ def cmd_generate(opts):
     kw = {}
     for flag, name in (("--page-size", "page_size"), ("--num-pages", "num_pages"), ("--max-batch-tokens", "max_batch_tokens"),
                        ("--max-batch-seqs", "max_batch_seqs"), ("--chunk-size", "chunk_size"),
-                       ("--max-model-len", "max_model_len")):
+                       ("--max-model-len", "max_model_len"), ("--cache-bits", "cache_bits")):
         if flag in opts:
             kw[name] = opts[flag]
     eng = Engine(model, dtype=opts.get("--dtype", "bfloat16"), random_weights=bool(opts.get("--random-weights")),
                  seed=opts.get("--weights-seed", 0), profile=bool(opts.get("--profile")), **kw)
-    sp = SamplingParams(opts.get("--temperature", 0.0), opts.get("--top-p", 1.0), opts.get("--seed", 0))
+    sp = SamplingParams(opts.get("--temperature", 0.0), opts.get("--top-p", 1.0), opts.get("--seed", 0), opts.get("--top-k", 0), opts.get("--min-p", 0.0))
     ids = [eng.submit(p, opts.get("--max-new-tokens", 16), sp, opts.get("--stop-tokens", [])) for p in prompts]
     out, reasons = {i: [] for i in ids}, {}
     while len(reasons) < len(ids):
@@ -202,7 +202,8 @@ def cmd_bench(opts):
     else:
         model, _ = load_model(model_arg, dtype, max_positions=max_len)
     eng = Engine(model=model, page_size=page, num_pages=B * (-(-max_len // page)), max_batch_tokens=max(2048, B),
-                 max_batch_seqs=B, chunk_size=opts.get("--chunk-size", 0), max_model_len=max_len)
+                 max_batch_seqs=B, chunk_size=opts.get("--chunk-size", 0), max_model_len=max_len,
+                 cache_bits=opts.get("--cache-bits"))
     rng = random.Random(opts.get("--seed", 0))
     vocab = model.n_vocab
     for rep in range(2):                       # the first run captures the decode graphs

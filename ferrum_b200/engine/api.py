@@ -4,12 +4,12 @@
 (docs/ARCHITECTURE.md:15-26): registry -> model -> cache -> runner -> scheduler -> sampler.
 Request fields and their meanings follow the reference's `SubmitRequest` and
 `SamplingParams` (crates/core-types/src/schedule.rs:16-49): prompt_tokens, max_new_tokens,
-temperature (0 = greedy), top_p (kept for the interface, must be 1), seed, stop_tokens.
+temperature (0 = greedy), top_p, seed, stop_tokens; top_k and min_p are this engine's own.
 """
 from __future__ import annotations
 
 import os
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
 from typing import Dict, List, Optional, Sequence
 
 import numpy as np
@@ -20,7 +20,7 @@ from ..cache import CacheStorage
 from ..config import registry
 from ..errors import ConfigError, InvalidRequest
 from ..ops import lib as ops
-from ..sampling import DeviceSampler
+from ..sampling import DeviceSampler, Filters
 from ..weights import init_random, load_weights
 from .batch import StepEntry
 from .runner import ModelRunner
@@ -38,13 +38,15 @@ def parse_dtype(name):
         raise ConfigError(f"unsupported dtype {name!r}; choose bfloat16, float16 or float32") from None
 
 
-def load_model(path, dtype="bfloat16", device="cuda", max_positions=None, random_seed=None):
+def load_model(path, dtype="bfloat16", device="cuda", max_positions=None, random_seed=None, cache_bits=None):
     """(model, torch dtype) from a model folder.  With random_seed the folder needs only
-    config.json and the weights are drawn on the device."""
+    config.json and the weights are drawn on the device.  cache_bits: see `Engine`."""
     ops.require_cuda()
     td = parse_dtype(dtype)
     arch, cfg = registry.read_config(path)
     model = arch.build(cfg, td, device, max_positions=max_positions)
+    if cache_bits is not None:
+        model.set_cache_bits(int(cache_bits))
     if random_seed is not None:
         init_random(model, random_seed, device)
     else:
@@ -55,10 +57,14 @@ def load_model(path, dtype="bfloat16", device="cuda", max_positions=None, random
 
 @dataclass
 class SamplingParams:
-    """crates/core-types/src/schedule.rs:16-29."""
+    """crates/core-types/src/schedule.rs:16-29, and two more filters.  With a temperature a token is drawn from the logits' softmax at
+    that temperature after, in this order: the top_k largest stay (0: all), of these the smallest set of the likeliest that
+    holds a part top_p of their mass (1: all), of these the ones at least min_p times as likely as the likeliest (0: all)."""
     temperature: float = 0.0
     top_p: float = 1.0
     seed: int = 0
+    top_k: int = 0
+    min_p: float = 0.0
 
     @staticmethod
     def greedy():
@@ -80,13 +86,18 @@ _NOTHING_SAMPLED = object()      # stands for the ticket of a batch without samp
 class Engine:
     def __init__(self, model_path=None, dtype="bfloat16", random_weights=False, seed=0, page_size=16,
                  num_pages=None, max_batch_tokens=2048, max_batch_seqs=64, chunk_size=0, max_model_len=None,
-                 gpu_memory_fraction=0.85, device="cuda", model=None, plan_ahead=True, profile=False):
+                 gpu_memory_fraction=0.85, device="cuda", model=None, plan_ahead=True, profile=False, cache_bits=None):
+        """cache_bits: 4 holds keys and values in 4 bits an element (4.5 with the steps and middles of their groups of 64) instead
+        of the compute type: about 3.5 times the tokens fit and a decoded token reads that much less, for what 16
+        levels cost in precision.  For 16-bit Llama models with heads of 64 or 128 elements; others are refused (`ConfigError`).  None: as the model says."""
         ops.require_cuda()
         if model is None:
             model, td = load_model(model_path, dtype, device, max_positions=max_model_len,
-                                   random_seed=seed if random_weights else None)
+                                   random_seed=seed if random_weights else None, cache_bits=cache_bits)
         else:
             td = model.dtype
+            if cache_bits is not None:
+                model.set_cache_bits(int(cache_bits))
         self.model, self.dtype, self.device = model, td, device
         cfg = model.config
         self.max_model_len = int(max_model_len or getattr(cfg, "n_ctx_train", 4096))
@@ -111,6 +122,7 @@ class Engine:
         sc.eos_token_ids = [int(t) for t in eos]
         self.scheduler = host.module().Scheduler(self.cache.manager, sc)
         self._next_id = 0
+        self._filters = {}           # request id -> Filters, of live requests that have any
         self.plan_ahead = bool(plan_ahead)
         self._in_flight = None       # the sampling ticket of a batch that is on the GPU's queue
         if profile:
@@ -124,17 +136,21 @@ class Engine:
                stop_tokens: Sequence[int] = (), request_id: Optional[int] = None, temperature=None, seed=None) -> int:
         sp = sampling or SamplingParams()
         if temperature is not None:
-            sp = SamplingParams(float(temperature), sp.top_p, sp.seed)
+            sp = replace(sp, temperature=float(temperature))
         if seed is not None:
-            sp = SamplingParams(sp.temperature, sp.top_p, int(seed))
+            sp = replace(sp, seed=int(seed))
+        filters = Filters(sp.top_k, sp.top_p, sp.min_p)
         rid = self._next_id if request_id is None else int(request_id)
         self._next_id = max(self._next_id, rid) + 1
         self.scheduler.submit(rid, [int(t) for t in prompt_tokens], int(max_new_tokens), float(sp.temperature),
-                              float(sp.top_p), int(sp.seed) & 0xFFFFFFFFFFFFFFFF, [int(t) for t in stop_tokens])
+                              1.0, int(sp.seed) & 0xFFFFFFFFFFFFFFFF, [int(t) for t in stop_tokens])
+        if filters.on and sp.temperature > 0:      # (the scheduler knows nothing of filters; a request it refuses leaves none behind)
+            self._filters[rid] = filters
         return rid
 
     def cancel(self, request_id: int) -> None:
         self.scheduler.cancel(int(request_id))
+        self._filters.pop(int(request_id), None)
 
     # ------------------------------------------------------------------ one step
     def step(self) -> List[StepEvent]:
@@ -185,18 +201,22 @@ class Engine:
         logits = self.runner.step(entries, commit=False, check=False, ahead_of_commit=ahead_of_commit,
                                   tokens_on_device=sum(1 for p in plan if p.from_device))
         # the ids also go where a step queued behind this one looks for its tokens
-        return self.sampler.launch(logits, rows, also_to=self.runner.ctx.token_store) if rows else _NOTHING_SAMPLED
+        filters = [self._filters.get(p.id) for p in rows] if self._filters else None
+        return self.sampler.launch(logits, rows, also_to=self.runner.ctx.token_store, filters=filters) if rows else _NOTHING_SAMPLED
 
-    @staticmethod
-    def _events(raw):
+    def _events(self, raw):
+        for e in raw if self._filters else ():
+            if e.kind != 0:
+                self._filters.pop(e.id, None)
         return [StepEvent("token", e.id, token=e.token) if e.kind == 0 else
                 StepEvent("finished", e.id, reason=FINISH_REASONS[e.reason]) for e in raw]
 
     # ------------------------------------------------------------------ whole generations
     def generate(self, prompts: Sequence[Sequence[int]], max_new_tokens=16, temperature=0.0, seed=0,
-                 stop_tokens: Sequence[int] = ()) -> List[List[int]]:
+                 stop_tokens: Sequence[int] = (), top_k=0, top_p=1.0, min_p=0.0) -> List[List[int]]:
         """Generates for every prompt (token ids in, token ids out), batching them continuously."""
-        ids = [self.submit(p, max_new_tokens, SamplingParams(temperature, 1.0, seed), stop_tokens) for p in prompts]
+        sampling = SamplingParams(temperature, top_p, seed, top_k, min_p)
+        ids = [self.submit(p, max_new_tokens, sampling, stop_tokens) for p in prompts]
         out: Dict[int, List[int]] = {i: [] for i in ids}
         live = set(ids)
         while live:

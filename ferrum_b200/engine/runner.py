@@ -22,6 +22,7 @@ _DEVICE_ERRORS = {
     1: "a token id is outside the vocabulary", 2: "a position is outside the rotary table",
     3: "a position is beyond the block table", 4: "a token's page is missing from the block table",
     5: "attention reached a position whose page is missing", 6: "a row of logits is all NaN",
+    7: "a temperature, top_p or min_p is out of range",
     10: "tensor-core product: the producer timed out", 11: "tensor-core product: the matrix unit timed out",
     12: "tensor-core product: the epilogue timed out", 13: "tensor-core product: the accumulator was not released in time",
     14: "tensor-core product: partial tiles did not arrive in time",

@@ -16,6 +16,7 @@ import os
 
 import torch
 
+from ..errors import ConfigError
 from ..parts.base import CacheNeed, Part
 
 # FERRUM_NVTX=1: every step and every run of a block is an NVTX range (for a system profiler's timeline)
@@ -78,6 +79,25 @@ class DecoderModel(Part):
     def embedding_need(self):
         """What the embedding keeps per request beside the runs of the schedule (a `CacheNeed`)."""
         return self.embedding.cache_need() if hasattr(self.embedding, "cache_need") else CacheNeed()
+
+    def set_cache_bits(self, bits):
+        """Holds every layer's pages in `bits` bits an element: 4, or those of the compute type (the default).  Before the cache is
+        laid out (`CacheStorage`).  A model with a mixer that cannot is refused and stays as it was."""
+        mixers = [b.mixer for b in self.blocks if b.mixer is not None and b.mixer.cache_need().paged is not None]
+        own = 8 * self.dtype.itemsize
+        if not mixers and bits != own:
+            raise ConfigError(f"the model keeps no keys and values to hold in {bits} bits")
+        done = []
+        try:
+            for m in mixers:
+                packed = m.cache_need().paged.packed
+                if bits != own or packed:
+                    m.set_cache_bits(bits)
+                    done.append((m, 4 if packed else own))
+        except ConfigError:
+            for m, before in done:
+                m.set_cache_bits(before)
+            raise
 
     @property
     def n_vocab(self):

@@ -27,7 +27,7 @@ TC_STORE_BF16, TC_STORE_F32, TC_RESIDUAL, TC_SWIGLU, TC_GEGLU, TC_SWISH_CLAMP, T
 
 _lib = None
 _lock = threading.Lock()
-ABI = 24
+ABI = 25
 
 
 _CTYPES = (ctypes._SimpleCData, ctypes.Array, type(ctypes.byref(c_int())))
@@ -65,6 +65,7 @@ def lib():
                     raise KernelError(f"cannot load the kernel library {path}: {e}") from None
                 handle.ferrum_last_error.restype = ctypes.c_char_p
                 handle.ferrum_gemm_tc_workspace.restype = c_longlong
+                handle.ferrum_attention_packed_workspace.restype = c_longlong
                 handle.ferrum_matrix_memory_state_floats.restype = c_longlong
                 if handle.ferrum_kernels_abi() != ABI:
                     raise KernelError(f"{path} is a stale build; delete it and call again")
@@ -758,6 +759,96 @@ def attention_combine(out, part_o, part_ml, q_start, req_of_token, req_tile0, ti
            "attention_combine")
 
 
+# ----------------------------------------------------------------------------- a cache held in 4 bits
+def packed_block_bytes(D):
+    """Bytes of a block of a cache held in 4 bits: what 16 positions of a KV head of D elements take, keys and values (4.5 bits an
+    element); 0 for a head size that such a cache is not built for."""
+    return int(lib().ferrum_packed_block_bytes(D))
+
+
+def _need_packed(plane, page_stride, page_size, Hkv, D, name):
+    """The checks of a plane of packed pages, uint8 [pages, Hkv, page_size / 16, bytes of a block]."""
+    _need(plane, torch.uint8, "plane", 4)
+    if page_size <= 0 or page_size % 16 or packed_block_bytes(D) == 0:
+        raise KernelError(f"{name}: a cache in 4 bits has pages of a multiple of 16 positions and heads of 64 or 128 elements, found {page_size} and {D}")
+    if tuple(plane.shape[1:]) != (Hkv, page_size // 16, packed_block_bytes(D)) or not plane[0].is_contiguous() or page_stride != plane.stride(0):
+        raise KernelError(f"{name}: the plane must be [pages, {Hkv}, {page_size // 16}, {packed_block_bytes(D)}] with dense pages {page_stride} bytes apart")
+
+
+def _need_table(block_table, name):
+    _need(block_table, torch.int32, "block_table", 2)
+    if not block_table.is_contiguous():
+        raise KernelError(f"{name}: block_table must be contiguous")
+
+
+def rope_cache_write_packed(qkv, n_tokens, positions, req_of_token, block_table, cos_sin, plane, page_stride, page_size, Hq, Hkv, D, R, pairing,
+                            err, q_out=None, write_kv=True):
+    """Rotate q and k and store k and v in the pages of a cache held in 4 bits, quantised by groups of 64 elements.  The turned
+    q goes to `q_out` ([>= n_tokens, >= Hq * D]; None: in place).  plane: uint8 [pages, Hkv, page_size / 16, `packed_block_bytes(D)`]."""
+    _need16(qkv, "qkv", 2); _need(positions, torch.int32, "positions", 1); _need(req_of_token, torch.int32, "req_of_token", 1)
+    _need_table(block_table, "rope_cache_write_packed")
+    if q_out is not None:
+        _need16(q_out, "q_out", 2, like=qkv)
+    q = qkv if q_out is None else q_out
+    if R:
+        _need(cos_sin, torch.float32, "cos_sin", 3)
+        if cos_sin.shape[1] != R // 2 or cos_sin.shape[2] != 2 or not cos_sin.is_contiguous():
+            raise KernelError("rope_cache_write_packed: cos_sin must be contiguous [positions, rope_dim/2, 2]")
+    _need_packed(plane, page_stride, page_size, Hkv, D, "rope_cache_write_packed")
+    if min(qkv.shape[0], q.shape[0], positions.shape[0], req_of_token.shape[0]) < n_tokens:
+        raise KernelError(f"rope_cache_write_packed: fewer rows than {n_tokens} tokens")
+    global _work
+    if _profile is not None:
+        _work = (n_tokens * (2 * (2 * Hq + (2 * Hkv if write_kv else 0)) * D + (Hkv * 9 * D // 8 if write_kv else 0)), 0.0)
+    _check(lib().ferrum_rope_cache_write_packed(_ptr(qkv), dtype_code(qkv.dtype), n_tokens, qkv.stride(0), _ptr(q), q.stride(0), _ptr(positions),
+                                                _ptr(req_of_token), _ptr(block_table), block_table.shape[1], _ptr(cos_sin if R else None),
+                                                cos_sin.shape[0] if R else 0, _ptr(plane), c_longlong(page_stride), plane.shape[0], page_size,
+                                                Hq, Hkv, D, R, pairing, 1 if write_kv else 0, _ptr(err), _stream()), "rope_cache_write_packed")
+
+
+def unpack_cache(plane, page_stride, page_size, block_table, items, out, err):
+    """out[i] = the 16-bit keys and values of page items[i, 1] of request items[i, 0] (int32 [n, 2]); out: [>= n, 2, Hkv, page_size, D] of
+    the cache's 16-bit type.  A page that the request does not hold arrives as zeros and raises the error flag."""
+    _need16(out, "out", 5); _need(items, torch.int32, "items", 2); _need_table(block_table, "unpack_cache")
+    Hkv, D = out.shape[2], out.shape[4]
+    _need_packed(plane, page_stride, page_size, Hkv, D, "unpack_cache")
+    n = items.shape[0]
+    if items.shape[1] != 2 or not items.is_contiguous() or out.shape[0] < n or out.shape[1] != 2 or out.shape[3] != page_size or not out.is_contiguous():
+        raise KernelError("unpack_cache: items must be [n, 2] and out contiguous [>= n, 2, Hkv, page_size, D]")
+    global _work
+    if _profile is not None:
+        _work = (n * Hkv * page_size * D * (9 / 8 + 4), 0.0)
+    _check(lib().ferrum_unpack_cache(_ptr(plane), c_longlong(page_stride), plane.shape[0], page_size, _ptr(block_table), block_table.shape[1],
+                                     _ptr(items), n, _ptr(out), dtype_code(out.dtype), Hkv, D, _ptr(err), _stream()), "unpack_cache")
+
+
+def attention_packed_rows():
+    """A request is read by `attention_packed` while its tokens x query heads of a KV head are at most this many in the step."""
+    return int(lib().ferrum_attention_packed_rows())
+
+
+def attention_packed_workspace(D):
+    """float32 elements of the workspace of `attention_packed`."""
+    return int(lib().ferrum_attention_packed_workspace(D))
+
+
+def attention_packed(q, out, n_tokens, block_table, q_start, pos0, plane, page_stride, page_size, Hq, Hkv, D, scale, window, err, part):
+    """Causal grouped-query attention over a cache held in 4 bits, for the requests of the step that bring few rows (decoded tokens, see
+    `attention_packed_rows`); the rows of other requests stay as they are.  q_start (int32 [requests + 1]): first token of
+    each request; pos0 (int32 [requests]): positions cached before the step, whose own keys must be in the pages already.  part:
+    float32 workspace of `attention_packed_workspace(D)` elements; calls that may run at the same time need one each."""
+    _need16(q, "q", 2); _need16(out, "out", 2, like=q); _need(q_start, torch.int32, "q_start", 1); _need(pos0, torch.int32, "pos0", 1)
+    _need_table(block_table, "attention_packed"); _need_packed(plane, page_stride, page_size, Hkv, D, "attention_packed")
+    _need(part, torch.float32, "part", 1)
+    n_reqs = pos0.shape[0]
+    if q_start.shape[0] != n_reqs + 1 or block_table.shape[0] < n_reqs or min(q.shape[0], out.shape[0]) < n_tokens:
+        raise KernelError("attention_packed: q_start, pos0, block_table and the rows do not agree")
+    _check(lib().ferrum_attention_packed(_ptr(q), q.stride(0), _ptr(out), out.stride(0), dtype_code(q.dtype), _ptr(plane), c_longlong(page_stride),
+                                         plane.shape[0], page_size, _ptr(block_table), block_table.shape[1], _ptr(q_start), _ptr(pos0), n_reqs,
+                                         n_tokens, _ptr(part), c_longlong(part.numel()), Hq, Hkv, D, c_float(scale), window, _ptr(err), _stream()),
+           "attention_packed")
+
+
 def swiglu(gu, act, n_tokens, F):
     """act[t, f] = silu(gu[t, f]) * gu[t, F + f]."""
     _need(gu, None, "gu", 2); _need(act, gu.dtype, "act", 2)
@@ -775,6 +866,34 @@ def sample(logits, n_rows, out_ids, err, inv_temperature=None, seeds=None, count
     _check(lib().ferrum_sample(_ptr(logits), logits.stride(0), n_rows, logits.shape[1],
                                _ptr(inv_temperature), _ptr(seeds), _ptr(counters), _ptr(out_ids), _ptr(also_to),
                                _ptr(err), _stream()), "sample")
+
+
+def sample_filtered(logits, n_rows, out_ids, err, temperature, top_k, top_p, min_p, uniform, rows=None, also_to=None):
+    """out_ids[r] = a draw from row r of the logits with the given random number, r = rows[i] (int32) or i itself for i < n_rows.  Per i:
+    temperature (float32; 0: the largest logit), top_k (int32; <= 0: off), top_p (float32 in (0, 1]; 1: off), min_p (float32 up to 1;
+    <= 0: off) and uniform (float64 in [0, 1): a float32's 24 bits could not reach a token rarer than 6e-8).  top_k, top_p and
+    min_p may be None.  The filters work in this order: the top_k largest logits (of equal ones the lower index); of these, by descending logit, those with less than
+    top_p of their mass before them; of these, those with at least min_p times the largest one's probability.  The draw is the first
+    of them in index order at which their running mass exceeds uniform times their whole mass.  NaN logits are never drawn.  A row of NaN
+    raises error 6, a temperature, top_p or min_p out of range error 7 (id -1 each).  `also_to` (int32) receives the ids as well."""
+    _need(logits, torch.float32, "logits", 2); _need(out_ids, torch.int32, "out_ids", 1); _need(err, torch.int32, "err")
+    for t, dt, name in ((temperature, torch.float32, "temperature"), (top_k, torch.int32, "top_k"), (top_p, torch.float32, "top_p"),
+                        (min_p, torch.float32, "min_p"), (uniform, torch.float64, "uniform"), (rows, torch.int32, "rows")):
+        if t is None and name in ("top_k", "top_p", "min_p", "rows"):
+            continue
+        _need(t, dt, name, 1)
+        if t.shape[0] < n_rows or not t.is_contiguous():
+            raise KernelError(f"sample_filtered: {name} must be contiguous with {n_rows} elements")
+    if rows is None and min(logits.shape[0], out_ids.shape[0]) < n_rows:
+        raise KernelError(f"sample_filtered: fewer logits or ids than {n_rows} rows")
+    if also_to is not None:
+        _need(also_to, torch.int32, "also_to", 1)
+    global _work
+    if _profile is not None:
+        _work = (n_rows * logits.shape[1] * 4, 0.0)
+    _check(lib().ferrum_sample_filtered(_ptr(logits), logits.stride(0), n_rows, logits.shape[1], _ptr(rows), _ptr(temperature), _ptr(top_k),
+                                        _ptr(top_p), _ptr(min_p), _ptr(uniform), _ptr(out_ids), _ptr(also_to), _ptr(err), _stream()),
+           "sample_filtered")
 
 
 # ----------------------------------------------------------------------------- parallel gated block

@@ -5,6 +5,11 @@ write, attention of every token over its request's pages, output projection adde
 residual stream (crates/model/src/llama.rs:185-257).  Query head h reads KV head
 h / (Hq/Hkv); the score scale is 1/sqrt(head_dim) unless given.  `window` > 0 keeps the last
 `window` keys only; the reference has no window.
+
+The cache may be held in 4 bits (`set_cache_bits`): the rotary step quantises keys and values on their way into the pages, decoded
+tokens read the packed pages as they are, and the pages that a prompt portion sees are brought back to 16 bits in a scratch
+buffer for the kernels of prompt portions.  Every token reads quantised keys and values, its own portion's included, so a
+prompt's results do not depend on how it is cut.
 """
 from __future__ import annotations
 
@@ -12,6 +17,8 @@ import math
 
 import torch
 
+from ..cache.storage import LayerCache
+from ..errors import ConfigError
 from ..ops import lib as ops
 from . import attention_plan
 from .base import CacheNeed, Mixer, PagedKVNeed, ParamSpec
@@ -36,6 +43,8 @@ class PagedAttention(Mixer):
         head) fit the 16-row tile of the tensor-core kernel, whose padded work list has a shape
         that depends on the number of requests only; larger groups take the 64-row class, whose
         grid follows the context lengths.  The generic kernel has no work lists at all."""
+        if self.cache_bits == 4:
+            return self.Hq // self.Hkv <= ops.attention_packed_rows()
         if not ops.attention_flash_supported(self.dtype, self.D):
             return True
         return self.Hq // self.Hkv <= 16
@@ -49,6 +58,7 @@ class PagedAttention(Mixer):
         self.chunked = False     # True: `window` is a chunk length (a subclass sets it)
         self.keep_first = 0      # with a window: the sequence's first keys that every query sees (a subclass sets it)
         self.score_softcap, self.sink = 0.0, False      # (a subclass may bend the scores and add a sink to the softmax)
+        self.cache_bits = 16 if dtype != torch.float32 else 32
         self.wide_weights = False      # True: the tensor-core kernel keeps the softmax weights to float32 precision (a subclass sets it)
         self.w_q_weight = self.w_k_weight = self.w_v_weight = self.w_output_weight = None
         self.w_qkv = None
@@ -64,28 +74,67 @@ class PagedAttention(Mixer):
         self.w_q_weight = self.w_k_weight = self.w_v_weight = None
 
     def cache_need(self):
-        return CacheNeed(paged=PagedKVNeed(self.Hkv, self.D, self.window))
+        return CacheNeed(paged=PagedKVNeed(self.Hkv, self.D, self.window, packed=self.cache_bits == 4))
+
+    def set_cache_bits(self, bits):
+        """Holds the cache in 4 bits an element, or (the default) in the compute type.  Before the cache's memory is laid out."""
+        if bits == 4 and type(self) is PagedAttention:
+            if not ops.attention_flash_supported(self.dtype, self.D):
+                raise ConfigError(f"a cache in 4 bits needs a 16-bit compute type and heads of 64 or 128 elements, found {self.dtype} and {self.D}")
+        elif bits != 8 * self.dtype.itemsize:
+            return super().set_cache_bits(bits)
+        self.cache_bits = int(bits)
 
     def forward(self, x, ctx, cache, residual, accumulate=True, defer=False):
         T, Hq, Hkv, D = ctx.n_tokens, self.Hq, self.Hkv, self.D
         qw = Hq * D
         qkv = ctx.buf("attn_qkv", (ctx.token_capacity, (Hq + 2 * Hkv) * D), self.dtype)
         w = self.w_qkv if cache.writes else self.w_qkv[:qw]   # a run that reads another run's cache needs q only
-        part = linear_deferred(x, w, ctx, T) if ctx.defer_residuals else None
+        part = linear_deferred(x, w, ctx, T) if ctx.defer_residuals and self.cache_bits != 4 else None
         if part is None:
             linear(x, w, qkv, STORE, ctx, M=T)
         rot = self.position.rotary() if self.position is not None else None
-        table = ctx.block_tables[cache.group]
-        ops.rope_cache_write(qkv, T, ctx.positions, ctx.req_of_token, table,
-                             rot.cos_sin if rot is not None else None, cache.plane, cache.page_stride,
-                             cache.page_size, Hq, Hkv, D, rot.rope_dim if rot is not None else 0,
-                             rot.pairing if rot is not None else 0, cache.writes, ctx.err, partials=part)
+        cos_sin, rope_dim, pairing = (rot.cos_sin, rot.rope_dim, rot.pairing) if rot is not None else (None, 0, 0)
+        where = (ctx.positions, ctx.req_of_token, ctx.block_tables[cache.group], cos_sin, cache.plane, cache.page_stride, cache.page_size)
+        if self.cache_bits == 4:
+            ops.rope_cache_write_packed(qkv, T, *where, Hq, Hkv, D, rope_dim, pairing, ctx.err, write_kv=cache.writes)
+        else:
+            ops.rope_cache_write(qkv, T, *where, Hq, Hkv, D, rope_dim, pairing, cache.writes, ctx.err, partials=part)
         out = ctx.buf("attn_out", (ctx.token_capacity, qw), self.dtype)
-        if ops.attention_flash_supported(self.dtype, D):
+        self.attend(qkv, out, ctx, cache)
+        linear(out, self.w_output_weight, residual, RESIDUAL if accumulate else STORE_F32, ctx, M=T)
+
+    def attend(self, qkv, out, ctx, cache):
+        """out[t] = the attention of the step's token t (qkv's first Hq * D columns, turned already) over its request's pages."""
+        table = ctx.block_tables[cache.group]
+        if self.cache_bits == 4:
+            self._packed(qkv, out, ctx, cache, table)
+        elif ops.attention_flash_supported(self.dtype, self.D):
             self._flash(qkv, out, ctx, cache, table)
         else:
             self._generic(qkv, out, ctx, cache, table)
-        linear(out, self.w_output_weight, residual, RESIDUAL if accumulate else STORE_F32, ctx, M=T)
+
+    def _packed(self, qkv, out, ctx, cache, table):
+        """Over a cache held in 4 bits: decoded tokens from the packed pages; for prompt portions the pages they see are unpacked
+        into a scratch plane, which the kernels of prompt portions then read in the cache's place."""
+        Hq, Hkv, D = self.Hq, self.Hkv, self.D
+        few = ops.attention_packed_rows()
+        rows = [n * (Hq // Hkv) for n in ctx.h_q_len]
+        if min(rows) <= few:
+            part = ctx.buf("attn_packed_part", (ops.attention_packed_workspace(D),), torch.float32)
+            if ops.profiling():      # (a step with prompt portions counts the whole step's work for each kernel)
+                ops.set_work(ops.attention_work(ctx, Hq, Hkv, D, self.window, 9 / 16))
+            ops.attention_packed(qkv, out, ctx.n_tokens, table, ctx.q_start, ctx.pos0, cache.plane, cache.page_stride, cache.page_size,
+                                 Hq, Hkv, D, self.scale, self.window, ctx.err, part)
+        if max(rows) <= few:
+            return
+        items, pages = attention_plan.unpack_plan(ctx, cache.group, Hq // Hkv, self.window, cache.page_size, few)
+        n, whole = items.shape[0], cache.plane.shape[0]
+        plane = ctx.scratch.get("attn_unpacked", (n, 2, Hkv, cache.page_size, D), self.dtype, limit=cache.plane[0].numel() // (18 * D) * 32 * D * whole,
+                                captured=False)
+        ops.unpack_cache(cache.plane, cache.page_stride, cache.page_size, table, items, plane, ctx.err)
+        view = LayerCache(group=cache.group, plane=plane, page_stride=plane.stride(0), page_size=cache.page_size, writes=False, state=None)
+        self._flash(qkv, out, ctx, view, pages, few_rows=False)
 
     def _generic(self, qkv, out, ctx, cache, table, distance_penalty=None, out_scale=1.0):
         """CUDA-core path.  With enough rows to fill the GPU (a prompt portion) every row walks its
@@ -111,7 +160,7 @@ class PagedAttention(Mixer):
     def plan(self, ctx, cache):
         """The step's work lists of the tensor-core kernels for this layer's shape (None on the
         generic path, which has none)."""
-        if not ops.attention_flash_supported(self.dtype, self.D):
+        if not ops.attention_flash_supported(self.dtype, self.D) or self.cache_bits == 4:
             return None
         return self._tensor_core_plans(ctx, cache)
 
@@ -124,12 +173,12 @@ class PagedAttention(Mixer):
                                                                              cache.page_stride)
         return attention_plan.plans_for(ctx, Hq // Hkv, self.window, Hkv, tc_tokens)
 
-    def _flash(self, qkv, out, ctx, cache, table):
+    def _flash(self, qkv, out, ctx, cache, table, few_rows=True):
         """Tensor-core path: one launch per row-tile class of the step's plan, plus a merge
-        launch where key ranges were split."""
+        launch where key ranges were split.  few_rows=False leaves out the class of decoded tokens."""
         Hq, Hkv, D = self.Hq, self.Hkv, self.D
-        for plan in self.plan(ctx, cache):
-            if plan is None:
+        for plan in self._tensor_core_plans(ctx, cache):
+            if plan is None or (plan.bm == 16 and plan.kind == "flash" and not few_rows):
                 continue
             part_o = part_ml = None
             if plan.n_slots:

@@ -295,3 +295,36 @@ def plans_for(ctx, G, window, Hkv, tc_tokens=0) -> List[Optional[ClassPlan]]:
         plans.append(cp)
     ctx.step_cache[cache_key] = plans
     return plans
+
+
+def unpack_plan(ctx, group, G, window, page_size, few_rows):
+    """For a cache held in 4 bits: the pages that the step's prompt portions (requests of more than `few_rows` rows) see, as (int32
+    [n, 2] of (request, page of the request), block table of the plane that they are unpacked into, -1 elsewhere); built on
+    first use in a step and shared by the layers of a shape."""
+    key = ("unpack", group, G, window, page_size)
+    if key in ctx.step_cache:
+        return ctx.step_cache[key]
+    width, R = ctx.block_tables[group].shape[1], ctx.n_reqs
+    lo, hi = np.zeros(R, dtype=np.int64), np.zeros(R, dtype=np.int64)        # the request's pages [lo, hi)
+    for r, (p, n) in enumerate(zip(ctx.h_pos0, ctx.h_q_len)):
+        if n * G > few_rows:
+            lo[r] = max(0, p - window + 1) // page_size if window > 0 else 0
+            hi[r] = (p + n - 1) // page_size + 1
+    held = hi - lo
+    n = int(held.sum())
+    request = np.repeat(np.arange(R), held)
+    page = np.arange(n) - np.repeat(np.cumsum(held) - held, held) + lo[request]
+    table = np.full((R, width), -1, dtype=np.int32)
+    fits = page < width                      # (a page beyond the table is refused on the device)
+    table[request[fits], page[fits]] = np.nonzero(fits)[0]
+    total = 2 * n + R * width
+    ring, dev = ctx.plan_store.buffers(key, total, captured=False)
+    pinned = ring.next()
+    h = pinned.numpy()
+    h[:2 * n:2], h[1:2 * n:2] = request, page
+    h[2 * n:total] = table.reshape(-1)
+    dev[:total].copy_(pinned[:total], non_blocking=True)
+    ring.sent()
+    ctx.h2d_bytes += total * 4
+    ctx.step_cache[key] = dev[:2 * n].view(n, 2), dev[2 * n:total].view(R, width)
+    return ctx.step_cache[key]

@@ -34,6 +34,8 @@ from typing import Dict, Iterator, List, Optional, Tuple
 
 import torch
 
+from ..errors import ConfigError
+
 
 @dataclass(frozen=True)
 class ParamSpec:
@@ -55,12 +57,13 @@ class PagedKVNeed:
     """Keys and values of `n_kv_heads` x `head_dim` per position; `window` 0 keeps all keys.
     `parts` 2: a page holds keys, then values; 1: one row per position and head (a mixer that
     derives keys and values from the same cached row).  `keep_first`: with a window, the first so many
-    positions stay for the whole sequence."""
+    positions stay for the whole sequence.  `packed`: the pages hold 4-bit codes instead of the compute type."""
     n_kv_heads: int
     head_dim: int
     window: int = 0
     parts: int = 2
     keep_first: int = 0
+    packed: bool = False
 
 
 @dataclass(frozen=True)
@@ -125,6 +128,10 @@ class PositionEncoding(Part):
 class Mixer(Part):
     def cache_need(self) -> CacheNeed:
         return CacheNeed()
+
+    def set_cache_bits(self, bits) -> None:
+        """Asks for a cache of `bits` bits an element; a mixer that can hold its pages so overrides this."""
+        raise ConfigError(f"{type(self).__name__} does not hold its cache in {bits} bits")
 
     def plan(self, ctx, cache) -> None:
         """Optional: build what this step's kernels need from the host (work lists, split

@@ -1,3 +1,3 @@
-from .sampler import DeviceSampler
+from .sampler import DeviceSampler, Filters
 
-__all__ = ["DeviceSampler"]
+__all__ = ["DeviceSampler", "Filters"]

@@ -3,16 +3,58 @@
 Greedy is the reference's argmax (crates/core-types/src/model.rs:44-62: lowest index wins a
 tie, NaN is skipped).  With a temperature the kernel draws from softmax(logits / T) by the
 Gumbel-max trick with a counter-based hash keyed by (seed, tokens generated so far,
-vocabulary index): a request's draw does not depend on the batch it shares a step with.  The
-reference's `SamplingParams` (crates/core-types/src/schedule.rs:16-40) also carries `top_p`;
-like the reference this engine accepts only 1.
+vocabulary index): a request's draw does not depend on the batch it shares a step with.  Rows with
+filters (top-k, top-p, which the reference's `SamplingParams` carries and accepts only as 1,
+crates/core-types/src/schedule.rs:16-40, and min-p) are drawn by a kernel of their own from one random number each, a hash of (seed, tokens
+generated so far) again.
 """
 from __future__ import annotations
+
+from dataclasses import dataclass
 
 import numpy as np
 import torch
 
+from ..errors import InvalidRequest
 from ..ops import lib as ops
+
+
+_MASK = (1 << 64) - 1
+
+
+def _mix64(x):
+    """The finaliser of the splitmix64 generator (Steele, Lea and Flood 2014)."""
+    x = (x + 0x9E3779B97F4A7C15) & _MASK
+    x = ((x ^ (x >> 30)) * 0xBF58476D1CE4E5B9) & _MASK
+    x = ((x ^ (x >> 27)) * 0x94D049BB133111EB) & _MASK
+    return x ^ (x >> 31)
+
+
+def uniform(seed, counter):
+    """The random number in [0, 1) of a request's draw number `counter`: 53 bits that depend on (seed, counter) alone."""
+    return (_mix64(_mix64(int(seed) & _MASK) ^ int(counter)) >> 11) * 2.0 ** -53
+
+
+@dataclass(frozen=True)
+class Filters:
+    """What a draw leaves out (in this order; `ops.sample_filtered` has the definition): all but the top_k largest logits (0:
+    off), what lies beyond the top_p part of their mass (1: off), what is less likely than min_p times the likeliest (0: off)."""
+    top_k: int = 0
+    top_p: float = 1.0
+    min_p: float = 0.0
+
+    def __post_init__(self):
+        if isinstance(self.top_k, bool) or int(self.top_k) != self.top_k or not 0 <= self.top_k < 1 << 31:
+            raise InvalidRequest("top_k must be a whole number, 0 (off) or more")
+        # what the kernel gets are float32 numbers: one below 2^-149 would be 0 there
+        if not 0 < float(np.float32(self.top_p)) <= 1:
+            raise InvalidRequest("top_p must be in (0, 1]")
+        if not 0 <= float(np.float32(self.min_p)) <= 1:
+            raise InvalidRequest("min_p must be in [0, 1]")
+
+    @property
+    def on(self):
+        return self.top_k > 0 or self.top_p < 1 or self.min_p > 0
 
 
 class Ticket:
@@ -42,6 +84,8 @@ class DeviceSampler:
         self._inv_t = (PinnedRing(n + 1, torch.float32, device, self.DEPTH), dev(torch.float32))
         self._seeds = (PinnedRing(n + 1, torch.int64, device, self.DEPTH), dev(torch.int64))
         self._counters = (PinnedRing(n + 1, torch.int32, device, self.DEPTH), dev(torch.int32))
+        # rows with filters: uniform (float64), then temperature, top_p, min_p (float32), then row, top_k (int32)
+        self._filtered = (PinnedRing(28 * (n + 1), torch.uint8, device, self.DEPTH), torch.empty(28 * (n + 1), dtype=torch.uint8, device=device))
         self._ids_host = [torch.empty(n + 1, dtype=torch.int32).pin_memory() for _ in range(self.DEPTH)]
         self._events = [torch.cuda.Event() for _ in range(self.DEPTH)]
         self._turn = 0
@@ -52,15 +96,37 @@ class DeviceSampler:
         self.err = self.ids_device[n:n + 1]
         self.d2h_bytes = 0
 
-    def launch(self, logits, rows, also_to=None) -> Ticket:
-        """rows: objects with `temperature`, `seed`, `counter`, one per row of `logits`.  The ids
+    def _launch_filtered(self, logits, rows, filters, picked, also_to):
+        """Draws the rows `picked` (indices) with their filters."""
+        ring, dev = self._filtered
+        m = len(picked)
+        host = ring.next()
+        h = host.numpy()[:28 * m]
+        h[:8 * m].view(np.float64)[:] = [uniform(rows[i].seed, rows[i].counter) for i in picked]
+        f = h[8 * m:20 * m].view(np.float32)
+        f[:m] = [rows[i].temperature for i in picked]
+        f[m:2 * m] = [filters[i].top_p for i in picked]
+        f[2 * m:] = [filters[i].min_p for i in picked]
+        k = h[20 * m:].view(np.int32)
+        k[:m], k[m:] = picked, [filters[i].top_k for i in picked]
+        dev[:28 * m].copy_(host[:28 * m], non_blocking=True)
+        ring.sent()
+        u, f, k = dev[:8 * m].view(torch.float64), dev[8 * m:20 * m].view(torch.float32), dev[20 * m:28 * m].view(torch.int32)
+        ops.sample_filtered(logits, m, self.ids_device, self.err, f[:m], k[m:], f[m:2 * m], f[2 * m:], u, rows=k[:m], also_to=also_to)
+
+    def launch(self, logits, rows, also_to=None, filters=None) -> Ticket:
+        """rows: objects with `temperature`, `seed`, `counter`, one per row of `logits`; filters: `Filters` or None per row
+        (they act on rows with a temperature).  The ids
         and the error flag (`self.err`, which the step's kernels must have been given) travel to
         the host in one copy.  also_to: an int32 device tensor that receives the ids as well."""
         n, err = len(rows), self.err
         if n > self.max_rows:
             raise ValueError(f"{n} rows to sample, the sampler was made for {self.max_rows}")
         ids_d = self.ids_device
-        if any(r.temperature > 0 for r in rows):
+        picked = [i for i, (r, f) in enumerate(zip(rows, filters)) if f is not None and f.on and r.temperature > 0] if filters else []
+        if len(picked) == n and n:
+            pass                       # no row is left for the kernel of plain draws
+        elif any(r.temperature > 0 for r in rows):
             (it_r, it_d), (sd_r, sd_d), (ct_r, ct_d) = self._inv_t, self._seeds, self._counters
             it_h, sd_h, ct_h = it_r.next(), sd_r.next(), ct_r.next()
             for i, r in enumerate(rows):
@@ -73,6 +139,8 @@ class DeviceSampler:
             ops.sample(logits, n, ids_d, err, it_d[:n], sd_d[:n], ct_d[:n], also_to=also_to)
         else:
             ops.sample(logits, n, ids_d, err, also_to=also_to)
+        if picked:
+            self._launch_filtered(logits, rows, filters, picked, also_to)
         self._turn = (self._turn + 1) % self.DEPTH
         host, event = self._ids_host[self._turn], self._events[self._turn]
         host.copy_(ids_d, non_blocking=True)
@@ -88,6 +156,6 @@ class DeviceSampler:
         out = ticket.host.tolist()
         return out[:ticket.n], out[-1]
 
-    def sample(self, logits, rows):
+    def sample(self, logits, rows, filters=None):
         """launch + collect."""
-        return self.collect(self.launch(logits, rows))
+        return self.collect(self.launch(logits, rows, filters=filters))
