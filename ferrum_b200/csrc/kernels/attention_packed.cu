@@ -2,11 +2,31 @@
 //   o = sum_j p_j v_j,  p = softmax_j(scale * q . k_j),  over the keys j of the request up to the token itself, the last `window` of them
 // where a window is set.
 //
-// Simplest form: a block per (request, KV head) walks its rows one after the other; its four warps take every fourth key, a lane holds
-// D / 32 elements, the softmax runs with the data, and the warps' (maximum, sum, values) meet at the end.
+// What bounds it is the cache's bytes, 9 D / 8 a position and KV head, as long as a position's codes become matrix operands in few
+// instructions.  So the codes themselves are the operands, exactly, and steps and middles join on either side of the products:
+//   a nibble c in a 16-bit half is the subnormal float16 c * 2^-24, one position higher 16 c * 2^-24: two elements by one AND, every
+//   other pair by one shift more;
+//   scores       s = scale * sum_g (step_g * (q . c)_g + (middle_g - 8 step_g) * (sum of q)_g), g the groups of 64 elements: keys are the rows
+//                of the product (m16n8k16), the packed rows (tokens x query heads of the KV head) its columns;
+//   values       o = sum_j (p_j step_j) (c_j - 8) + p_j middle_j: elements are the rows, keys the contraction; the codes less 8 by one
+//                subtraction (exact), so that the sums do not cancel; the middles' sum on the CUDA cores in float32.
+// Roundings: q, a power of two times itself that puts a row's largest element at 2^14 to 2^15, is a float16 (exactly, from bfloat16 also, but for what is
+// 2^-30 below the largest); p step, times a power of two that follows the largest step seen, is rounded to float16: a weight's half
+// step of 2^-12, and the result's own.  All sums are float32.
+//
+// The work is handed out on the device: all (request, KV head, rows of 8 NT, 64 keys) units form one line, and CTA c of P takes the units
+// [c U / P, (c + 1) U / P): the launch does not depend on the lengths, so that a captured one serves any.  A CTA's four warps take every
+// fourth block of 16 positions; a block is one bulk copy into the warp's own ring of stages, and no warp waits for another until
+// its part of a (request, head) is done.  Parts of a (request, head) cut between CTAs meet in a second launch, in a fixed order.
 #include "packed_cache.cuh"
+#include "ptx_sm100.cuh"
 
 namespace {
+
+constexpr int WARPS = 4;
+constexpr int TILE = WARPS * PACKED_POS;     // keys of a unit
+constexpr int STAGES = 4;                    // blocks in a warp's ring
+constexpr int PART_ROWS = 16;                // rows of a partial's slot
 
 struct PackedParams {
   const void* q;
@@ -15,92 +35,653 @@ struct PackedParams {
   const int* block_table;
   const int* q_start;
   const int* pos0;
+  float* part_o;        // [2 P][PART_ROWS][D]
+  float* part_ml;       // [2 P][PART_ROWS][2]
+  int2* part_info;      // [requests * Hkv * 2]: first slot's CTA, number of CTAs that share the rows
   int* err;
   long long page_stride;
-  int ldq, ldo, n_pages, page_size, table_width, Hq, Hkv, window;
-  float scale;
+  int ldq, ldo, n_pages, page_size, table_width, Hq, Hkv, G, window, n_reqs;
+  float scale_log2;
 };
 
-template <typename T, int D>
-__global__ void __launch_bounds__(128)
-attention_packed_kernel(const PackedParams p) {
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ unsigned transpose8(unsigned v) {
+  unsigned r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ unsigned less(unsigned a, unsigned b) {       // a - b, two float16 each
+  const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const unsigned*>(&r);
+}
+template <typename T> __device__ __forceinline__ float2 pair_values(unsigned v);
+template <> __device__ __forceinline__ float2 pair_values<__nv_bfloat16>(unsigned v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)); }
+template <> __device__ __forceinline__ float2 pair_values<__half>(unsigned v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
+
+// Waits for a copy, about a second at most (a moment once one has failed to come).
+__device__ __forceinline__ bool arrived(uint32_t bar, uint32_t parity, bool failed) {
+  if (sm100::mbar_try_wait(bar, parity)) return true;
+  const long long begin = clock64(), limit = failed ? 1000000 : sm100::WAIT_LIMIT_CYCLES;
+  while (clock64() - begin <= limit)
+    if (sm100::mbar_try_wait(bar, parity)) return true;
+  return false;
+}
+
+// CTAs that an SM holds, as the registers of the accumulators allow.
+template <int D, int NT>
+constexpr int RESIDENT = NT == 1 ? 4 : D == 64 ? 3 : 2;
+constexpr int MAX_RESIDENT = 4;
+
+// A request's part of the line.
+struct Span {
+  int lo, tiles, row_tiles;      // first key (a block's first), tiles of TILE keys, tiles of rows; none of either: not a request of few rows
+};
+template <int NT>
+__device__ __forceinline__ Span span_of(const PackedParams& p, int r) {
+  const int n = p.q_start[r + 1] - p.q_start[r], rows = n * p.G;
+  if (rows <= 0 || rows > PACKED_FEW_ROWS) return Span{0, 0, 0};
+  const int pos = p.pos0[r];
+  const int lo = (p.window > 0 ? max(0, pos - p.window + 1) : 0) / PACKED_POS * PACKED_POS;
+  return Span{lo, (pos + n - lo + TILE - 1) / TILE, (rows + 8 * NT - 1) / (8 * NT)};
+}
+
+// One CTA's share of the units of (request r, KV head kvh, row tile rt): tiles [t0, t1).  slot < 0: that is all of them, the result
+// is written; otherwise the partial goes to the slot.
+template <typename T, int D, int NT, int NB>
+__device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kvh, int rt, int key_lo, int t0, int t1, int slot, uint8_t* ring,
+                                            uint32_t bars, uint32_t& phases, float* merge, bool& failed) {
   using B = PackedBlock<D>;
-  constexpr int E = D / 32;
-  __shared__ float s_ml[4][2], s_o[4][D];
-  pdl_launch();
-  pdl_wait();
-  const int req = blockIdx.x, kvh = blockIdx.y, G = p.Hq / p.Hkv;
-  const int qs = p.q_start[req], n = p.q_start[req + 1] - qs;
-  if (n * G > PACKED_FEW_ROWS) return;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, pos0 = p.pos0[req];
-  for (int r = 0; r < n * G; ++r) {
-    const int token = qs + r / G, head = kvh * G + r % G, at = pos0 + r / G;
-    const T* q = (const T*)p.q + (size_t)token * p.ldq + (size_t)head * D + lane * E;
-    float x[E], o[E], m = -INFINITY, l = 0.f;
-    for (int e = 0; e < E; ++e) x[e] = to_f32<T>(q[e]) * p.scale, o[e] = 0.f;
-    for (int key = max(0, p.window > 0 ? at - p.window + 1 : 0) + warp; key <= at; key += 4) {
-      const int lp = key / p.page_size, in_page = key % p.page_size, row = in_page % PACKED_POS;
-      const int page = lp < p.table_width ? p.block_table[(size_t)req * p.table_width + lp] : -1;
-      if (page < 0 || page >= p.n_pages) {
-        if (lane == 0) atomicExch(p.err, 5);
-        continue;
+  constexpr int GN = B::GROUPS;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tig = lane & 3;
+  const int qs = p.q_start[r], n_rows = (p.q_start[r + 1] - qs) * p.G, pos0 = p.pos0[r];
+  const int row0 = rt * 8 * NT;
+  const int hi = pos0 + p.q_start[r + 1] - qs;                       // one past the last key
+  const int b_end = min((hi - key_lo + PACKED_POS - 1) / PACKED_POS, t1 * WARPS);
+  const int b0 = t0 * WARPS + warp;                                   // the warp's blocks: b0, b0 + WARPS, ... below b_end
+  const int n_blocks = b0 < b_end ? (b_end - b0 + WARPS - 1) / WARPS : 0;
+  const int* bt = p.block_table + (size_t)r * p.table_width;
+  const uint8_t* head = p.plane + (size_t)kvh * (p.page_size / PACKED_POS) * B::BYTES;
+
+  // ---- the pages of the warp's next 32 blocks, one a lane; the copies of the first STAGES
+  int my_page = -1, my_in_page = 0;
+  auto fetch_pages = [&](int i) {      // for blocks i .. i + 31 of the warp
+    const int k = i + lane;
+    my_page = -1;
+    if (k < n_blocks) {
+      const int key = key_lo + (b0 + k * WARPS) * PACKED_POS, lp = key / p.page_size;
+      my_in_page = (key - lp * p.page_size) / PACKED_POS;
+      my_page = lp < p.table_width ? bt[lp] : -1;
+      if (my_page < 0 || my_page >= p.n_pages) {
+        my_page = -1;
+        atomicExch(p.err, 5);
       }
-      const uint8_t* block = p.plane + (size_t)page * p.page_stride + ((size_t)kvh * (p.page_size / PACKED_POS) + in_page / PACKED_POS) * B::BYTES;
-      const T* kp = (const T*)(block + B::K_PAIRS) + (row * B::GROUPS + lane * E / PACKED_GROUP) * 2;
-      const T* vp = (const T*)(block + B::V_PAIRS) + (row * B::GROUPS + lane * E / PACKED_GROUP) * 2;
-      const uint8_t* kc = block + row * B::ROW + lane * (E / 2);
-      float dot = 0.f;
-      for (int e = 0; e < E; ++e) dot += x[e] * (to_f32<T>(kp[1]) + to_f32<T>(kp[0]) * (float)((kc[e / 2] >> (4 * (e & 1)) & 15) - 8));
-      dot = warp_sum(dot);
-      const float m_new = fmaxf(m, dot), keep = m == -INFINITY ? 0.f : expf(m - m_new), w = expf(dot - m_new);
-      l = l * keep + w;
-      for (int e = 0; e < E; ++e)
-        o[e] = o[e] * keep + w * (to_f32<T>(vp[1]) + to_f32<T>(vp[0]) * (float)((kc[B::V_CODES + e / 2] >> (4 * (e & 1)) & 15) - 8));
-      m = m_new;
     }
-    if (lane == 0) s_ml[warp][0] = m, s_ml[warp][1] = l;
-    for (int e = 0; e < E; ++e) s_o[warp][lane * E + e] = o[e];
-    __syncthreads();
-    if (warp == 0) {
-      float M = -INFINITY, L = 0.f, acc[E] = {};
-      for (int w = 0; w < 4; ++w) M = fmaxf(M, s_ml[w][0]);
-      for (int w = 0; w < 4; ++w) {
-        const float f = s_ml[w][0] == -INFINITY ? 0.f : expf(s_ml[w][0] - M);
-        L += s_ml[w][1] * f;
-        for (int e = 0; e < E; ++e) acc[e] += s_o[w][lane * E + e] * f;
+  };
+  unsigned missing = 0;                // per stage: its block has no page
+  auto request_block = [&](int i) {    // copies block i of the warp into its stage; called by the whole warp
+    const int s = i % STAGES;
+    const int page = __shfl_sync(0xffffffffu, my_page, i & 31), in_page = __shfl_sync(0xffffffffu, my_in_page, i & 31);
+    missing = (missing & ~(1u << s)) | ((page < 0 ? 1u : 0u) << s);
+    if (page >= 0 && lane == 0) {
+      sm100::mbar_expect_tx(bars + 8 * s, B::BYTES);
+      bulk_load(sm100::smem_u32(ring + s * B::BYTES), head + (size_t)page * p.page_stride + (size_t)in_page * B::BYTES, B::BYTES, bars + 8 * s);
+    }
+  };
+  int asked = 0;
+  fetch_pages(0);
+  for (; asked < min(STAGES, n_blocks); ++asked) request_block(asked);
+
+  // ---- the rows' queries as float16 operands, their sums per group and their scale
+  unsigned qf[NT][GN][4][2];
+  float q_sum[NT][GN][2], f_row[NT][2];
+  int row_pos[NT][2], row_lo[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int row = row0 + nt * 8 + gid;
+    float x[GN][16], big = 0.f;
+#pragma unroll
+    for (int g = 0; g < GN; ++g) {
+      uint4 raw[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+      if (row < n_rows) {
+        const uint4* src = reinterpret_cast<const uint4*>((const T*)p.q + (size_t)(qs + row / p.G) * p.ldq + (size_t)(kvh * p.G + row % p.G) * D + g * PACKED_GROUP + tig * 16);
+        raw[0] = src[0];
+        raw[1] = src[1];
       }
-      for (int e = 0; e < E; ++e) ((T*)p.out)[(size_t)token * p.ldo + (size_t)head * D + lane * E + e] = from_f32<T>(L > 0.f ? acc[e] / L : 0.f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float2 v = pair_values<T>(reinterpret_cast<const unsigned*>(raw)[i]);
+        x[g][2 * i] = v.x;
+        x[g][2 * i + 1] = v.y;
+        big = fmaxf(big, fmaxf(fabsf(v.x), fabsf(v.y)));
+      }
+    }
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+    // 2^e brings the largest element to [2^14, 2^15); a row of zeros (or of subnormals) keeps e within a float's exponents
+    const int e = max(-100, min(100, 14 + 127 - (int)(__float_as_uint(big) >> 23)));
+    const float up = __uint_as_float((unsigned)(127 + e) << 23);
+    float sum[GN];
+#pragma unroll
+    for (int g = 0; g < GN; ++g) {
+      sum[g] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        x[g][i] = __half2float(__float2half_rn(x[g][i] * up));
+        sum[g] += x[g][i];
+      }
+      sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 1);
+      sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 2);
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {      // step 2 j + h of the contraction: nibbles 2 h and 2 h + 4, then 2 h + 1 and 2 h + 5 (16 times as large)
+          qf[nt][g][2 * j + h][0] = pack2<__half>(x[g][8 * j + 2 * h], x[g][8 * j + 2 * h + 4]);
+          qf[nt][g][2 * j + h][1] = pack2<__half>(x[g][8 * j + 2 * h + 1] * 0.0625f, x[g][8 * j + 2 * h + 5] * 0.0625f);
+        }
+    }
+    // the scores' columns: this thread meets rows 2 tig and 2 tig + 1
+    const float f = p.scale_log2 * __uint_as_float((unsigned)(127 - e) << 23) * 16777216.f;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int from = (2 * tig + c) * 4;
+      f_row[nt][c] = __shfl_sync(0xffffffffu, f, from);
+#pragma unroll
+      for (int g = 0; g < GN; ++g) q_sum[nt][g][c] = __shfl_sync(0xffffffffu, sum[g], from) * 0x1p-24f;
+      row_pos[nt][c] = pos0 + (row0 + nt * 8 + 2 * tig + c) / p.G;
+      row_lo[nt][c] = p.window > 0 ? max(0, row_pos[nt][c] - p.window + 1) : 0;
+    }
+  }
+  // keys that every row sees: from the last row's window on, up to the first row's position
+  const int all_hi = pos0 + row0 / p.G, all_lo = p.window > 0 ? max(0, pos0 + (min(n_rows, row0 + 8 * NT) - 1) / p.G - p.window + 1) : 0;
+
+  float m_run[NT][2], l_run[NT][2], mid_acc[NT][GN][2], o[NT][GN][4][4];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      m_run[nt][c] = -INFINITY;
+      l_run[nt][c] = 0.f;
+#pragma unroll
+      for (int g = 0; g < GN; ++g) {
+        mid_acc[nt][g][c] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[nt][g][j][c] = o[nt][g][j][2 + c] = 0.f;
+      }
+    }
+  float step_limit = 0x1p-100f, v_up = 0x1p114f;       // the largest step seen is at most step_limit = 2^14 / v_up
+
+  for (int i = 0; i < n_blocks; i += NB) {
+    const uint8_t* block[NB];
+    bool have[NB];
+    int key0[NB];
+    bool whole = true;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const int s = (i + b) % STAGES;
+      block[b] = ring + s * B::BYTES;
+      have[b] = i + b < n_blocks && !(missing >> s & 1);
+      key0[b] = key_lo + (b0 + (i + b) * WARPS) * PACKED_POS;
+      if (have[b]) {
+        failed = __any_sync(0xffffffffu, !arrived(bars + 8 * s, phases >> s & 1, failed) || failed);
+        phases ^= 1u << s;
+      }
+      whole &= have[b] && key0[b] + PACKED_POS - 1 <= all_hi && key0[b] >= all_lo;
+    }
+    // ---- scores
+    float s[NB][NT][4];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      float part[NT][GN][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int g = 0; g < GN; ++g)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) part[nt][g][e] = 0.f;
+#pragma unroll
+      for (int g = 0; g < GN; ++g) {
+        const uint2 u = *reinterpret_cast<const uint2*>(block[b] + gid * B::ROW + g * 32 + tig * 8);
+        const uint2 v = *reinterpret_cast<const uint2*>(block[b] + (gid + 8) * B::ROW + g * 32 + tig * 8);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          unsigned wu = j ? u.y : u.x, wv = j ? v.y : v.x;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              mma_f16(part[nt][g], wu & 0x000F000Fu, wv & 0x000F000Fu, wu & 0x00F000F0u, wv & 0x00F000F0u, qf[nt][g][2 * j + h][0], qf[nt][g][2 * j + h][1]);
+            wu >>= 8;
+            wv >>= 8;
+          }
+        }
+      }
+      float step[GN][2], mid[GN][2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int g = 0; g < GN; ++g) {
+          const float2 v = pair_values<T>(reinterpret_cast<const unsigned*>(block[b] + B::K_PAIRS)[(gid + 8 * k) * GN + g]);
+          step[g][k] = v.x;
+          mid[g][k] = fmaf(-8.f, v.x, v.y);
+        }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float t = 0.f;
+#pragma unroll
+          for (int g = 0; g < GN; ++g) t = fmaf(step[g][e >> 1], part[nt][g][e], fmaf(mid[g][e >> 1], q_sum[nt][g][e & 1], t));
+          s[b][nt][e] = t * f_row[nt][e & 1];
+        }
+      if (!whole) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int key = key0[b] + gid + 8 * (e >> 1);
+            if (!have[b] || key > row_pos[nt][e & 1] || key < row_lo[nt][e & 1] || key >= hi) s[b][nt][e] = -INFINITY;
+          }
+      }
+    }
+    // ---- the running maximum and sum
+    bool moved = false;
+    float corr[NT][2], m_use[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float mx = fmaxf(s[0][nt][c], s[0][nt][2 + c]);
+#pragma unroll
+        for (int b = 1; b < NB; ++b) mx = fmaxf(mx, fmaxf(s[b][nt][c], s[b][nt][2 + c]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        const float m_new = fmaxf(m_run[nt][c], mx);
+        m_use[nt][c] = m_new == -INFINITY ? 0.f : m_new;
+        corr[nt][c] = exp2f(m_run[nt][c] - m_use[nt][c]);
+        moved |= m_new != m_run[nt][c];
+        m_run[nt][c] = m_new;
+      }
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          l_run[nt][c] *= corr[nt][c];
+#pragma unroll
+          for (int g = 0; g < GN; ++g) {
+            mid_acc[nt][g][c] *= corr[nt][c];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              o[nt][g][j][c] *= corr[nt][c];
+              o[nt][g][j][2 + c] *= corr[nt][c];
+            }
+          }
+        }
+    }
+    // ---- values
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      float step[GN][2], mid[GN][2], most = 0.f;
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int g = 0; g < GN; ++g) {
+          float2 v = pair_values<T>(reinterpret_cast<const unsigned*>(block[b] + B::V_PAIRS)[(gid + 8 * k) * GN + g]);
+          if (!whole && (!have[b] || key0[b] + gid + 8 * k >= hi)) v = make_float2(0.f, 0.f);      // (what lies behind the last key may be a NaN)
+          step[g][k] = v.x;
+          mid[g][k] = v.y;
+          most = fmaxf(most, v.x);
+        }
+      if (__any_sync(0xffffffffu, most > step_limit)) {
+        const unsigned top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
+        const int e = min(127, (int)(top >> 23) - 126);              // top < 2^e
+        const float up = __uint_as_float((unsigned)(127 + 14 - e) << 23), ratio = up / v_up;
+        step_limit = __uint_as_float(min((unsigned)(127 + e), 254u) << 23);
+        v_up = up;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int g = 0; g < GN; ++g)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) o[nt][g][j][c] *= ratio;
+      }
+      unsigned pf[NT][GN][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          w[e] = exp2f(s[b][nt][e] - m_use[nt][e & 1]);
+          l_run[nt][e & 1] += w[e];
+        }
+#pragma unroll
+        for (int g = 0; g < GN; ++g) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float up = step[g][k] * v_up;
+            float x0 = w[2 * k] * up, x1 = w[2 * k + 1] * up;
+            float y0 = w[2 * k] * mid[g][k], y1 = w[2 * k + 1] * mid[g][k];
+            if (!whole) {              // a key that a row does not see counts for nothing, whatever it holds
+              if (w[2 * k] == 0.f) x0 = y0 = 0.f;
+              if (w[2 * k + 1] == 0.f) x1 = y1 = 0.f;
+            }
+            mid_acc[nt][g][0] += y0;
+            mid_acc[nt][g][1] += y1;
+            pf[nt][g][k] = transpose8(pack2<__half>(x0, x1));
+          }
+        }
+      }
+      // keys of the contraction: index 2 tig + i of the first half is row tig * 2 + i of the block, of the second half 8 more
+#pragma unroll
+      for (int g = 0; g < GN; ++g) {
+        unsigned w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          w[k] = *reinterpret_cast<const unsigned*>(block[b] + B::V_CODES + (2 * tig + (k & 1) + 8 * (k >> 1)) * B::ROW + g * 32 + gid * 4);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          unsigned x = __byte_perm(w[0], w[1], half ? 0x7632 : 0x5410), y = __byte_perm(w[2], w[3], half ? 0x7632 : 0x5410);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const unsigned a0 = less(x & 0x000F000Fu, 0x00080008u), a1 = less(x & 0x00F000F0u, 0x00800080u);
+            const unsigned a2 = less(y & 0x000F000Fu, 0x00080008u), a3 = less(y & 0x00F000F0u, 0x00800080u);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][g][2 * half + h], a0, a1, a2, a3, pf[nt][g][0], pf[nt][g][1]);
+            x >>= 8;
+            y >>= 8;
+          }
+        }
+      }
+    }
+    // ---- the stages are free: the next blocks
+    __syncwarp();
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+      if (asked < n_blocks && !failed) {
+        if ((asked & 31) == 0) fetch_pages(asked);
+        request_block(asked++);
+      } else if (asked < n_blocks) {
+        missing |= 1u << (asked++ % STAGES);
+      }
+  }
+  if (failed && lane == 0) atomicExch(p.err, 29);
+
+  // ---- the warps' parts meet, eight rows at a time
+  const float down = 1.f / v_up;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) {
+        l_run[nt][c] += __shfl_xor_sync(0xffffffffu, l_run[nt][c], d);
+#pragma unroll
+        for (int g = 0; g < GN; ++g) mid_acc[nt][g][c] += __shfl_xor_sync(0xffffffffu, mid_acc[nt][g][c], d);
+      }
+    }
+    float* ml = merge + WARPS * 8 * D;
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int row = 2 * tig + c;
+      if (gid == 0) {
+        ml[(warp * 8 + row) * 2] = m_run[nt][c];
+        ml[(warp * 8 + row) * 2 + 1] = l_run[nt][c];
+      }
+#pragma unroll
+      for (int g = 0; g < GN; ++g)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {      // tile j of the group: elements 8 gid + 2 j and, 16 times as large, 8 gid + 2 j + 1
+          float2 v = make_float2(fmaf(o[nt][g][j][c] * 0x1p24f, down, mid_acc[nt][g][c]), fmaf(o[nt][g][j][2 + c] * 0x1p20f, down, mid_acc[nt][g][c]));
+          *reinterpret_cast<float2*>(merge + (warp * 8 + row) * D + g * PACKED_GROUP + 8 * gid + 2 * j) = v;
+        }
     }
     __syncthreads();
+    for (int idx = tid; idx < 8 * (D / 4); idx += WARPS * 32) {
+      const int rr = idx / (D / 4), d = idx % (D / 4) * 4, row = row0 + nt * 8 + rr;
+      if (row >= n_rows) continue;
+      float M = -INFINITY, L = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) M = fmaxf(M, ml[(w * 8 + rr) * 2]);
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        const float mw = ml[(w * 8 + rr) * 2], f = mw == -INFINITY ? 0.f : exp2f(mw - M);
+        const float4 v = *reinterpret_cast<const float4*>(merge + (w * 8 + rr) * D + d);
+        L += ml[(w * 8 + rr) * 2 + 1] * f;
+        acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
+      }
+      if (slot < 0) {
+        const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
+        uint2 r2;
+        r2.x = pack2<T>(acc.x * inv, acc.y * inv);
+        r2.y = pack2<T>(acc.z * inv, acc.w * inv);
+        *reinterpret_cast<uint2*>((T*)p.out + (size_t)(qs + row / p.G) * p.ldo + (size_t)(kvh * p.G + row % p.G) * D + d) = r2;
+      } else {
+        const size_t at = (size_t)slot * PART_ROWS + nt * 8 + rr;
+        *reinterpret_cast<float4*>(p.part_o + at * D + d) = acc;
+        if (d == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(M, L);
+      }
+    }
   }
 }
+
+template <typename T, int D, int NT, int NB>
+__global__ void __launch_bounds__(WARPS * 32, RESIDENT<D, NT>)
+attention_packed_kernel(const PackedParams p) {
+  using B = PackedBlock<D>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ __align__(8) unsigned long long bars_mem[WARPS * STAGES];
+  __shared__ long long s_scan[WARPS], s_start;
+  __shared__ int s_req;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint8_t* ring = smem + warp * STAGES * B::BYTES;
+  float* merge = reinterpret_cast<float*>(smem + WARPS * STAGES * B::BYTES);
+  const uint32_t bars = sm100::smem_u32(bars_mem + warp * STAGES);
+  if (lane == 0)
+    for (int s = 0; s < STAGES; ++s) sm100::mbar_init(bars + 8 * s, 1);
+  sm100::fence_barrier_init();
+  sm100::fence_proxy_async();
+  pdl_launch();
+  pdl_wait();
+  // ---- the line's length, then the request in which the CTA's share begins
+  long long U = 0;
+  for (int base = 0; base < p.n_reqs; base += WARPS * 32) {
+    const int r = base + tid;
+    const Span sp = r < p.n_reqs ? span_of<NT>(p, r) : Span{0, 0, 0};
+    long long u = (long long)sp.tiles * sp.row_tiles * p.Hkv;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) u += __shfl_xor_sync(0xffffffffu, u, d);
+    __syncthreads();
+    if (lane == 0) s_scan[warp] = u;
+    __syncthreads();
+    for (int w = 0; w < WARPS; ++w) U += s_scan[w];
+  }
+  const long long P = min((long long)gridDim.x, U);
+  const long long c = blockIdx.x;
+  if (c >= P) return;
+  const long long first = c * U / P, last = (c + 1) * U / P;
+  long long before = 0;
+  for (int base = 0; base < p.n_reqs; base += WARPS * 32) {
+    const int r = base + tid;
+    const Span sp = r < p.n_reqs ? span_of<NT>(p, r) : Span{0, 0, 0};
+    const long long mine = (long long)sp.tiles * sp.row_tiles * p.Hkv;
+    long long u = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, u, d);
+      if (lane >= d) u += v;
+    }
+    __syncthreads();
+    if (lane == 31) s_scan[warp] = u;
+    __syncthreads();
+    long long at = before + u - mine;
+    for (int w = 0; w < WARPS; ++w) {
+      if (w < warp) at += s_scan[w];
+      before += s_scan[w];
+    }
+    if (first >= at && first < at + mine) {
+      s_req = r;
+      s_start = at;
+    }
+    if (before > first) break;
+  }
+  __syncthreads();
+  // ---- walk the share
+  uint32_t phases = 0;
+  bool failed = false;
+  long long u = first, start = s_start;
+  for (int r = s_req; u < last; ++r) {
+    const Span sp = span_of<NT>(p, r);
+    const long long all = (long long)sp.tiles * sp.row_tiles * p.Hkv;
+    while (u < last && u < start + all) {
+      const int pair = (int)((u - start) / sp.tiles), t0 = (int)((u - start) % sp.tiles);
+      const long long pair_start = start + (long long)pair * sp.tiles, pair_end = pair_start + sp.tiles;
+      const int t1 = (int)(min(pair_end, last) - pair_start);
+      const int kvh = pair / sp.row_tiles, rt = pair % sp.row_tiles;
+      const bool split = t0 > 0 || t1 < sp.tiles;
+      if (tid == 0 && t0 == 0) {
+        // the CTA of the pair's last unit: the largest k with k U / P <= pair_end - 1
+        const int k = (int)((pair_end * P - 1) / U);
+        p.part_info[((size_t)r * p.Hkv + kvh) * 2 + rt] = make_int2((int)c * 2 + (u == first ? 0 : 1), k - (int)c + 1);
+      }
+      packed_item<T, D, NT, NB>(p, r, kvh, rt, sp.lo, t0, t1, split ? (int)c * 2 + (u == first ? 0 : 1) : -1, ring, bars, phases, merge, failed);
+      u = pair_start + t1;
+    }
+    start += all;
+  }
+}
+
+// A block per (request, KV head); its 16 warps share the rows and, with fewer rows, the parts of a row.
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(512)
+packed_merge_kernel(const PackedParams p) {
+  constexpr int E = D / 32;
+  __shared__ float s_acc[16][D];
+  __shared__ float2 s_ml[16];
+  pdl_launch();
+  const int r = blockIdx.x, kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_wait();
+  const int qs = p.q_start[r], rows = (p.q_start[r + 1] - qs) * p.G;
+  if (rows <= 0 || rows > PACKED_FEW_ROWS) return;
+  const int share = 16 / rows, row = warp % rows, k = warp / rows;      // warps of a row; warps beyond share * rows have none
+  const int2 info = p.part_info[((size_t)r * p.Hkv + kvh) * 2 + row / (8 * NT)];
+  if (rows <= 8 * NT ? info.y <= 1 : (info.y <= 1 && p.part_info[((size_t)r * p.Hkv + kvh) * 2 + 1 - row / (8 * NT)].y <= 1)) return;
+  float M = -INFINITY, L = 0.f, acc[E] = {};
+  if (k < share && info.y > 1) {
+    constexpr int GROUP = 8;      // parts whose loads are in flight together
+    for (int s0 = k * GROUP; s0 < info.y; s0 += share * GROUP) {
+      float m[GROUP], l[GROUP], v[GROUP][E];
+#pragma unroll
+      for (int i = 0; i < GROUP; ++i) {
+        const bool have = s0 + i < info.y;
+        // the first CTA's slot, then the first of each CTA that follows
+        const size_t at = (size_t)(s0 + i == 0 || !have ? info.x : (info.x / 2 + s0 + i) * 2) * PART_ROWS + row % (8 * NT);
+        m[i] = have ? __ldcg(p.part_ml + at * 2) : -INFINITY;
+        l[i] = have ? __ldcg(p.part_ml + at * 2 + 1) : 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[i][e] = __ldcg(p.part_o + at * D + lane * E + e);
+      }
+      float m_new = M;
+#pragma unroll
+      for (int i = 0; i < GROUP; ++i) m_new = fmaxf(m_new, m[i]);
+      const float keep = M == -INFINITY ? 0.f : exp2f(M - m_new);
+      L *= keep;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] *= keep;
+#pragma unroll
+      for (int i = 0; i < GROUP; ++i) {
+        const float f = m[i] == -INFINITY ? 0.f : exp2f(m[i] - m_new);
+        L += l[i] * f;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (s0 + i < info.y) acc[e] += v[i][e] * f;
+      }
+      M = m_new;
+    }
+  }
+  s_ml[warp] = make_float2(M, L);
+#pragma unroll
+  for (int e = 0; e < E; ++e) s_acc[warp][lane * E + e] = acc[e];
+  __syncthreads();
+  if (k != 0 || info.y <= 1) return;
+  float top = -INFINITY, sum = 0.f, out[E] = {};
+  for (int i = 0; i < share; ++i) top = fmaxf(top, s_ml[row + i * rows].x);
+  for (int i = 0; i < share; ++i) {
+    const float2 ml = s_ml[row + i * rows];
+    const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - top);
+    sum += ml.y * f;
+    for (int e = 0; e < E; ++e) out[e] += s_acc[row + i * rows][lane * E + e] * f;
+  }
+  const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+  T* dst = (T*)p.out + (size_t)(qs + row / p.G) * p.ldo + (size_t)(kvh * p.G + row % p.G) * D + lane * E;
+#pragma unroll
+  for (int e = 0; e < E; e += 2) reinterpret_cast<unsigned*>(dst)[e / 2] = pack2<T>(out[e] * inv, out[e + 1] * inv);
+}
+
+template <typename T, int D, int NT, int NB>
+int launch_packed(const PackedParams& p, cudaStream_t stream) {
+  constexpr int smem = WARPS * STAGES * PackedBlock<D>::BYTES + WARPS * 8 * (D + 2) * 4;
+  static bool configured = false;
+  if (!configured) {
+    cudaError_t e = cudaFuncSetAttribute(attention_packed_kernel<T, D, NT, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    FERRUM_CHECK_ARG(e == cudaSuccess, "attention_packed: cannot reserve %d bytes of shared memory: %s", smem, cudaGetErrorString(e));
+    configured = true;
+  }
+  launch_kernel(attention_packed_kernel<T, D, NT, NB>, dim3(RESIDENT<D, NT> * ferrum_sm_count()), dim3(WARPS * 32), smem, stream, p);
+  FERRUM_CHECK_LAUNCH("attention_packed");
+  launch_kernel(packed_merge_kernel<T, D, NT>, dim3(p.n_reqs, p.Hkv), dim3(512), 0, stream, p);
+  FERRUM_CHECK_LAUNCH("attention_packed merge");
+  return 0;
+}
+
+int most_ctas() { return MAX_RESIDENT * ferrum_sm_count(); }
 
 }  // namespace
 
 FERRUM_API int ferrum_attention_packed_rows() { return PACKED_FEW_ROWS; }
 
-// Floats of workspace that a call needs.
-FERRUM_API long long ferrum_attention_packed_workspace(int D) { return 0; }
+// Floats of workspace that a call needs: the slots of the CTAs' partials, and where the parts of every (request, head, row tile) lie.
+FERRUM_API long long ferrum_attention_packed_workspace(int D, int Hkv, int n_reqs) {
+  return (long long)most_ctas() * 2 * PART_ROWS * (D + 2) + (long long)n_reqs * Hkv * 2 * 2;
+}
 
+// part: workspace of ferrum_attention_packed_workspace(D, Hkv, n_reqs) floats; calls that may run at the same time need one each.
 FERRUM_API int ferrum_attention_packed(const void* q, int ldq, void* out, int ldo, int dtype, const void* plane, long long page_stride, int n_pages,
                                        int page_size, const int* block_table, int table_width, const int* q_start, const int* pos0, int n_reqs,
                                        int n_tokens, float* part, long long part_floats, int Hq, int Hkv, int D, float scale, int window,
                                        int* err_flag, cudaStream_t stream) {
-  FERRUM_CHECK_ARG(Hq > 0 && Hkv > 0 && Hq % Hkv == 0, "attention_packed: bad head counts Hq=%d Hkv=%d", Hq, Hkv);
+  FERRUM_CHECK_ARG(Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && Hkv <= 65535, "attention_packed: bad head counts Hq=%d Hkv=%d", Hq, Hkv);
   FERRUM_CHECK_ARG(D == 64 || D == 128, "attention_packed: a cache in 4 bits has heads of 64 or 128 elements, found %d", D);
   FERRUM_CHECK_ARG(packed_page_ok(page_size) && table_width > 0 && n_pages > 0 && window >= 0 && n_reqs >= 0 && n_tokens >= 0,
                    "attention_packed: bad sizes (page size %d must be a multiple of %d)", page_size, PACKED_POS);
   FERRUM_CHECK_ARG(err_flag != nullptr, "attention_packed: the error flag is required");
-  FERRUM_CHECK_ARG((((uintptr_t)q | (uintptr_t)out | (uintptr_t)plane) & 15) == 0 && ldq % 8 == 0 && ldo % 8 == 0 && page_stride % 16 == 0,
+  FERRUM_CHECK_ARG((((uintptr_t)q | (uintptr_t)out | (uintptr_t)plane | (uintptr_t)part) & 15) == 0 && ldq % 8 == 0 && ldo % 8 == 0 && page_stride % 16 == 0,
                    "attention_packed: operands must be 16-byte aligned");
   FERRUM_CHECK_ARG(ldq >= Hq * D && ldo >= Hq * D, "attention_packed: rows of %d and %d elements are too short", ldq, ldo);
-  FERRUM_CHECK_ARG(part_floats >= ferrum_attention_packed_workspace(D), "attention_packed: the workspace is too small");
+  FERRUM_CHECK_ARG(part_floats >= ferrum_attention_packed_workspace(D, Hkv, n_reqs), "attention_packed: the workspace is too small");
   if (n_reqs == 0 || n_tokens == 0) return 0;
-  PackedParams p{q, out, (const uint8_t*)plane, block_table, q_start, pos0, err_flag, page_stride, ldq, ldo, n_pages, page_size, table_width, Hq, Hkv, window, scale};
+  const int ctas = most_ctas(), G = Hq / Hkv;
+  float* part_ml = part + (size_t)ctas * 2 * PART_ROWS * D;
+  PackedParams p{q, out, (const uint8_t*)plane, block_table, q_start, pos0, part, part_ml, reinterpret_cast<int2*>(part_ml + (size_t)ctas * 2 * PART_ROWS * 2),
+                 err_flag, page_stride, ldq, ldo, n_pages, page_size, table_width, Hq, Hkv, G, window, n_reqs, scale * 1.4426950408889634f};
+  // One row tile of 8 where every request brings a token of at most 8 rows (a longer one takes two passes over its keys), else 16 rows
+  // in one pass.
+  const bool narrow = G <= 8 && n_tokens <= n_reqs;
   FERRUM_DISPATCH_16BIT(dtype, T, {
-    if (D == 64) launch_kernel(attention_packed_kernel<T, 64>, dim3(n_reqs, Hkv), dim3(128), 0, stream, p);
-    else launch_kernel(attention_packed_kernel<T, 128>, dim3(n_reqs, Hkv), dim3(128), 0, stream, p);
+    if (D == 64) return narrow ? launch_packed<T, 64, 1, 2>(p, stream) : launch_packed<T, 64, 2, 1>(p, stream);
+    return narrow ? launch_packed<T, 128, 1, 2>(p, stream) : launch_packed<T, 128, 2, 1>(p, stream);
   });
-  FERRUM_CHECK_LAUNCH("attention_packed");
   return 0;
 }

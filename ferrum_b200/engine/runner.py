@@ -31,6 +31,7 @@ _DEVICE_ERRORS = {
     23: "tensor-core attention: keys or values did not arrive in time", 24: "tensor-core attention: the weights were not ready in time",
     25: "tensor-core attention: the scores were not ready in time", 26: "tensor-core attention: the output was not ready in time",
     27: "tensor-core attention: a product did not finish in time", 28: "tensor-core attention: the last values did not arrive in time",
+    29: "attention over a cache in 4 bits: keys and values did not arrive in time",
 }
 
 

@@ -827,16 +827,16 @@ def attention_packed_rows():
     return int(lib().ferrum_attention_packed_rows())
 
 
-def attention_packed_workspace(D):
+def attention_packed_workspace(D, Hkv, n_reqs):
     """float32 elements of the workspace of `attention_packed`."""
-    return int(lib().ferrum_attention_packed_workspace(D))
+    return int(lib().ferrum_attention_packed_workspace(D, Hkv, n_reqs))
 
 
 def attention_packed(q, out, n_tokens, block_table, q_start, pos0, plane, page_stride, page_size, Hq, Hkv, D, scale, window, err, part):
     """Causal grouped-query attention over a cache held in 4 bits, for the requests of the step that bring few rows (decoded tokens, see
     `attention_packed_rows`); the rows of other requests stay as they are.  q_start (int32 [requests + 1]): first token of
     each request; pos0 (int32 [requests]): positions cached before the step, whose own keys must be in the pages already.  part:
-    float32 workspace of `attention_packed_workspace(D)` elements; calls that may run at the same time need one each."""
+    float32 workspace of `attention_packed_workspace(D, Hkv, requests)` elements; calls that may run at the same time need one each."""
     _need16(q, "q", 2); _need16(out, "out", 2, like=q); _need(q_start, torch.int32, "q_start", 1); _need(pos0, torch.int32, "pos0", 1)
     _need_table(block_table, "attention_packed"); _need_packed(plane, page_stride, page_size, Hkv, D, "attention_packed")
     _need(part, torch.float32, "part", 1)

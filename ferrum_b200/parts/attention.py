@@ -121,7 +121,7 @@ class PagedAttention(Mixer):
         few = ops.attention_packed_rows()
         rows = [n * (Hq // Hkv) for n in ctx.h_q_len]
         if min(rows) <= few:
-            part = ctx.buf("attn_packed_part", (ops.attention_packed_workspace(D),), torch.float32)
+            part = ctx.buf("attn_packed_part", (ops.attention_packed_workspace(D, Hkv, ctx.n_reqs),), torch.float32)
             if ops.profiling():      # (a step with prompt portions counts the whole step's work for each kernel)
                 ops.set_work(ops.attention_work(ctx, Hq, Hkv, D, self.window, 9 / 16))
             ops.attention_packed(qkv, out, ctx.n_tokens, table, ctx.q_start, ctx.pos0, cache.plane, cache.page_stride, cache.page_size,
