@@ -21,6 +21,8 @@
 #include "packed_cache.cuh"
 #include "ptx_sm100.cuh"
 
+#include <type_traits>
+
 namespace {
 
 constexpr int WARPS = 4;
@@ -65,6 +67,12 @@ __device__ __forceinline__ unsigned less(unsigned a, unsigned b) {       // a - 
 template <typename T> __device__ __forceinline__ float2 pair_values(unsigned v);
 template <> __device__ __forceinline__ float2 pair_values<__nv_bfloat16>(unsigned v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)); }
 template <> __device__ __forceinline__ float2 pair_values<__half>(unsigned v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
+
+__device__ __forceinline__ float exp2_fast(float x) {      // 2 ulp; below 2^-126: 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 // Waits for a copy, about a second at most (a moment once one has failed to come).
 __device__ __forceinline__ bool arrived(uint32_t bar, uint32_t parity, bool failed) {
@@ -142,7 +150,6 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
   // ---- the rows' queries as float16 operands, their sums per group and their scale
   unsigned qf[NT][GN][4][2];
   float q_sum[NT][GN][2], f_row[NT][2];
-  int row_pos[NT][2], row_lo[NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int row = row0 + nt * 8 + gid;
@@ -167,7 +174,7 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
     big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
     // 2^e brings the largest element to [2^14, 2^15); a row of zeros (or of subnormals) keeps e within a float's exponents
     const int e = max(-100, min(100, 14 + 127 - (int)(__float_as_uint(big) >> 23)));
-    const float up = __uint_as_float((unsigned)(127 + e) << 23);
+    const float up = copysignf(__uint_as_float((unsigned)(127 + e) << 23), p.scale_log2);      // (f_row is not negative: it orders the scores)
     float sum[GN];
 #pragma unroll
     for (int g = 0; g < GN; ++g) {
@@ -188,15 +195,13 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
         }
     }
     // the scores' columns: this thread meets rows 2 tig and 2 tig + 1
-    const float f = p.scale_log2 * __uint_as_float((unsigned)(127 - e) << 23) * 16777216.f;
+    const float f = fabsf(p.scale_log2) * __uint_as_float((unsigned)(127 - e) << 23) * 16777216.f;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int from = (2 * tig + c) * 4;
       f_row[nt][c] = __shfl_sync(0xffffffffu, f, from);
 #pragma unroll
       for (int g = 0; g < GN; ++g) q_sum[nt][g][c] = __shfl_sync(0xffffffffu, sum[g], from) * 0x1p-24f;
-      row_pos[nt][c] = pos0 + (row0 + nt * 8 + 2 * tig + c) / p.G;
-      row_lo[nt][c] = p.window > 0 ? max(0, row_pos[nt][c] - p.window + 1) : 0;
     }
   }
   // keys that every row sees: from the last row's window on, up to the first row's position
@@ -218,24 +223,13 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
     }
   float step_limit = 0x1p-100f, v_up = 0x1p114f;       // the largest step seen is at most step_limit = 2^14 / v_up
 
-  for (int i = 0; i < n_blocks; i += NB) {
+  // Blocks i .. i + NB - 1 of the warp.  MASKED: some key of theirs is hidden from some row, lies behind the last key or has no page.
+  auto blocks_step = [&](auto masked, int i, const bool (&have)[NB], const int (&key0)[NB]) {
+    constexpr bool MASKED = decltype(masked)::value;
     const uint8_t* block[NB];
-    bool have[NB];
-    int key0[NB];
-    bool whole = true;
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      const int s = (i + b) % STAGES;
-      block[b] = ring + s * B::BYTES;
-      have[b] = i + b < n_blocks && !(missing >> s & 1);
-      key0[b] = key_lo + (b0 + (i + b) * WARPS) * PACKED_POS;
-      if (have[b]) {
-        failed = __any_sync(0xffffffffu, !arrived(bars + 8 * s, phases >> s & 1, failed) || failed);
-        phases ^= 1u << s;
-      }
-      whole &= have[b] && key0[b] + PACKED_POS - 1 <= all_hi && key0[b] >= all_lo;
-    }
-    // ---- scores
+    for (int b = 0; b < NB; ++b) block[b] = ring + (i + b) % STAGES * B::BYTES;
+    // ---- scores, still to be multiplied by f_row
     float s[NB][NT][4];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
@@ -263,37 +257,35 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
           }
         }
       }
-      float step[GN][2], mid[GN][2];
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
+      for (int k = 0; k < 2; ++k) {
 #pragma unroll
         for (int g = 0; g < GN; ++g) {
           const float2 v = pair_values<T>(reinterpret_cast<const unsigned*>(block[b] + B::K_PAIRS)[(gid + 8 * k) * GN + g]);
-          step[g][k] = v.x;
-          mid[g][k] = fmaf(-8.f, v.x, v.y);
+          const float mid = fmaf(-8.f, v.x, v.y);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const float t = fmaf(v.x, part[nt][g][2 * k + c], mid * q_sum[nt][g][c]);
+              s[b][nt][2 * k + c] = g == 0 ? t : s[b][nt][2 * k + c] + t;
+            }
         }
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float t = 0.f;
-#pragma unroll
-          for (int g = 0; g < GN; ++g) t = fmaf(step[g][e >> 1], part[nt][g][e], fmaf(mid[g][e >> 1], q_sum[nt][g][e & 1], t));
-          s[b][nt][e] = t * f_row[nt][e & 1];
-        }
-      if (!whole) {
+      }
+      if (MASKED) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int key = key0[b] + gid + 8 * (e >> 1);
-            if (!have[b] || key > row_pos[nt][e & 1] || key < row_lo[nt][e & 1] || key >= hi) s[b][nt][e] = -INFINITY;
+            const int key = key0[b] + gid + 8 * (e >> 1), row = row0 + nt * 8 + 2 * tig + (e & 1);
+            const int at = pos0 + row / p.G;
+            if (!have[b] || key > at || (p.window > 0 && key <= at - p.window) || key >= hi) s[b][nt][e] = -INFINITY;
           }
       }
     }
     // ---- the running maximum and sum
     bool moved = false;
-    float corr[NT][2], m_use[NT][2];
+    float m_use[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -304,29 +296,33 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-        const float m_new = fmaxf(m_run[nt][c], mx);
-        m_use[nt][c] = m_new == -INFINITY ? 0.f : m_new;
-        corr[nt][c] = exp2f(m_run[nt][c] - m_use[nt][c]);
-        moved |= m_new != m_run[nt][c];
-        m_run[nt][c] = m_new;
+        m_use[nt][c] = fmaxf(m_run[nt][c], mx);
+        moved |= m_use[nt][c] != m_run[nt][c];
       }
     if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          l_run[nt][c] *= corr[nt][c];
+          // (nothing seen so far: the sums are zeros)
+          const float corr = m_run[nt][c] == -INFINITY ? 0.f : exp2_fast((m_run[nt][c] - m_use[nt][c]) * f_row[nt][c]);
+          m_run[nt][c] = m_use[nt][c];
+          l_run[nt][c] *= corr;
 #pragma unroll
           for (int g = 0; g < GN; ++g) {
-            mid_acc[nt][g][c] *= corr[nt][c];
+            mid_acc[nt][g][c] *= corr;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              o[nt][g][j][c] *= corr[nt][c];
-              o[nt][g][j][2 + c] *= corr[nt][c];
+              o[nt][g][j][c] *= corr;
+              o[nt][g][j][2 + c] *= corr;
             }
           }
         }
     }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) m_use[nt][c] = MASKED && m_run[nt][c] == -INFINITY ? 0.f : -m_run[nt][c] * f_row[nt][c];
     // ---- values
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
@@ -336,7 +332,7 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
 #pragma unroll
         for (int g = 0; g < GN; ++g) {
           float2 v = pair_values<T>(reinterpret_cast<const unsigned*>(block[b] + B::V_PAIRS)[(gid + 8 * k) * GN + g]);
-          if (!whole && (!have[b] || key0[b] + gid + 8 * k >= hi)) v = make_float2(0.f, 0.f);      // (what lies behind the last key may be a NaN)
+          if (MASKED && (!have[b] || key0[b] + gid + 8 * k >= hi)) v = make_float2(0.f, 0.f);      // (what lies behind the last key may be a NaN)
           step[g][k] = v.x;
           mid[g][k] = v.y;
           most = fmaxf(most, v.x);
@@ -362,7 +358,8 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
         float w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          w[e] = exp2f(s[b][nt][e] - m_use[nt][e & 1]);
+          w[e] = exp2_fast(fmaf(s[b][nt][e], f_row[nt][e & 1], m_use[nt][e & 1]));
+          if (MASKED && s[b][nt][e] == -INFINITY) w[e] = 0.f;      // (f_row may be 0)
           l_run[nt][e & 1] += w[e];
         }
 #pragma unroll
@@ -371,13 +368,15 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
           for (int k = 0; k < 2; ++k) {
             const float up = step[g][k] * v_up;
             float x0 = w[2 * k] * up, x1 = w[2 * k + 1] * up;
-            float y0 = w[2 * k] * mid[g][k], y1 = w[2 * k + 1] * mid[g][k];
-            if (!whole) {              // a key that a row does not see counts for nothing, whatever it holds
-              if (w[2 * k] == 0.f) x0 = y0 = 0.f;
-              if (w[2 * k + 1] == 0.f) x1 = y1 = 0.f;
+            if (MASKED) {              // a key that a row does not see counts for nothing, whatever it holds
+              if (w[2 * k] == 0.f) x0 = 0.f;
+              if (w[2 * k + 1] == 0.f) x1 = 0.f;
+              if (w[2 * k] != 0.f) mid_acc[nt][g][0] = fmaf(w[2 * k], mid[g][k], mid_acc[nt][g][0]);
+              if (w[2 * k + 1] != 0.f) mid_acc[nt][g][1] = fmaf(w[2 * k + 1], mid[g][k], mid_acc[nt][g][1]);
+            } else {
+              mid_acc[nt][g][0] = fmaf(w[2 * k], mid[g][k], mid_acc[nt][g][0]);
+              mid_acc[nt][g][1] = fmaf(w[2 * k + 1], mid[g][k], mid_acc[nt][g][1]);
             }
-            mid_acc[nt][g][0] += y0;
-            mid_acc[nt][g][1] += y1;
             pf[nt][g][k] = transpose8(pack2<__half>(x0, x1));
           }
         }
@@ -404,6 +403,24 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
         }
       }
     }
+  };
+
+  for (int i = 0; i < n_blocks; i += NB) {
+    bool have[NB], whole = true;
+    int key0[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const int s = (i + b) % STAGES;
+      have[b] = i + b < n_blocks && !(missing >> s & 1);
+      key0[b] = key_lo + (b0 + (i + b) * WARPS) * PACKED_POS;
+      if (have[b]) {
+        failed = __any_sync(0xffffffffu, !arrived(bars + 8 * s, phases >> s & 1, failed) || failed);
+        phases ^= 1u << s;
+      }
+      whole &= have[b] && key0[b] + PACKED_POS - 1 <= all_hi && key0[b] >= all_lo;
+    }
+    if (whole) blocks_step(std::false_type{}, i, have, key0);
+    else blocks_step(std::true_type{}, i, have, key0);
     // ---- the stages are free: the next blocks
     __syncwarp();
 #pragma unroll
@@ -436,7 +453,7 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
     for (int c = 0; c < 2; ++c) {
       const int row = 2 * tig + c;
       if (gid == 0) {
-        ml[(warp * 8 + row) * 2] = m_run[nt][c];
+        ml[(warp * 8 + row) * 2] = m_run[nt][c] == -INFINITY ? -INFINITY : m_run[nt][c] * f_row[nt][c];
         ml[(warp * 8 + row) * 2 + 1] = l_run[nt][c];
       }
 #pragma unroll
