@@ -27,7 +27,8 @@ namespace {
 
 constexpr int WARPS = 4;
 constexpr int TILE = WARPS * PACKED_POS;     // keys of a unit
-constexpr int STAGES = 4;                    // blocks in a warp's ring
+constexpr int NB = 2;                        // blocks of a step: one running maximum for 32 keys
+constexpr int HALVES = 2;                    // steps in a warp's ring: one is read while the next arrives
 constexpr int PART_ROWS = 16;                // rows of a partial's slot
 
 struct PackedParams {
@@ -68,6 +69,17 @@ template <typename T> __device__ __forceinline__ float2 pair_values(unsigned v);
 template <> __device__ __forceinline__ float2 pair_values<__nv_bfloat16>(unsigned v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)); }
 template <> __device__ __forceinline__ float2 pair_values<__half>(unsigned v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
 
+template <int N>
+__device__ __forceinline__ void load_words(unsigned (&w)[N], const uint8_t* p) {
+  if (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x;
+    w[N - 1] = v.y;
+  } else {
+    w[0] = *reinterpret_cast<const unsigned*>(p);
+  }
+}
+
 __device__ __forceinline__ float exp2_fast(float x) {      // 2 ulp; below 2^-126: 0
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -103,9 +115,9 @@ __device__ __forceinline__ Span span_of(const PackedParams& p, int r) {
 
 // One CTA's share of the units of (request r, KV head kvh, row tile rt): tiles [t0, t1).  slot < 0: that is all of them, the result
 // is written; otherwise the partial goes to the slot.
-template <typename T, int D, int NT, int NB>
+template <typename T, int D, int NT>
 __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kvh, int rt, int key_lo, int t0, int t1, int slot, uint8_t* ring,
-                                            uint32_t bars, uint32_t& phases, float* merge, bool& failed) {
+                                            uint32_t bars, uint32_t& turn, float* merge, bool& failed) {
   using B = PackedBlock<D>;
   constexpr int GN = B::GROUPS;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tig = lane & 3;
@@ -118,34 +130,29 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
   const int* bt = p.block_table + (size_t)r * p.table_width;
   const uint8_t* head = p.plane + (size_t)kvh * (p.page_size / PACKED_POS) * B::BYTES;
 
-  // ---- the pages of the warp's next 32 blocks, one a lane; the copies of the first STAGES
-  int my_page = -1, my_in_page = 0;
-  auto fetch_pages = [&](int i) {      // for blocks i .. i + 31 of the warp
+  // ---- where the warp's next 32 blocks lie, one a lane, which also asks for its copy when the step's turn comes
+  const uint8_t* my_src = head;
+  auto find_blocks = [&](int i) {      // blocks i .. i + 31 of the warp
     const int k = i + lane;
-    my_page = -1;
     if (k < n_blocks) {
       const int key = key_lo + (b0 + k * WARPS) * PACKED_POS, lp = key / p.page_size;
-      my_in_page = (key - lp * p.page_size) / PACKED_POS;
-      my_page = lp < p.table_width ? bt[lp] : -1;
-      if (my_page < 0 || my_page >= p.n_pages) {
-        my_page = -1;
+      int page = lp < p.table_width ? bt[lp] : -1;
+      if (page < 0 || page >= p.n_pages) {      // the flag fails the step; the request's rows are nobody's then, and page 0 will do
         atomicExch(p.err, 5);
+        page = 0;
       }
+      my_src = head + (size_t)page * p.page_stride + (size_t)((key - lp * p.page_size) / PACKED_POS) * B::BYTES;
     }
   };
-  unsigned missing = 0;                // per stage: its block has no page
-  auto request_block = [&](int i) {    // copies block i of the warp into its stage; called by the whole warp
-    const int s = i % STAGES;
-    const int page = __shfl_sync(0xffffffffu, my_page, i & 31), in_page = __shfl_sync(0xffffffffu, my_in_page, i & 31);
-    missing = (missing & ~(1u << s)) | ((page < 0 ? 1u : 0u) << s);
-    if (page >= 0 && lane == 0) {
-      sm100::mbar_expect_tx(bars + 8 * s, B::BYTES);
-      bulk_load(sm100::smem_u32(ring + s * B::BYTES), head + (size_t)page * p.page_stride + (size_t)in_page * B::BYTES, B::BYTES, bars + 8 * s);
-    }
+  auto request = [&](int j) {          // the copies of step j: blocks NB j .. NB j + NB - 1, those that there are
+    if ((NB * j & 31) == 0) find_blocks(NB * j);
+    const uint32_t half = (turn + j) % HALVES, bar = bars + 8 * half;
+    const int b = lane - (NB * j & 31), n = min(NB, n_blocks - NB * j);
+    if (b == 0) sm100::mbar_expect_tx(bar, n * B::BYTES);
+    if (b >= 0 && b < n) bulk_load(sm100::smem_u32(ring + (half * NB + b) * B::BYTES), my_src, B::BYTES, bar);
   };
-  int asked = 0;
-  fetch_pages(0);
-  for (; asked < min(STAGES, n_blocks); ++asked) request_block(asked);
+  const int n_steps = (n_blocks + NB - 1) / NB;
+  for (int j = 0; j < min(HALVES, n_steps); ++j) request(j);
 
   // ---- the rows' queries as float16 operands, their sums per group and their scale
   unsigned qf[NT][GN][4][2];
@@ -223,12 +230,9 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
     }
   float step_limit = 0x1p-100f, v_up = 0x1p114f;       // the largest step seen is at most step_limit = 2^14 / v_up
 
-  // Blocks i .. i + NB - 1 of the warp.  MASKED: some key of theirs is hidden from some row, lies behind the last key or has no page.
-  auto blocks_step = [&](auto masked, int i, const bool (&have)[NB], const int (&key0)[NB]) {
+  // The step's blocks, the first at key0.  MASKED: some key of theirs is hidden from some row or lies behind the last key.
+  auto step_of = [&](auto masked, const uint8_t* const first, const int key0, const int n) {
     constexpr bool MASKED = decltype(masked)::value;
-    const uint8_t* block[NB];
-#pragma unroll
-    for (int b = 0; b < NB; ++b) block[b] = ring + (i + b) % STAGES * B::BYTES;
     // ---- scores, still to be multiplied by f_row
     float s[NB][NT][4];
 #pragma unroll
@@ -242,8 +246,8 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
           for (int e = 0; e < 4; ++e) part[nt][g][e] = 0.f;
 #pragma unroll
       for (int g = 0; g < GN; ++g) {
-        const uint2 u = *reinterpret_cast<const uint2*>(block[b] + gid * B::ROW + g * 32 + tig * 8);
-        const uint2 v = *reinterpret_cast<const uint2*>(block[b] + (gid + 8) * B::ROW + g * 32 + tig * 8);
+        const uint2 u = *reinterpret_cast<const uint2*>(first + b * B::BYTES + gid * B::ROW + g * 32 + tig * 8);
+        const uint2 v = *reinterpret_cast<const uint2*>(first + b * B::BYTES + (gid + 8) * B::ROW + g * 32 + tig * 8);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           unsigned wu = j ? u.y : u.x, wv = j ? v.y : v.x;
@@ -259,9 +263,11 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
       }
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
+        unsigned pairs[GN];
+        load_words<GN>(pairs, first + b * B::BYTES + B::K_PAIRS + (gid + 8 * k) * GN * 4);
 #pragma unroll
         for (int g = 0; g < GN; ++g) {
-          const float2 v = pair_values<T>(reinterpret_cast<const unsigned*>(block[b] + B::K_PAIRS)[(gid + 8 * k) * GN + g]);
+          const float2 v = pair_values<T>(pairs[g]);
           const float mid = fmaf(-8.f, v.x, v.y);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
@@ -277,9 +283,9 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int key = key0[b] + gid + 8 * (e >> 1), row = row0 + nt * 8 + 2 * tig + (e & 1);
+            const int key = key0 + b * TILE + gid + 8 * (e >> 1), row = row0 + nt * 8 + 2 * tig + (e & 1);
             const int at = pos0 + row / p.G;
-            if (!have[b] || key > at || (p.window > 0 && key <= at - p.window) || key >= hi) s[b][nt][e] = -INFINITY;
+            if (b >= n || key > at || (p.window > 0 && key <= at - p.window) || key >= hi) s[b][nt][e] = -INFINITY;
           }
       }
     }
@@ -324,34 +330,39 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
 #pragma unroll
       for (int c = 0; c < 2; ++c) m_use[nt][c] = MASKED && m_run[nt][c] == -INFINITY ? 0.f : -m_run[nt][c] * f_row[nt][c];
     // ---- values
+    float step[NB][GN][2], mid[NB][GN][2], most = 0.f;
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      float step[GN][2], mid[GN][2], most = 0.f;
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
+      for (int k = 0; k < 2; ++k) {
+        unsigned pairs[GN];
+        load_words<GN>(pairs, first + b * B::BYTES + B::V_PAIRS + (gid + 8 * k) * GN * 4);
 #pragma unroll
         for (int g = 0; g < GN; ++g) {
-          float2 v = pair_values<T>(reinterpret_cast<const unsigned*>(block[b] + B::V_PAIRS)[(gid + 8 * k) * GN + g]);
-          if (MASKED && (!have[b] || key0[b] + gid + 8 * k >= hi)) v = make_float2(0.f, 0.f);      // (what lies behind the last key may be a NaN)
-          step[g][k] = v.x;
-          mid[g][k] = v.y;
+          float2 v = pair_values<T>(pairs[g]);
+          if (MASKED && (b >= n || key0 + b * TILE + gid + 8 * k >= hi)) v = make_float2(0.f, 0.f);      // (what lies behind the last key may be a NaN)
+          step[b][g][k] = v.x;
+          mid[b][g][k] = v.y;
           most = fmaxf(most, v.x);
         }
-      if (__any_sync(0xffffffffu, most > step_limit)) {
-        const unsigned top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
-        const int e = min(127, (int)(top >> 23) - 126);              // top < 2^e
-        const float up = __uint_as_float((unsigned)(127 + 14 - e) << 23), ratio = up / v_up;
-        step_limit = __uint_as_float(min((unsigned)(127 + e), 254u) << 23);
-        v_up = up;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int g = 0; g < GN; ++g)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-              for (int c = 0; c < 4; ++c) o[nt][g][j][c] *= ratio;
       }
+    if (__any_sync(0xffffffffu, most > step_limit)) {
+      const unsigned top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
+      const int e = min(127, (int)(top >> 23) - 126);              // top < 2^e
+      const float up = __uint_as_float((unsigned)(127 + 14 - e) << 23), ratio = up / v_up;
+      step_limit = __uint_as_float(min((unsigned)(127 + e), 254u) << 23);
+      v_up = up;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int g = 0; g < GN; ++g)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[nt][g][j][c] *= ratio;
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
       unsigned pf[NT][GN][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -366,16 +377,16 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
         for (int g = 0; g < GN; ++g) {
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            const float up = step[g][k] * v_up;
+            const float up = step[b][g][k] * v_up;
             float x0 = w[2 * k] * up, x1 = w[2 * k + 1] * up;
             if (MASKED) {              // a key that a row does not see counts for nothing, whatever it holds
               if (w[2 * k] == 0.f) x0 = 0.f;
               if (w[2 * k + 1] == 0.f) x1 = 0.f;
-              if (w[2 * k] != 0.f) mid_acc[nt][g][0] = fmaf(w[2 * k], mid[g][k], mid_acc[nt][g][0]);
-              if (w[2 * k + 1] != 0.f) mid_acc[nt][g][1] = fmaf(w[2 * k + 1], mid[g][k], mid_acc[nt][g][1]);
+              if (w[2 * k] != 0.f) mid_acc[nt][g][0] = fmaf(w[2 * k], mid[b][g][k], mid_acc[nt][g][0]);
+              if (w[2 * k + 1] != 0.f) mid_acc[nt][g][1] = fmaf(w[2 * k + 1], mid[b][g][k], mid_acc[nt][g][1]);
             } else {
-              mid_acc[nt][g][0] = fmaf(w[2 * k], mid[g][k], mid_acc[nt][g][0]);
-              mid_acc[nt][g][1] = fmaf(w[2 * k + 1], mid[g][k], mid_acc[nt][g][1]);
+              mid_acc[nt][g][0] = fmaf(w[2 * k], mid[b][g][k], mid_acc[nt][g][0]);
+              mid_acc[nt][g][1] = fmaf(w[2 * k + 1], mid[b][g][k], mid_acc[nt][g][1]);
             }
             pf[nt][g][k] = transpose8(pack2<__half>(x0, x1));
           }
@@ -387,7 +398,7 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
         unsigned w[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          w[k] = *reinterpret_cast<const unsigned*>(block[b] + B::V_CODES + (2 * tig + (k & 1) + 8 * (k >> 1)) * B::ROW + g * 32 + gid * 4);
+          w[k] = *reinterpret_cast<const unsigned*>(first + b * B::BYTES + B::V_CODES + (2 * tig + (k & 1) + 8 * (k >> 1)) * B::ROW + g * 32 + gid * 4);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           unsigned x = __byte_perm(w[0], w[1], half ? 0x7632 : 0x5410), y = __byte_perm(w[2], w[3], half ? 0x7632 : 0x5410);
@@ -405,34 +416,20 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
     }
   };
 
-  for (int i = 0; i < n_blocks; i += NB) {
-    bool have[NB], whole = true;
-    int key0[NB];
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      const int s = (i + b) % STAGES;
-      have[b] = i + b < n_blocks && !(missing >> s & 1);
-      key0[b] = key_lo + (b0 + (i + b) * WARPS) * PACKED_POS;
-      if (have[b]) {
-        failed = __any_sync(0xffffffffu, !arrived(bars + 8 * s, phases >> s & 1, failed) || failed);
-        phases ^= 1u << s;
-      }
-      whole &= have[b] && key0[b] + PACKED_POS - 1 <= all_hi && key0[b] >= all_lo;
-    }
-    if (whole) blocks_step(std::false_type{}, i, have, key0);
-    else blocks_step(std::true_type{}, i, have, key0);
-    // ---- the stages are free: the next blocks
-    __syncwarp();
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-      if (asked < n_blocks && !failed) {
-        if ((asked & 31) == 0) fetch_pages(asked);
-        request_block(asked++);
-      } else if (asked < n_blocks) {
-        missing |= 1u << (asked++ % STAGES);
-      }
+  // whole blocks, by their number in the warp: [k_lo, k_hi) hide no key from any row
+  const int base = key_lo + b0 * PACKED_POS;
+  const int k_lo = all_lo > base ? (all_lo - base + TILE - 1) / TILE : 0, k_hi = all_hi - PACKED_POS + 1 >= base ? (all_hi - PACKED_POS + 1 - base) / TILE + 1 : 0;
+  for (int j = 0; j < n_steps; ++j) {
+    const uint32_t half = (turn + j) % HALVES;
+    failed |= !arrived(bars + 8 * half, (turn + j) / HALVES & 1, failed);
+    const uint8_t* first = ring + half * NB * B::BYTES;
+    if (NB * j >= k_lo && NB * j + NB <= min(k_hi, n_blocks)) step_of(std::false_type{}, first, 0, NB);
+    else step_of(std::true_type{}, first, base + NB * j * TILE, n_blocks - NB * j);
+    __syncwarp();                      // the half is free
+    if (j + HALVES < n_steps) request(j + HALVES);
   }
-  if (failed && lane == 0) atomicExch(p.err, 29);
+  turn += n_steps;
+  if (failed) atomicExch(p.err, 29);
 
   // ---- the warps' parts meet, eight rows at a time
   const float down = 1.f / v_up;
@@ -494,20 +491,20 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
   }
 }
 
-template <typename T, int D, int NT, int NB>
+template <typename T, int D, int NT>
 __global__ void __launch_bounds__(WARPS * 32, RESIDENT<D, NT>)
 attention_packed_kernel(const PackedParams p) {
   using B = PackedBlock<D>;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ __align__(8) unsigned long long bars_mem[WARPS * STAGES];
+  __shared__ __align__(8) unsigned long long bars_mem[WARPS * HALVES];
   __shared__ long long s_scan[WARPS], s_start;
   __shared__ int s_req;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  uint8_t* ring = smem + warp * STAGES * B::BYTES;
-  float* merge = reinterpret_cast<float*>(smem + WARPS * STAGES * B::BYTES);
-  const uint32_t bars = sm100::smem_u32(bars_mem + warp * STAGES);
+  uint8_t* ring = smem + warp * HALVES * NB * B::BYTES;
+  float* merge = reinterpret_cast<float*>(smem + WARPS * HALVES * NB * B::BYTES);
+  const uint32_t bars = sm100::smem_u32(bars_mem + warp * HALVES);
   if (lane == 0)
-    for (int s = 0; s < STAGES; ++s) sm100::mbar_init(bars + 8 * s, 1);
+    for (int s = 0; s < HALVES; ++s) sm100::mbar_init(bars + 8 * s, 1);
   sm100::fence_barrier_init();
   sm100::fence_proxy_async();
   pdl_launch();
@@ -556,7 +553,7 @@ attention_packed_kernel(const PackedParams p) {
   }
   __syncthreads();
   // ---- walk the share
-  uint32_t phases = 0;
+  uint32_t turn = 0;      // steps that the warp has run: a step's half of the ring and its barrier's phase follow from its number
   bool failed = false;
   long long u = first, start = s_start;
   for (int r = s_req; u < last; ++r) {
@@ -573,7 +570,7 @@ attention_packed_kernel(const PackedParams p) {
         const int k = (int)((pair_end * P - 1) / U);
         p.part_info[((size_t)r * p.Hkv + kvh) * 2 + rt] = make_int2((int)c * 2 + (u == first ? 0 : 1), k - (int)c + 1);
       }
-      packed_item<T, D, NT, NB>(p, r, kvh, rt, sp.lo, t0, t1, split ? (int)c * 2 + (u == first ? 0 : 1) : -1, ring, bars, phases, merge, failed);
+      packed_item<T, D, NT>(p, r, kvh, rt, sp.lo, t0, t1, split ? (int)c * 2 + (u == first ? 0 : 1) : -1, ring, bars, turn, merge, failed);
       u = pair_start + t1;
     }
     start += all;
@@ -647,16 +644,16 @@ packed_merge_kernel(const PackedParams p) {
   for (int e = 0; e < E; e += 2) reinterpret_cast<unsigned*>(dst)[e / 2] = pack2<T>(out[e] * inv, out[e + 1] * inv);
 }
 
-template <typename T, int D, int NT, int NB>
+template <typename T, int D, int NT>
 int launch_packed(const PackedParams& p, cudaStream_t stream) {
-  constexpr int smem = WARPS * STAGES * PackedBlock<D>::BYTES + WARPS * 8 * (D + 2) * 4;
+  constexpr int smem = WARPS * HALVES * NB * PackedBlock<D>::BYTES + WARPS * 8 * (D + 2) * 4;
   static bool configured = false;
   if (!configured) {
-    cudaError_t e = cudaFuncSetAttribute(attention_packed_kernel<T, D, NT, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaError_t e = cudaFuncSetAttribute(attention_packed_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     FERRUM_CHECK_ARG(e == cudaSuccess, "attention_packed: cannot reserve %d bytes of shared memory: %s", smem, cudaGetErrorString(e));
     configured = true;
   }
-  launch_kernel(attention_packed_kernel<T, D, NT, NB>, dim3(RESIDENT<D, NT> * ferrum_sm_count()), dim3(WARPS * 32), smem, stream, p);
+  launch_kernel(attention_packed_kernel<T, D, NT>, dim3(RESIDENT<D, NT> * ferrum_sm_count()), dim3(WARPS * 32), smem, stream, p);
   FERRUM_CHECK_LAUNCH("attention_packed");
   launch_kernel(packed_merge_kernel<T, D, NT>, dim3(p.n_reqs, p.Hkv), dim3(512), 0, stream, p);
   FERRUM_CHECK_LAUNCH("attention_packed merge");
@@ -697,8 +694,8 @@ FERRUM_API int ferrum_attention_packed(const void* q, int ldq, void* out, int ld
   // in one pass.
   const bool narrow = G <= 8 && n_tokens <= n_reqs;
   FERRUM_DISPATCH_16BIT(dtype, T, {
-    if (D == 64) return narrow ? launch_packed<T, 64, 1, 2>(p, stream) : launch_packed<T, 64, 2, 1>(p, stream);
-    return narrow ? launch_packed<T, 128, 1, 2>(p, stream) : launch_packed<T, 128, 2, 1>(p, stream);
+    if (D == 64) return narrow ? launch_packed<T, 64, 1>(p, stream) : launch_packed<T, 64, 2>(p, stream);
+    return narrow ? launch_packed<T, 128, 1>(p, stream) : launch_packed<T, 128, 2>(p, stream);
   });
   return 0;
 }
