@@ -8,8 +8,9 @@
 //   other pair by one shift more;
 //   scores       s = scale * sum_g (step_g * (q . c)_g + (middle_g - 8 step_g) * (sum of q)_g), g the groups of 64 elements: keys are the rows
 //                of the product (m16n8k16), the packed rows (tokens x query heads of the KV head) its columns;
-//   values       o = sum_j (p_j step_j) (c_j - 8) + p_j middle_j: elements are the rows, keys the contraction; the codes less 8 by one
-//                subtraction (exact), so that the sums do not cancel; the middles' sum on the CUDA cores in float32.
+//   values       o = sum_j (p_j step_j) (c_j - 8) + p_j middle_j: elements are the rows, keys the contraction; 8 times the sum of the very
+//                weights comes from a product with a constant and goes off every 512 keys, so that the sums do not outgrow what they
+//                stand for; the middles' sum on the CUDA cores in float32.
 // Roundings: q, a power of two times itself that puts a row's largest element at 2^14 to 2^15, is a float16 (exactly, from bfloat16 also, but for what is
 // 2^-30 below the largest); p step, times a power of two that follows the largest step seen, is rounded to float16: a weight's half
 // step of 2^-12, and the result's own.  All sums are float32.
@@ -28,7 +29,9 @@ namespace {
 constexpr int WARPS = 4;
 constexpr int TILE = WARPS * PACKED_POS;     // keys of a unit
 constexpr int NB = 2;                        // blocks of a step: one running maximum for 32 keys
+constexpr int SETTLE = 16;                   // steps after which the sums of codes are centred
 constexpr int HALVES = 2;                    // steps in a warp's ring: one is read while the next arrives
+static_assert(32 % NB == 0, "the blocks of a step lie in one window of 32 blocks, one a lane");
 constexpr int PART_ROWS = 16;                // rows of a partial's slot
 
 struct PackedParams {
@@ -51,19 +54,21 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
                : "memory");
 }
-__device__ __forceinline__ void mma_f16(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// c += a b, or c = a b for the first product of a sum.
+__device__ __forceinline__ void mma_f16(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1, bool first = false) {
+  if (first)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ unsigned transpose8(unsigned v) {
   unsigned r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
-}
-__device__ __forceinline__ unsigned less(unsigned a, unsigned b) {       // a - b, two float16 each
-  const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
-  return *reinterpret_cast<const unsigned*>(&r);
 }
 template <typename T> __device__ __forceinline__ float2 pair_values(unsigned v);
 template <> __device__ __forceinline__ float2 pair_values<__nv_bfloat16>(unsigned v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)); }
@@ -97,7 +102,7 @@ __device__ __forceinline__ bool arrived(uint32_t bar, uint32_t parity, bool fail
 
 // CTAs that an SM holds, as the registers of the accumulators allow.
 template <int D, int NT>
-constexpr int RESIDENT = NT == 1 ? 4 : D == 64 ? 3 : 2;
+constexpr int RESIDENT = NT == 1 ? 3 : D == 64 ? 3 : 2;
 constexpr int MAX_RESIDENT = 4;
 
 // A request's part of the line.
@@ -214,7 +219,7 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
   // keys that every row sees: from the last row's window on, up to the first row's position
   const int all_hi = pos0 + row0 / p.G, all_lo = p.window > 0 ? max(0, pos0 + (min(n_rows, row0 + 8 * NT) - 1) / p.G - p.window + 1) : 0;
 
-  float m_run[NT][2], l_run[NT][2], mid_acc[NT][GN][2], o[NT][GN][4][4];
+  float m_run[NT][2], l_run[NT][2], mid_acc[NT][GN][2], o[NT][GN][4][4], eights[NT][GN][4];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -223,7 +228,7 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
       l_run[nt][c] = 0.f;
 #pragma unroll
       for (int g = 0; g < GN; ++g) {
-        mid_acc[nt][g][c] = 0.f;
+        mid_acc[nt][g][c] = eights[nt][g][c] = eights[nt][g][2 + c] = 0.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[nt][g][j][c] = o[nt][g][j][2 + c] = 0.f;
       }
@@ -238,29 +243,23 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       float part[NT][GN][4];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int g = 0; g < GN; ++g)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) part[nt][g][e] = 0.f;
+      unsigned wu[GN][2], wv[GN][2];       // keys gid and gid + 8
 #pragma unroll
       for (int g = 0; g < GN; ++g) {
-        const uint2 u = *reinterpret_cast<const uint2*>(first + b * B::BYTES + gid * B::ROW + g * 32 + tig * 8);
-        const uint2 v = *reinterpret_cast<const uint2*>(first + b * B::BYTES + (gid + 8) * B::ROW + g * 32 + tig * 8);
+        load_words<2>(wu[g], first + b * B::BYTES + gid * B::ROW + g * 32 + tig * 8);
+        load_words<2>(wv[g], first + b * B::BYTES + (gid + 8) * B::ROW + g * 32 + tig * 8);
+      }
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          unsigned wu = j ? u.y : u.x, wv = j ? v.y : v.x;
+      for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int g = 0; g < GN; ++g) {
+            const unsigned u = wu[g][j] >> (8 * h), v = wv[g][j] >> (8 * h);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-              mma_f16(part[nt][g], wu & 0x000F000Fu, wv & 0x000F000Fu, wu & 0x00F000F0u, wv & 0x00F000F0u, qf[nt][g][2 * j + h][0], qf[nt][g][2 * j + h][1]);
-            wu >>= 8;
-            wv >>= 8;
+              mma_f16(part[nt][g], u & 0x000F000Fu, v & 0x000F000Fu, u & 0x00F000F0u, v & 0x00F000F0u, qf[nt][g][2 * j + h][0], qf[nt][g][2 * j + h][1], j + h == 0);
           }
-        }
-      }
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         unsigned pairs[GN];
@@ -273,8 +272,8 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              const float t = fmaf(v.x, part[nt][g][2 * k + c], mid * q_sum[nt][g][c]);
-              s[b][nt][2 * k + c] = g == 0 ? t : s[b][nt][2 * k + c] + t;
+              float& t = s[b][nt][2 * k + c];
+              t = fmaf(v.x, part[nt][g][2 * k + c], g == 0 ? mid * q_sum[nt][g][c] : fmaf(mid, q_sum[nt][g][c], t));
             }
         }
       }
@@ -317,6 +316,7 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
 #pragma unroll
           for (int g = 0; g < GN; ++g) {
             mid_acc[nt][g][c] *= corr;
+            eights[nt][g][c] *= corr;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               o[nt][g][j][c] *= corr;
@@ -357,9 +357,11 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
 #pragma unroll
         for (int g = 0; g < GN; ++g)
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
+          for (int c = 0; c < 4; ++c) {
+            eights[nt][g][c] *= ratio;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) o[nt][g][j][c] *= ratio;
+            for (int j = 0; j < 4; ++j) o[nt][g][j][c] *= ratio;
+          }
     }
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
@@ -392,6 +394,10 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
           }
         }
       }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int g = 0; g < GN; ++g) mma_f16(eights[nt][g], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, pf[nt][g][0], pf[nt][g][1]);
       // keys of the contraction: index 2 tig + i of the first half is row tig * 2 + i of the block, of the second half 8 more
 #pragma unroll
       for (int g = 0; g < GN; ++g) {
@@ -404,10 +410,9 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
           unsigned x = __byte_perm(w[0], w[1], half ? 0x7632 : 0x5410), y = __byte_perm(w[2], w[3], half ? 0x7632 : 0x5410);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const unsigned a0 = less(x & 0x000F000Fu, 0x00080008u), a1 = less(x & 0x00F000F0u, 0x00800080u);
-            const unsigned a2 = less(y & 0x000F000Fu, 0x00080008u), a3 = less(y & 0x00F000F0u, 0x00800080u);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][g][2 * half + h], a0, a1, a2, a3, pf[nt][g][0], pf[nt][g][1]);
+            for (int nt = 0; nt < NT; ++nt)
+              mma_f16(o[nt][g][2 * half + h], x & 0x000F000Fu, x & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u, pf[nt][g][0], pf[nt][g][1]);
             x >>= 8;
             y >>= 8;
           }
@@ -416,6 +421,22 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
     }
   };
 
+  // The 8 of (c - 8) comes off the sums now and then: they grow with the keys otherwise, and what they stand for does not.
+  auto settle = [&]() {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int g = 0; g < GN; ++g)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            o[nt][g][j][c] -= eights[nt][g][c];
+            o[nt][g][j][2 + c] = fmaf(-16.f, eights[nt][g][c], o[nt][g][j][2 + c]);
+          }
+          eights[nt][g][c] = 0.f;
+        }
+  };
   // whole blocks, by their number in the warp: [k_lo, k_hi) hide no key from any row
   const int base = key_lo + b0 * PACKED_POS;
   const int k_lo = all_lo > base ? (all_lo - base + TILE - 1) / TILE : 0, k_hi = all_hi - PACKED_POS + 1 >= base ? (all_hi - PACKED_POS + 1 - base) / TILE + 1 : 0;
@@ -425,9 +446,11 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
     const uint8_t* first = ring + half * NB * B::BYTES;
     if (NB * j >= k_lo && NB * j + NB <= min(k_hi, n_blocks)) step_of(std::false_type{}, first, 0, NB);
     else step_of(std::true_type{}, first, base + NB * j * TILE, n_blocks - NB * j);
+    if (j % SETTLE == SETTLE - 1) settle();
     __syncwarp();                      // the half is free
     if (j + HALVES < n_steps) request(j + HALVES);
   }
+  settle();
   turn += n_steps;
   if (failed) atomicExch(p.err, 29);
 
