@@ -29,6 +29,8 @@ namespace {
 constexpr int WARPS = 4;
 constexpr int TILE = WARPS * PACKED_POS;     // keys of a unit
 constexpr int NB = 2;                        // blocks of a step: one running maximum for 32 keys
+constexpr float SLACK = 6.f;                 // a weight is at most 2^SLACK times that of the maximum in use
+constexpr int HEAD = 15 - (int)SLACK;        // p step times its power of two is at most 2^(HEAD + SLACK), within float16
 constexpr int SETTLE = 16;                   // steps after which the sums of codes are centred
 constexpr int HALVES = 2;                    // steps in a warp's ring: one is read while the next arrives
 static_assert(32 % NB == 0, "the blocks of a step lie in one window of 32 blocks, one a lane");
@@ -233,8 +235,9 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
         for (int j = 0; j < 4; ++j) o[nt][g][j][c] = o[nt][g][j][2 + c] = 0.f;
       }
     }
-  float step_limit = 0x1p-100f, v_up = 0x1p114f;       // the largest step seen is at most step_limit = 2^14 / v_up
+  float step_limit = 0x1p-100f, v_up = __uint_as_float((unsigned)(127 + 100 + HEAD) << 23);       // the largest step seen is at most step_limit = 2^HEAD / v_up
 
+  // (m_run: the maximum in use, a score times f_row.)
   // The step's blocks, the first at key0.  MASKED: some key of theirs is hidden from some row or lies behind the last key.
   auto step_of = [&](auto masked, const uint8_t* const first, const int key0, const int n) {
     constexpr bool MASKED = decltype(masked)::value;
@@ -288,48 +291,7 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
           }
       }
     }
-    // ---- the running maximum and sum
-    bool moved = false;
-    float m_use[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float mx = fmaxf(s[0][nt][c], s[0][nt][2 + c]);
-#pragma unroll
-        for (int b = 1; b < NB; ++b) mx = fmaxf(mx, fmaxf(s[b][nt][c], s[b][nt][2 + c]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-        m_use[nt][c] = fmaxf(m_run[nt][c], mx);
-        moved |= m_use[nt][c] != m_run[nt][c];
-      }
-    if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          // (nothing seen so far: the sums are zeros)
-          const float corr = m_run[nt][c] == -INFINITY ? 0.f : exp2_fast((m_run[nt][c] - m_use[nt][c]) * f_row[nt][c]);
-          m_run[nt][c] = m_use[nt][c];
-          l_run[nt][c] *= corr;
-#pragma unroll
-          for (int g = 0; g < GN; ++g) {
-            mid_acc[nt][g][c] *= corr;
-            eights[nt][g][c] *= corr;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              o[nt][g][j][c] *= corr;
-              o[nt][g][j][2 + c] *= corr;
-            }
-          }
-        }
-    }
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) m_use[nt][c] = MASKED && m_run[nt][c] == -INFINITY ? 0.f : -m_run[nt][c] * f_row[nt][c];
-    // ---- values
+    // ---- the values' steps and middles
     float step[NB][GN][2], mid[NB][GN][2], most = 0.f;
 #pragma unroll
     for (int b = 0; b < NB; ++b)
@@ -346,23 +308,78 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
           most = fmaxf(most, v.x);
         }
       }
-    if (__any_sync(0xffffffffu, most > step_limit)) {
-      const unsigned top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
-      const int e = min(127, (int)(top >> 23) - 126);              // top < 2^e
-      const float up = __uint_as_float((unsigned)(127 + 14 - e) << 23), ratio = up / v_up;
-      step_limit = __uint_as_float(min((unsigned)(127 + e), 254u) << 23);
-      v_up = up;
+    // ---- exponents against the maximum in use, which moves only when a score leaves it 2^SLACK behind: a vote in its place
+    // otherwise.  The largest step in use likewise.
+    float x[NB][NT][4], far = -INFINITY;
+    auto exponents = [&]() {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int g = 0; g < GN; ++g)
+        for (int e = 0; e < 4; ++e)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            eights[nt][g][c] *= ratio;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[nt][g][j][c] *= ratio;
+          for (int b = 0; b < NB; ++b) {
+            x[b][nt][e] = fmaf(s[b][nt][e], f_row[nt][e & 1], -m_run[nt][e & 1]);
+            far = fmaxf(far, x[b][nt][e]);
           }
+    };
+    if (!MASKED) exponents();
+    if (MASKED || __any_sync(0xffffffffu, far > SLACK || most > step_limit)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float mx = fmaxf(s[0][nt][c], s[0][nt][2 + c]);
+#pragma unroll
+          for (int b = 1; b < NB; ++b) mx = fmaxf(mx, fmaxf(s[b][nt][c], s[b][nt][2 + c]));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          const float m_new = fmaxf(m_run[nt][c], mx == -INFINITY ? mx : mx * f_row[nt][c]);
+          // (nothing seen so far: the sums are zeros)
+          const float corr = m_run[nt][c] == -INFINITY ? 0.f : exp2_fast(m_run[nt][c] - m_new);
+          m_run[nt][c] = m_new;
+          l_run[nt][c] *= corr;
+#pragma unroll
+          for (int g = 0; g < GN; ++g) {
+            mid_acc[nt][g][c] *= corr;
+            eights[nt][g][c] *= corr;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              o[nt][g][j][c] *= corr;
+              o[nt][g][j][2 + c] *= corr;
+            }
+          }
+        }
+      const unsigned top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
+      if (__uint_as_float(top) > step_limit) {
+        const int e = min(127, (int)(top >> 23) - 126);              // top < 2^e
+        const float up = __uint_as_float((unsigned)(127 + HEAD - e) << 23), ratio = up / v_up;
+        step_limit = __uint_as_float(min((unsigned)(127 + e), 254u) << 23);
+        v_up = up;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int g = 0; g < GN; ++g)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              eights[nt][g][c] *= ratio;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) o[nt][g][j][c] *= ratio;
+            }
+      }
+      if (MASKED) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+              x[b][nt][e] = s[b][nt][e] == -INFINITY ? -INFINITY : fmaf(s[b][nt][e], f_row[nt][e & 1], -m_run[nt][e & 1]);
+      } else {
+        exponents();
+      }
     }
+    // ---- values
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       unsigned pf[NT][GN][2];
@@ -371,8 +388,7 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
         float w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          w[e] = exp2_fast(fmaf(s[b][nt][e], f_row[nt][e & 1], m_use[nt][e & 1]));
-          if (MASKED && s[b][nt][e] == -INFINITY) w[e] = 0.f;      // (f_row may be 0)
+          w[e] = exp2_fast(x[b][nt][e]);
           l_run[nt][e & 1] += w[e];
         }
 #pragma unroll
@@ -380,17 +396,17 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             const float up = step[b][g][k] * v_up;
-            float x0 = w[2 * k] * up, x1 = w[2 * k + 1] * up;
+            float y0 = w[2 * k] * up, y1 = w[2 * k + 1] * up;
             if (MASKED) {              // a key that a row does not see counts for nothing, whatever it holds
-              if (w[2 * k] == 0.f) x0 = 0.f;
-              if (w[2 * k + 1] == 0.f) x1 = 0.f;
+              if (w[2 * k] == 0.f) y0 = 0.f;
+              if (w[2 * k + 1] == 0.f) y1 = 0.f;
               if (w[2 * k] != 0.f) mid_acc[nt][g][0] = fmaf(w[2 * k], mid[b][g][k], mid_acc[nt][g][0]);
               if (w[2 * k + 1] != 0.f) mid_acc[nt][g][1] = fmaf(w[2 * k + 1], mid[b][g][k], mid_acc[nt][g][1]);
             } else {
               mid_acc[nt][g][0] = fmaf(w[2 * k], mid[b][g][k], mid_acc[nt][g][0]);
               mid_acc[nt][g][1] = fmaf(w[2 * k + 1], mid[b][g][k], mid_acc[nt][g][1]);
             }
-            pf[nt][g][k] = transpose8(pack2<__half>(x0, x1));
+            pf[nt][g][k] = transpose8(pack2<__half>(y0, y1));
           }
         }
       }
@@ -473,7 +489,7 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
     for (int c = 0; c < 2; ++c) {
       const int row = 2 * tig + c;
       if (gid == 0) {
-        ml[(warp * 8 + row) * 2] = m_run[nt][c] == -INFINITY ? -INFINITY : m_run[nt][c] * f_row[nt][c];
+        ml[(warp * 8 + row) * 2] = m_run[nt][c];
         ml[(warp * 8 + row) * 2 + 1] = l_run[nt][c];
       }
 #pragma unroll
