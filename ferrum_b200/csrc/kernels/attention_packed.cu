@@ -18,10 +18,11 @@
 // The work is handed out on the device: all (request, KV head, rows of 8 NT, 64 keys) units form one line, and CTA c of P takes the units
 // [c U / P, (c + 1) U / P): the launch does not depend on the lengths, so that a captured one serves any.  A CTA's four warps take every
 // fourth block of 16 positions; a block is one bulk copy into the warp's own ring of stages, and no warp waits for another until
-// its part of a (request, head) is done.  Parts of a (request, head) cut between CTAs meet in a second launch, in a fixed order.
+// its part of a (request, head) is done.  Of the CTAs that share a (request, head) the one that comes last adds up the parts, in a fixed order.
 #include "packed_cache.cuh"
 #include "ptx_sm100.cuh"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace {
@@ -45,7 +46,7 @@ struct PackedParams {
   const int* pos0;
   float* part_o;        // [2 P][PART_ROWS][D]
   float* part_ml;       // [2 P][PART_ROWS][2]
-  int2* part_info;      // [requests * Hkv * 2]: first slot's CTA, number of CTAs that share the rows
+  int* counters;        // [requests * Hkv * 2], zeros before and after: the parts of a (request, head, row tile) that are there
   int* err;
   long long page_stride;
   int ldq, ldo, n_pages, page_size, table_width, Hq, Hkv, G, window, n_reqs;
@@ -120,10 +121,25 @@ __device__ __forceinline__ Span span_of(const PackedParams& p, int r) {
   return Span{lo, (pos + n - lo + TILE - 1) / TILE, (rows + 8 * NT - 1) / (8 * NT)};
 }
 
-// One CTA's share of the units of (request r, KV head kvh, row tile rt): tiles [t0, t1).  slot < 0: that is all of them, the result
-// is written; otherwise the partial goes to the slot.
+// Where the parts of a (request, head, row tile) lie: n CTAs from `cta` on; the first one's is in slot 2 cta + odd, the others' in the even slots
+// of theirs.  n = 1: not cut.
+struct Parts {
+  int cta, n, odd;
+  __device__ __forceinline__ int slot(int i) const { return i == 0 ? 2 * cta + odd : 2 * (cta + i); }
+};
+
+template <typename T>
+__device__ __forceinline__ void write_row4(const PackedParams& p, int token, int head, int D, int d, float4 acc, float L) {
+  const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
+  uint2 r;
+  r.x = pack2<T>(acc.x * inv, acc.y * inv);
+  r.y = pack2<T>(acc.z * inv, acc.w * inv);
+  *reinterpret_cast<uint2*>((T*)p.out + (size_t)token * p.ldo + (size_t)head * D + d) = r;
+}
+
+// One CTA's share of the units of (request r, KV head kvh, row tile rt): tiles [t0, t1).
 template <typename T, int D, int NT>
-__device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kvh, int rt, int key_lo, int t0, int t1, int slot, uint8_t* ring,
+__device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kvh, int rt, int key_lo, int t0, int t1, const Parts parts, uint8_t* ring,
                                             uint32_t bars, uint32_t& turn, float* merge, bool& failed) {
   using B = PackedBlock<D>;
   constexpr int GN = B::GROUPS;
@@ -515,18 +531,59 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
         L += ml[(w * 8 + rr) * 2 + 1] * f;
         acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
       }
-      if (slot < 0) {
-        const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
-        uint2 r2;
-        r2.x = pack2<T>(acc.x * inv, acc.y * inv);
-        r2.y = pack2<T>(acc.z * inv, acc.w * inv);
-        *reinterpret_cast<uint2*>((T*)p.out + (size_t)(qs + row / p.G) * p.ldo + (size_t)(kvh * p.G + row % p.G) * D + d) = r2;
+      if (parts.n == 1) {
+        write_row4<T>(p, qs + row / p.G, kvh * p.G + row % p.G, D, d, acc, L);
       } else {
-        const size_t at = (size_t)slot * PART_ROWS + nt * 8 + rr;
-        *reinterpret_cast<float4*>(p.part_o + at * D + d) = acc;
-        if (d == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(M, L);
+        const size_t at = (size_t)parts.slot((int)blockIdx.x - parts.cta) * PART_ROWS + nt * 8 + rr;
+        __stcg(reinterpret_cast<float4*>(p.part_o + at * D + d), acc);
+        if (d == 0) __stcg(reinterpret_cast<float2*>(p.part_ml + at * 2), make_float2(M, L));
       }
     }
+  }
+  if (parts.n == 1) return;
+  // ---- the last CTA to come adds the parts up
+  __shared__ int s_last;
+  __threadfence();
+  __syncthreads();
+  if (tid == 0) {
+    int* count = p.counters + ((size_t)r * p.Hkv + kvh) * 2 + rt;
+    s_last = atomicAdd(count, 1) == parts.n - 1;
+    if (s_last) *count = 0;
+    __threadfence();
+  }
+  __syncthreads();
+  if (!s_last) return;
+  constexpr int GROUP = 8;             // parts whose loads are in flight together
+  for (int idx = tid; idx < min(8 * NT, n_rows - row0) * (D / 4); idx += WARPS * 32) {
+    const int rr = idx / (D / 4), d = idx % (D / 4) * 4, row = row0 + rr;
+    float M = -INFINITY, L = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = 0; i0 < parts.n; i0 += GROUP) {
+      float2 ml[GROUP];
+      float4 v[GROUP];
+#pragma unroll
+      for (int i = 0; i < GROUP; ++i) {
+        const bool have = i0 + i < parts.n;
+        const size_t at = (size_t)parts.slot(have ? i0 + i : 0) * PART_ROWS + rr;
+        ml[i] = have ? __ldcg(reinterpret_cast<const float2*>(p.part_ml + at * 2)) : make_float2(-INFINITY, 0.f);
+        v[i] = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * D + d));
+      }
+      float m_new = M;
+#pragma unroll
+      for (int i = 0; i < GROUP; ++i) m_new = fmaxf(m_new, ml[i].x);
+      const float keep = M == -INFINITY ? 0.f : exp2f(M - m_new);
+      L *= keep;
+      acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
+#pragma unroll
+      for (int i = 0; i < GROUP; ++i) {
+        if (ml[i].x == -INFINITY && ml[i].y == 0.f) continue;      // (no key of the part was seen by the row)
+        const float f = exp2f(ml[i].x - m_new);
+        L += ml[i].y * f;
+        acc.x += v[i].x * f; acc.y += v[i].y * f; acc.z += v[i].z * f; acc.w += v[i].w * f;
+      }
+      M = m_new;
+    }
+    write_row4<T>(p, qs + row / p.G, kvh * p.G + row % p.G, D, d, acc, L);
   }
 }
 
@@ -546,30 +603,14 @@ attention_packed_kernel(const PackedParams p) {
     for (int s = 0; s < HALVES; ++s) sm100::mbar_init(bars + 8 * s, 1);
   sm100::fence_barrier_init();
   sm100::fence_proxy_async();
-  pdl_launch();
   pdl_wait();
-  // ---- the line's length, then the request in which the CTA's share begins
-  long long U = 0;
-  for (int base = 0; base < p.n_reqs; base += WARPS * 32) {
+  pdl_launch();
+  // ---- the line's length, then the request in which the CTA's share begins (up to 128 requests: one look at their lengths)
+  long long U = 0, mine = 0, at = 0;
+  auto scan = [&](int base) {          // requests base .. base + 127, one a thread: mine, and the units before it in `at`; their sum is added to U
     const int r = base + tid;
     const Span sp = r < p.n_reqs ? span_of<NT>(p, r) : Span{0, 0, 0};
-    long long u = (long long)sp.tiles * sp.row_tiles * p.Hkv;
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) u += __shfl_xor_sync(0xffffffffu, u, d);
-    __syncthreads();
-    if (lane == 0) s_scan[warp] = u;
-    __syncthreads();
-    for (int w = 0; w < WARPS; ++w) U += s_scan[w];
-  }
-  const long long P = min((long long)gridDim.x, U);
-  const long long c = blockIdx.x;
-  if (c >= P) return;
-  const long long first = c * U / P, last = (c + 1) * U / P;
-  long long before = 0;
-  for (int base = 0; base < p.n_reqs; base += WARPS * 32) {
-    const int r = base + tid;
-    const Span sp = r < p.n_reqs ? span_of<NT>(p, r) : Span{0, 0, 0};
-    const long long mine = (long long)sp.tiles * sp.row_tiles * p.Hkv;
+    mine = (long long)sp.tiles * sp.row_tiles * p.Hkv;
     long long u = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -579,17 +620,26 @@ attention_packed_kernel(const PackedParams p) {
     __syncthreads();
     if (lane == 31) s_scan[warp] = u;
     __syncthreads();
-    long long at = before + u - mine;
+    at = U + u - mine;
     for (int w = 0; w < WARPS; ++w) {
       if (w < warp) at += s_scan[w];
-      before += s_scan[w];
+      U += s_scan[w];
     }
+  };
+  for (int base = 0; base < p.n_reqs; base += WARPS * 32) scan(base);
+  const long long P = min((long long)gridDim.x, U), all_units = U;
+  const long long c = blockIdx.x;
+  if (c >= P) return;
+  const long long first = c * all_units / P, last = (c + 1) * all_units / P;
+  if (p.n_reqs > WARPS * 32) U = 0;
+  for (int base = 0; base < p.n_reqs; base += WARPS * 32) {
+    if (p.n_reqs > WARPS * 32) scan(base);
     if (first >= at && first < at + mine) {
-      s_req = r;
+      s_req = base + tid;
       s_start = at;
     }
-    if (before > first) break;
   }
+  U = all_units;
   __syncthreads();
   // ---- walk the share
   uint32_t turn = 0;      // steps that the warp has run: a step's half of the ring and its barrier's phase follow from its number
@@ -603,84 +653,14 @@ attention_packed_kernel(const PackedParams p) {
       const long long pair_start = start + (long long)pair * sp.tiles, pair_end = pair_start + sp.tiles;
       const int t1 = (int)(min(pair_end, last) - pair_start);
       const int kvh = pair / sp.row_tiles, rt = pair % sp.row_tiles;
-      const bool split = t0 > 0 || t1 < sp.tiles;
-      if (tid == 0 && t0 == 0) {
-        // the CTA of the pair's last unit: the largest k with k U / P <= pair_end - 1
-        const int k = (int)((pair_end * P - 1) / U);
-        p.part_info[((size_t)r * p.Hkv + kvh) * 2 + rt] = make_int2((int)c * 2 + (u == first ? 0 : 1), k - (int)c + 1);
-      }
-      packed_item<T, D, NT>(p, r, kvh, rt, sp.lo, t0, t1, split ? (int)c * 2 + (u == first ? 0 : 1) : -1, ring, bars, turn, merge, failed);
+      // the CTAs of the pair's first and last units: the largest k with k U / P <= that unit
+      const int k0 = (int)(((pair_start + 1) * P - 1) / U), k1 = (int)((pair_end * P - 1) / U);
+      const Parts parts{k0, k1 - k0 + 1, k0 * U / P == pair_start ? 0 : 1};
+      packed_item<T, D, NT>(p, r, kvh, rt, sp.lo, t0, t1, parts, ring, bars, turn, merge, failed);
       u = pair_start + t1;
     }
     start += all;
   }
-}
-
-// A block per (request, KV head); its 16 warps share the rows and, with fewer rows, the parts of a row.
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(512)
-packed_merge_kernel(const PackedParams p) {
-  constexpr int E = D / 32;
-  __shared__ float s_acc[16][D];
-  __shared__ float2 s_ml[16];
-  pdl_launch();
-  const int r = blockIdx.x, kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  pdl_wait();
-  const int qs = p.q_start[r], rows = (p.q_start[r + 1] - qs) * p.G;
-  if (rows <= 0 || rows > PACKED_FEW_ROWS) return;
-  const int share = 16 / rows, row = warp % rows, k = warp / rows;      // warps of a row; warps beyond share * rows have none
-  const int2 info = p.part_info[((size_t)r * p.Hkv + kvh) * 2 + row / (8 * NT)];
-  if (rows <= 8 * NT ? info.y <= 1 : (info.y <= 1 && p.part_info[((size_t)r * p.Hkv + kvh) * 2 + 1 - row / (8 * NT)].y <= 1)) return;
-  float M = -INFINITY, L = 0.f, acc[E] = {};
-  if (k < share && info.y > 1) {
-    constexpr int GROUP = 8;      // parts whose loads are in flight together
-    for (int s0 = k * GROUP; s0 < info.y; s0 += share * GROUP) {
-      float m[GROUP], l[GROUP], v[GROUP][E];
-#pragma unroll
-      for (int i = 0; i < GROUP; ++i) {
-        const bool have = s0 + i < info.y;
-        // the first CTA's slot, then the first of each CTA that follows
-        const size_t at = (size_t)(s0 + i == 0 || !have ? info.x : (info.x / 2 + s0 + i) * 2) * PART_ROWS + row % (8 * NT);
-        m[i] = have ? __ldcg(p.part_ml + at * 2) : -INFINITY;
-        l[i] = have ? __ldcg(p.part_ml + at * 2 + 1) : 0.f;
-#pragma unroll
-        for (int e = 0; e < E; ++e) v[i][e] = __ldcg(p.part_o + at * D + lane * E + e);
-      }
-      float m_new = M;
-#pragma unroll
-      for (int i = 0; i < GROUP; ++i) m_new = fmaxf(m_new, m[i]);
-      const float keep = M == -INFINITY ? 0.f : exp2f(M - m_new);
-      L *= keep;
-#pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] *= keep;
-#pragma unroll
-      for (int i = 0; i < GROUP; ++i) {
-        const float f = m[i] == -INFINITY ? 0.f : exp2f(m[i] - m_new);
-        L += l[i] * f;
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (s0 + i < info.y) acc[e] += v[i][e] * f;
-      }
-      M = m_new;
-    }
-  }
-  s_ml[warp] = make_float2(M, L);
-#pragma unroll
-  for (int e = 0; e < E; ++e) s_acc[warp][lane * E + e] = acc[e];
-  __syncthreads();
-  if (k != 0 || info.y <= 1) return;
-  float top = -INFINITY, sum = 0.f, out[E] = {};
-  for (int i = 0; i < share; ++i) top = fmaxf(top, s_ml[row + i * rows].x);
-  for (int i = 0; i < share; ++i) {
-    const float2 ml = s_ml[row + i * rows];
-    const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - top);
-    sum += ml.y * f;
-    for (int e = 0; e < E; ++e) out[e] += s_acc[row + i * rows][lane * E + e] * f;
-  }
-  const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
-  T* dst = (T*)p.out + (size_t)(qs + row / p.G) * p.ldo + (size_t)(kvh * p.G + row % p.G) * D + lane * E;
-#pragma unroll
-  for (int e = 0; e < E; e += 2) reinterpret_cast<unsigned*>(dst)[e / 2] = pack2<T>(out[e] * inv, out[e + 1] * inv);
 }
 
 template <typename T, int D, int NT>
@@ -692,10 +672,11 @@ int launch_packed(const PackedParams& p, cudaStream_t stream) {
     FERRUM_CHECK_ARG(e == cudaSuccess, "attention_packed: cannot reserve %d bytes of shared memory: %s", smem, cudaGetErrorString(e));
     configured = true;
   }
-  launch_kernel(attention_packed_kernel<T, D, NT>, dim3(RESIDENT<D, NT> * ferrum_sm_count()), dim3(WARPS * 32), smem, stream, p);
+  // no more CTAs than the longest requests that the tables can hold have units
+  const long long units = (long long)p.n_reqs * p.Hkv * (NT == 1 ? 2 : 1) * (((long long)p.table_width * p.page_size + TILE - 1) / TILE + 1);
+  const int ctas = (int)std::min<long long>(RESIDENT<D, NT> * ferrum_sm_count(), units);
+  launch_kernel(attention_packed_kernel<T, D, NT>, dim3(ctas), dim3(WARPS * 32), smem, stream, p);
   FERRUM_CHECK_LAUNCH("attention_packed");
-  launch_kernel(packed_merge_kernel<T, D, NT>, dim3(p.n_reqs, p.Hkv), dim3(512), 0, stream, p);
-  FERRUM_CHECK_LAUNCH("attention_packed merge");
   return 0;
 }
 
@@ -705,17 +686,16 @@ int most_ctas() { return MAX_RESIDENT * ferrum_sm_count(); }
 
 FERRUM_API int ferrum_attention_packed_rows() { return PACKED_FEW_ROWS; }
 
-// Floats of workspace that a call needs: the slots of the CTAs' partials, and where the parts of every (request, head, row tile) lie.
-FERRUM_API long long ferrum_attention_packed_workspace(int D, int Hkv, int n_reqs) {
-  return (long long)most_ctas() * 2 * PART_ROWS * (D + 2) + (long long)n_reqs * Hkv * 2 * 2;
-}
+// Floats of workspace that a call needs: two slots a CTA for partials.
+FERRUM_API long long ferrum_attention_packed_workspace(int D) { return (long long)most_ctas() * 2 * PART_ROWS * (D + 2); }
 
-// part: workspace of ferrum_attention_packed_workspace(D, Hkv, n_reqs) floats; calls that may run at the same time need one each.
+// part: workspace of ferrum_attention_packed_workspace(D) floats; counters: n_reqs * Hkv * 2 int32 zeros, which the call leaves zeros.
+// Calls that may run at the same time need one of each for themselves.
 FERRUM_API int ferrum_attention_packed(const void* q, int ldq, void* out, int ldo, int dtype, const void* plane, long long page_stride, int n_pages,
                                        int page_size, const int* block_table, int table_width, const int* q_start, const int* pos0, int n_reqs,
-                                       int n_tokens, float* part, long long part_floats, int Hq, int Hkv, int D, float scale, int window,
+                                       int n_tokens, float* part, long long part_floats, int* counters, int n_counters, int Hq, int Hkv, int D, float scale, int window,
                                        int* err_flag, cudaStream_t stream) {
-  FERRUM_CHECK_ARG(Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && Hkv <= 65535, "attention_packed: bad head counts Hq=%d Hkv=%d", Hq, Hkv);
+  FERRUM_CHECK_ARG(Hq > 0 && Hkv > 0 && Hq % Hkv == 0, "attention_packed: bad head counts Hq=%d Hkv=%d", Hq, Hkv);
   FERRUM_CHECK_ARG(D == 64 || D == 128, "attention_packed: a cache in 4 bits has heads of 64 or 128 elements, found %d", D);
   FERRUM_CHECK_ARG(packed_page_ok(page_size) && table_width > 0 && n_pages > 0 && window >= 0 && n_reqs >= 0 && n_tokens >= 0,
                    "attention_packed: bad sizes (page size %d must be a multiple of %d)", page_size, PACKED_POS);
@@ -723,11 +703,11 @@ FERRUM_API int ferrum_attention_packed(const void* q, int ldq, void* out, int ld
   FERRUM_CHECK_ARG((((uintptr_t)q | (uintptr_t)out | (uintptr_t)plane | (uintptr_t)part) & 15) == 0 && ldq % 8 == 0 && ldo % 8 == 0 && page_stride % 16 == 0,
                    "attention_packed: operands must be 16-byte aligned");
   FERRUM_CHECK_ARG(ldq >= Hq * D && ldo >= Hq * D, "attention_packed: rows of %d and %d elements are too short", ldq, ldo);
-  FERRUM_CHECK_ARG(part_floats >= ferrum_attention_packed_workspace(D, Hkv, n_reqs), "attention_packed: the workspace is too small");
+  FERRUM_CHECK_ARG(part_floats >= ferrum_attention_packed_workspace(D) && n_counters >= (long long)n_reqs * Hkv * 2, "attention_packed: the workspace is too small");
   if (n_reqs == 0 || n_tokens == 0) return 0;
-  const int ctas = most_ctas(), G = Hq / Hkv;
-  float* part_ml = part + (size_t)ctas * 2 * PART_ROWS * D;
-  PackedParams p{q, out, (const uint8_t*)plane, block_table, q_start, pos0, part, part_ml, reinterpret_cast<int2*>(part_ml + (size_t)ctas * 2 * PART_ROWS * 2),
+  const int G = Hq / Hkv;
+  float* part_ml = part + (size_t)most_ctas() * 2 * PART_ROWS * D;
+  PackedParams p{q, out, (const uint8_t*)plane, block_table, q_start, pos0, part, part_ml, counters,
                  err_flag, page_stride, ldq, ldo, n_pages, page_size, table_width, Hq, Hkv, G, window, n_reqs, scale * 1.4426950408889634f};
   // One row tile of 8 where every request brings a token of at most 8 rows (a longer one takes two passes over its keys), else 16 rows
   // in one pass.

@@ -165,6 +165,7 @@ class StepContext:
         self._splitk_counters_side = torch.zeros(4096, dtype=torch.int32, device=device)
         self.lane = 0
         self._side = None
+        self._zeros = {}
         self.step_cache: Dict[object, object] = {}
         self.plan_store = PlanStore(device)
         self.n_tokens = self.n_reqs = self.n_want = 0
@@ -353,6 +354,14 @@ class StepContext:
     # ------------------------------------------------------------------ scratch
     def buf(self, name, shape, dtype):
         return self.scratch.get(name, shape, dtype)
+
+    def zeros(self, name, n):
+        """int32 counters of zeros (at least n) for kernels that leave them zeros."""
+        t = self._zeros.get(name)
+        if t is None or t.numel() < n:
+            t = self._zeros[name] = torch.zeros(max(2 * n, 1024), dtype=torch.int32, device=self.device)
+            self.scratch.generation += 1       # (a captured graph counts in the old ones)
+        return t
 
     def gemm_scratch(self, M, N, K, dual):
         """(float32 workspace, zeroed int32 tile counters) for the tensor-core product."""

@@ -760,6 +760,7 @@ def attention_combine(out, part_o, part_ml, q_start, req_of_token, req_tile0, ti
 
 
 # ----------------------------------------------------------------------------- a cache held in 4 bits
+@functools.lru_cache(maxsize=None)
 def packed_block_bytes(D):
     """Bytes of a block of a cache held in 4 bits: what 16 positions of a KV head of D elements take, keys and values (4.5 bits an
     element); 0 for a head size that such a cache is not built for."""
@@ -769,10 +770,11 @@ def packed_block_bytes(D):
 def _need_packed(plane, page_stride, page_size, Hkv, D, name):
     """The checks of a plane of packed pages, uint8 [pages, Hkv, page_size / 16, bytes of a block]."""
     _need(plane, torch.uint8, "plane", 4)
-    if page_size <= 0 or page_size % 16 or packed_block_bytes(D) == 0:
+    block = packed_block_bytes(D)
+    if page_size <= 0 or page_size % 16 or block == 0:
         raise KernelError(f"{name}: a cache in 4 bits has pages of a multiple of 16 positions and heads of 64 or 128 elements, found {page_size} and {D}")
-    if tuple(plane.shape[1:]) != (Hkv, page_size // 16, packed_block_bytes(D)) or not plane[0].is_contiguous() or page_stride != plane.stride(0):
-        raise KernelError(f"{name}: the plane must be [pages, {Hkv}, {page_size // 16}, {packed_block_bytes(D)}] with dense pages {page_stride} bytes apart")
+    if plane.shape[1:] != (Hkv, page_size // 16, block) or page_stride != plane.stride(0) or not (plane.is_contiguous() or plane[0].is_contiguous()):
+        raise KernelError(f"{name}: the plane must be [pages, {Hkv}, {page_size // 16}, {block}] with dense pages {page_stride} bytes apart")
 
 
 def _need_table(block_table, name):
@@ -822,30 +824,36 @@ def unpack_cache(plane, page_stride, page_size, block_table, items, out, err):
                                      _ptr(items), n, _ptr(out), dtype_code(out.dtype), Hkv, D, _ptr(err), _stream()), "unpack_cache")
 
 
+@functools.lru_cache(maxsize=None)
 def attention_packed_rows():
     """A request is read by `attention_packed` while its tokens x query heads of a KV head are at most this many in the step."""
     return int(lib().ferrum_attention_packed_rows())
 
 
-def attention_packed_workspace(D, Hkv, n_reqs):
+@functools.lru_cache(maxsize=None)
+def attention_packed_workspace(D):
     """float32 elements of the workspace of `attention_packed`."""
-    return int(lib().ferrum_attention_packed_workspace(D, Hkv, n_reqs))
+    return int(lib().ferrum_attention_packed_workspace(D))
 
 
-def attention_packed(q, out, n_tokens, block_table, q_start, pos0, plane, page_stride, page_size, Hq, Hkv, D, scale, window, err, part):
+def attention_packed(q, out, n_tokens, block_table, q_start, pos0, plane, page_stride, page_size, Hq, Hkv, D, scale, window, err, part, counters):
     """Causal grouped-query attention over a cache held in 4 bits, for the requests of the step that bring few rows (decoded tokens, see
     `attention_packed_rows`); the rows of other requests stay as they are.  q_start (int32 [requests + 1]): first token of
     each request; pos0 (int32 [requests]): positions cached before the step, whose own keys must be in the pages already.  part:
-    float32 workspace of `attention_packed_workspace(D, Hkv, requests)` elements; calls that may run at the same time need one each."""
+    float32 workspace of `attention_packed_workspace(D)` elements; counters: int32, requests x Hkv x 2 zeros, which the call leaves
+    zeros.  Calls that may run at the same time need one of each for themselves."""
     _need16(q, "q", 2); _need16(out, "out", 2, like=q); _need(q_start, torch.int32, "q_start", 1); _need(pos0, torch.int32, "pos0", 1)
     _need_table(block_table, "attention_packed"); _need_packed(plane, page_stride, page_size, Hkv, D, "attention_packed")
-    _need(part, torch.float32, "part", 1)
+    _need(part, torch.float32, "part", 1); _need(counters, torch.int32, "counters", 1)
     n_reqs = pos0.shape[0]
     if q_start.shape[0] != n_reqs + 1 or block_table.shape[0] < n_reqs or min(q.shape[0], out.shape[0]) < n_tokens:
         raise KernelError("attention_packed: q_start, pos0, block_table and the rows do not agree")
+    if not (q_start.is_contiguous() and pos0.is_contiguous() and part.is_contiguous() and counters.is_contiguous()):
+        raise KernelError("attention_packed: q_start, pos0, part and counters must be contiguous")
     _check(lib().ferrum_attention_packed(_ptr(q), q.stride(0), _ptr(out), out.stride(0), dtype_code(q.dtype), _ptr(plane), c_longlong(page_stride),
                                          plane.shape[0], page_size, _ptr(block_table), block_table.shape[1], _ptr(q_start), _ptr(pos0), n_reqs,
-                                         n_tokens, _ptr(part), c_longlong(part.numel()), Hq, Hkv, D, c_float(scale), window, _ptr(err), _stream()),
+                                         n_tokens, _ptr(part), c_longlong(part.numel()), _ptr(counters), counters.numel(), Hq, Hkv, D, c_float(scale),
+                                         window, _ptr(err), _stream()),
            "attention_packed")
 
 

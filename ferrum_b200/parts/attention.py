@@ -118,17 +118,16 @@ class PagedAttention(Mixer):
         """Over a cache held in 4 bits: decoded tokens from the packed pages; for prompt portions the pages they see are unpacked
         into a scratch plane, which the kernels of prompt portions then read in the cache's place."""
         Hq, Hkv, D = self.Hq, self.Hkv, self.D
-        few = ops.attention_packed_rows()
-        rows = [n * (Hq // Hkv) for n in ctx.h_q_len]
-        if min(rows) <= few:
-            part = ctx.buf("attn_packed_part", (ops.attention_packed_workspace(D, Hkv, ctx.n_reqs),), torch.float32)
+        few, G = ops.attention_packed_rows(), Hq // Hkv
+        if min(ctx.h_q_len) * G <= few:
+            part = ctx.buf("attn_packed_part", (ops.attention_packed_workspace(D),), torch.float32)
             if ops.profiling():      # (a step with prompt portions counts the whole step's work for each kernel)
                 ops.set_work(ops.attention_work(ctx, Hq, Hkv, D, self.window, 9 / 16))
             ops.attention_packed(qkv, out, ctx.n_tokens, table, ctx.q_start, ctx.pos0, cache.plane, cache.page_stride, cache.page_size,
-                                 Hq, Hkv, D, self.scale, self.window, ctx.err, part)
-        if max(rows) <= few:
+                                 Hq, Hkv, D, self.scale, self.window, ctx.err, part, ctx.zeros("attn_packed_counters", 2 * ctx.n_reqs * Hkv))
+        if ctx.max_q_len * G <= few:
             return
-        items, pages = attention_plan.unpack_plan(ctx, cache.group, Hq // Hkv, self.window, cache.page_size, few)
+        items, pages = attention_plan.unpack_plan(ctx, cache.group, G, self.window, cache.page_size, few)
         n, whole = items.shape[0], cache.plane.shape[0]
         plane = ctx.scratch.get("attn_unpacked", (n, 2, Hkv, cache.page_size, D), self.dtype, limit=cache.plane[0].numel() // (18 * D) * 32 * D * whole,
                                 captured=False)

@@ -87,14 +87,14 @@ def test_wrappers_refuse_what_the_kernels_are_not_built_for():
     with pytest.raises(KernelError, match="CUDA tensor"):
         ops.rope_cache_write_packed(cpu, 4, i32, i32, i32.view(2, 2), None, plane, 1152, 16, 2, 1, 64, 0, 0, i32)
     with pytest.raises(KernelError, match="CUDA tensor"):
-        ops.attention_packed(cpu, cpu, 1, i32.view(2, 2), i32, i32, plane, 1152, 16, 2, 1, 64, 1.0, 0, i32, torch.zeros(1))
+        ops.attention_packed(cpu, cpu, 1, i32.view(2, 2), i32, i32, plane, 1152, 16, 2, 1, 64, 1.0, 0, i32, torch.zeros(1), i32)
     lib = ops.lib()
     null = None
     # the library's own checks come before any launch
-    assert lib.ferrum_attention_packed(null, 512, null, 512, ops.BF16, null, 1152, 2, 24, null, 4, null, null, 1, 1, null, ops.c_longlong(1 << 40), 2, 1, 64,
+    assert lib.ferrum_attention_packed(null, 512, null, 512, ops.BF16, null, 1152, 2, 24, null, 4, null, null, 1, 1, null, ops.c_longlong(1 << 40), null, 99, 2, 1, 64,
                                        ops.c_float(1.0), 0, ops.c_void_p(16), null) == 1
     assert b"multiple of 16" in lib.ferrum_last_error()
-    assert lib.ferrum_attention_packed(null, 512, null, 512, ops.BF16, null, 1152, 2, 16, null, 4, null, null, 1, 1, null, ops.c_longlong(1 << 40), 2, 1, 96,
+    assert lib.ferrum_attention_packed(null, 512, null, 512, ops.BF16, null, 1152, 2, 16, null, 4, null, null, 1, 1, null, ops.c_longlong(1 << 40), null, 99, 2, 1, 96,
                                        ops.c_float(1.0), 0, ops.c_void_p(16), null) == 1
     assert b"64 or 128" in lib.ferrum_last_error()
     assert lib.ferrum_unpack_cache(null, 1152, 2, 16, null, 4, null, 1, null, ops.F32, 1, 64, ops.c_void_p(16), null) == 1

@@ -193,9 +193,9 @@ def test_rows_of_other_requests_and_wider_rows(cuda):
     s = H.Step(c, [1, 50, 4], 8, 9, extra_columns=24)
     s.qkv[:, -24:] = float("nan")
     out = torch.full((60, 8 * 64 + 8), 3, dtype=torch.bfloat16, device="cuda")
-    part = torch.empty(ops.attention_packed_workspace(64, 2, 3), device="cuda")
-    ops.attention_packed(s.qkv, out, 55, s.ctx.block_tables[0], s.ctx.q_start, s.ctx.pos0, c.plane, c.plane.stride(0), 16, 8, 2, 64, 0.125, 0, s.ctx.err, part)
-    assert s.ctx.err.item() == 0 and bool((out[1:51] == 3).all()) and bool((out[55:] == 3).all()) and bool((out[:, 512:] == 3).all())
+    part, counters = torch.empty(ops.attention_packed_workspace(64), device="cuda"), torch.zeros(12, dtype=torch.int32, device="cuda")
+    ops.attention_packed(s.qkv, out, 55, s.ctx.block_tables[0], s.ctx.q_start, s.ctx.pos0, c.plane, c.plane.stride(0), 16, 8, 2, 64, 0.125, 0, s.ctx.err, part, counters)
+    assert s.ctx.err.item() == 0 and not counters.any() and bool((out[1:51] == 3).all()) and bool((out[55:] == 3).all()) and bool((out[:, 512:] == 3).all())
     want = s.attend()
     for rows in (slice(0, 1), slice(51, 55)):
         assert torch.equal(out[rows, :512], want[rows])
