@@ -553,7 +553,7 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
   }
   __syncthreads();
   if (!s_last) return;
-  constexpr int GROUP = 8;             // parts whose loads are in flight together
+  constexpr int GROUP = 16;            // parts whose loads are in flight together
   for (int idx = tid; idx < min(8 * NT, n_rows - row0) * (D / 4); idx += WARPS * 32) {
     const int rr = idx / (D / 4), d = idx % (D / 4) * 4, row = row0 + rr;
     float M = -INFINITY, L = 0.f;
