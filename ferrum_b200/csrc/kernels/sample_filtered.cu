@@ -1,20 +1,30 @@
 // Next-token draw from given random numbers: temperature, top-k, top-p and min-p, in this order.
 //
-// Of a row x of logits, with z_i = (x_i - max) / T and w_i = exp(z_i) in 64 bits (NaN logits are left out):
+// Of a row x of logits, with z_i = (x_i - max) / T and w_i = exp(z_i) (NaN logits are left out):
 //   top-k   the k largest stay (of equal ones the lower index)
 //   top-p   in that order a token stays while the mass of the tokens before it is below p times the mass that top-k left
 //   min-p   a token stays if w_i >= min_p (the largest w is 1)
 //   draw    the first token in index order at which the running mass of those that stay exceeds u times their whole mass
-// T = 0 takes the largest logit.  Masses are whole numbers, w_i rounded to 2^-s with s = 62 - ceil(log2 V): their sums are exact whatever
-// their order, and 2^-s (2^-45 at 128 Ki tokens) is far below what a draw's 53 random bits can tell from 0.
+// T = 0 takes the largest logit.  Masses are whole numbers, w_i rounded to 2^-s with s = min(45, 62 - ceil(log2 V)): their sums are exact
+// whatever their order, and 2^-45 is far below what a row's sum of 32-bit weights could tell apart.
 //
-// Simplest form: a block per row; every threshold by bisection over the logits' bits as ordered integers, a pass over the row each.
+// A cluster of CTAs holds a row's logits in its shared memory, as integers of the same order, and reads them from there as often as it
+// takes.  Where top-k or top-p cuts is found by histograms: 2,048 bins of equal width below the maximum, then the range of keys in the
+// bin that holds the cut, cut into 2,048 again, until that bin holds a single key (one or two histograms for logits of any real
+// model, four at most).  Each CTA counts its slice; of the bins' sums over the cluster each CTA makes its share.  Of equal keys at the
+// cut the first in index order stay: a threshold is a key and an index.
+//
 // The reference samples greedily only (crates/core-types/src/model.rs:44-62).
 #include "common.cuh"
 
 namespace {
 
 typedef unsigned long long u64;
+
+constexpr int BINS = 2048;
+constexpr int MAX_CLUSTER = 8;
+constexpr int THREADS = 512;
+constexpr int SEGMENTS = 8;         // parts of a warp's range whose masses are kept for the draw
 
 // Order-preserving integer of a logit; 0 stands for NaN, which comes after everything and is never kept.
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -35,164 +45,411 @@ struct FilterParams {
   int* out_ids;
   int* also_to;
   int* err;
-  int ld, V, shift;
+  int ld, V, per, shift;            // per: logits of a CTA's slice
 };
 
-__device__ __forceinline__ u64 block_sum64(u64 v, u64* red) {
+// A token stays while (key, index) comes no later than the threshold: larger keys first, then lower indices.
+struct Cut {
+  uint32_t key;
+  int index;
+  __device__ __forceinline__ bool stays(uint32_t k, int i) const { return k > key || (k == key && i <= index); }
+};
+
+__device__ __forceinline__ uint32_t peer(uint32_t local, int rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(local), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ u64 load_peer(uint32_t addr) {
+  u64 v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void store_peer(uint32_t addr, u64 v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory"); }
+__device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+struct Shared {
+  u64 hist[BINS];
+  u64 exchange[4][2][MAX_CLUSTER];
+  u64 warp[THREADS / 32][2];
+  u64 segment[THREADS / 32][SEGMENTS];
+  u64 found[2];
+  double powers[64];                // 2^(j / 64)
+};
+
+// The CTA's view of its row.
+template <bool RESIDENT>
+struct Row {
+  const FilterParams& p;
+  Shared& sh;
+  const uint32_t* keys;             // the slice in shared memory, or
+  const float* row;                 // in global memory
+  int rank, n_ctas, lo, n;          // the slice: logits lo .. lo + n - 1
+  int turn;                         // exchanges so far
+  uint32_t best;
+  float top;
+  double inv_t;
+
+  __device__ __forceinline__ uint32_t key(int i) const { return RESIDENT ? keys[i] : order_key(row[lo + i]); }
+
+  // w * 2^shift of a key, not rounded.  exp by 2^(n / 64) from a table and the series of the rest (below 2^-7 in size: the sixth term is
+  // 3e-17 of the sum); what is below 2^-1 after the scaling rounds to 0 whatever its value.
+  __device__ __forceinline__ double scaled_weight(uint32_t k) const {
+    if (k == best) return (double)(1ull << p.shift);
+    const double y = ((double)key_value(k) - (double)top) * inv_t * 92.332482616893656877;      // 64 log2(e)
+    if (!(y > -3000.0)) return 0.0;
+    const double t = y + 6755399441055744.0;                       // 1.5 * 2^52: the nearest whole number in the low bits
+    const int n = __double2loint(t);
+    const double q = (y - (t - 6755399441055744.0)) * 0.010830424696249145347;               // ln(2) / 64
+    const double s = fma(q, fma(q, fma(q, fma(q, fma(q, 1.0 / 120.0, 1.0 / 24.0), 1.0 / 6.0), 0.5), 1.0), 1.0);
+    const double v = sh.powers[n & 63] * s;
+    return __hiloint2double(__double2hiint(v) + (((n >> 6) + p.shift) << 20), __double2loint(v));
+  }
+  static __device__ __forceinline__ u64 whole(double v) { return (u64)__double_as_longlong(v + 4503599627370496.0) & 0xfffffffffffffull; }      // (v below 2^51)
+  __device__ __forceinline__ u64 mass(uint32_t k) const { return whole(scaled_weight(k)); }
+
+  // Sums (or maxima of) two numbers over the block, then hands them to every CTA; afterwards exchange[..][0 or 1][c] holds CTA c's.
+  template <bool MAXIMA>
+  __device__ __forceinline__ const u64 (&gather(u64 a, u64 b))[2][MAX_CLUSTER] {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  u64 t = 0;
-  for (int i = 0; i < (int)(blockDim.x >> 5); ++i) t += red[i];
-  return t;
-}
+    for (int o = 16; o > 0; o >>= 1) {
+      const u64 x = __shfl_xor_sync(0xffffffffu, a, o), y = __shfl_xor_sync(0xffffffffu, b, o);
+      a = MAXIMA ? max(a, x) : a + x;
+      b = MAXIMA ? max(b, y) : b + y;
+    }
+    __syncthreads();
+    if (lane == 0) sh.warp[warp][0] = a, sh.warp[warp][1] = b;
+    __syncthreads();
+    u64(&ex)[2][MAX_CLUSTER] = sh.exchange[turn++ & 3];
+    if (warp == 0) {
+      a = lane < (int)(blockDim.x >> 5) ? sh.warp[lane][0] : 0;
+      b = lane < (int)(blockDim.x >> 5) ? sh.warp[lane][1] : 0;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const u64 x = __shfl_xor_sync(0xffffffffu, a, o), y = __shfl_xor_sync(0xffffffffu, b, o);
+        a = MAXIMA ? max(a, x) : a + x;
+        b = MAXIMA ? max(b, y) : b + y;
+      }
+      if (lane < n_ctas) {
+        store_peer(peer((uint32_t)__cvta_generic_to_shared(&ex[0][rank]), lane), a);
+        store_peer(peer((uint32_t)__cvta_generic_to_shared(&ex[1][rank]), lane), b);
+      }
+    }
+    cluster_sync();
+    return ex;
+  }
+  // One thread of one CTA tells every CTA two numbers (the others pass `mine` false).
+  __device__ __forceinline__ void tell(bool mine, u64 a, u64 b) {
+    u64(&ex)[2][MAX_CLUSTER] = sh.exchange[turn++ & 3];
+    if (mine)
+      for (int c = 0; c < n_ctas; ++c) {
+        store_peer(peer((uint32_t)__cvta_generic_to_shared(&ex[0][0]), c), a);
+        store_peer(peer((uint32_t)__cvta_generic_to_shared(&ex[1][0]), c), b);
+      }
+    cluster_sync();
+    __syncthreads();
+    if (threadIdx.x == 0) sh.found[0] = ex[0][0], sh.found[1] = ex[1][0];
+    __syncthreads();
+  }
 
-__device__ __forceinline__ double weight(uint32_t key, float top, float T) {
-  const float x = key_value(key);
-  return x == top ? 1.0 : exp(((double)x - (double)top) / (double)T);
-}
-__device__ __forceinline__ u64 mass_of(double w, int shift) { return __double2ull_rn(w * (double)(1ull << shift)); }
+  // Where `limit` cuts: of the tokens that `cut` lets stay, ordered, a token stays while the sum of what comes before it is below the limit;
+  // a token counts 1 or (MASS) its mass.  lo_key, hi_key: the smallest and largest key that count.
+  template <bool MASS>
+  __device__ __forceinline__ Cut find(const Cut cut, double limit, uint32_t lo_key, uint32_t hi_key, float range) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+    u64 before = 0;
+    // the first histogram's bins are of equal width below the maximum, where that is a finite number
+    bool linear = isfinite(top) && isfinite(range);
+    const float scale = (float)BINS / range;
+    while (lo_key != hi_key) {
+      const int bits = 32 - __clz(hi_key - lo_key), down = max(0, bits - 11);
+      auto bin_of = [&](uint32_t k) {
+        if (!linear) return (int)((hi_key - k) >> down);
+        return min(BINS - 1, (int)((top - key_value(k)) * scale));
+      };
+      for (int i = tid; i < BINS; i += blockDim.x) sh.hist[i] = 0;
+      __syncthreads();
+      for (int i = tid; i < n; i += blockDim.x) {
+        const uint32_t k = key(i);
+        if (k < lo_key || k > hi_key || !cut.stays(k, lo + i)) continue;
+        const u64 v = MASS ? mass(k) : 1;
+        if (v) atomicAdd(&sh.hist[bin_of(k)], v);
+      }
+      cluster_sync();
+      // the CTA's share of the bins, BINS / n_ctas of them in the first threads: their sums over the cluster, and how they run
+      const int share = BINS / n_ctas;
+      u64 mine[BINS / THREADS] = {}, run = 0;
+      const int each = max(1, share / (int)blockDim.x), b0 = rank * share + tid * each;
+      const bool has = tid * each < share;
+      if (has)
+        for (int j = 0; j < each; ++j) {
+          for (int c = 0; c < n_ctas; ++c) mine[j] += load_peer(peer((uint32_t)__cvta_generic_to_shared(&sh.hist[b0 + j]), c));
+          run += mine[j];
+        }
+      const u64 own = run;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const u64 v = __shfl_up_sync(0xffffffffu, run, o);
+        if (lane >= o) run += v;
+      }
+      const u64(&ex)[2][MAX_CLUSTER] = gather<false>(own, 0);
+      // (gather's sums went over sh.warp; the warps' own totals for the running sums follow in it)
+      __syncthreads();
+      if (lane == 31) sh.warp[warp][0] = run;
+      __syncthreads();
+      u64 at = before + run - own;
+      for (int c = 0; c < rank; ++c) at += ex[0][c];
+      for (int w = 0; w < warp; ++w) at += sh.warp[w][0];
+      // the last bin with something in it whose predecessors stay below the limit
+      u64 best_bin = 0, best_at = 0;
+      if (has)
+        for (int j = 0; j < each; ++j) {
+          if (mine[j] && (double)at < limit) best_bin = b0 + j + 1, best_at = at;
+          at += mine[j];
+        }
+      // bins and their sums rise together: the largest of each belong together
+      const u64(&e2)[2][MAX_CLUSTER] = gather<true>(best_bin, best_at);
+      u64 bin = 0;
+      before = 0;
+      for (int c = 0; c < n_ctas; ++c) bin = max(bin, e2[0][c]), before = max(before, e2[1][c]);
+      // the keys in that bin: their range, for the next histogram
+      u64 a = 0, b = 0;             // maximum of ~key and of key
+      for (int i = tid; i < n; i += blockDim.x) {
+        const uint32_t k = key(i);
+        if (k < lo_key || k > hi_key || bin_of(k) != (int)bin - 1 || !cut.stays(k, lo + i)) continue;
+        if (MASS && !mass(k)) continue;
+        a = max(a, (u64)(uint32_t)~k);
+        b = max(b, (u64)k);
+      }
+      const u64(&e3)[2][MAX_CLUSTER] = gather<true>(a, b);
+      a = b = 0;
+      for (int c = 0; c < n_ctas; ++c) a = max(a, e3[0][c]), b = max(b, e3[1][c]);
+      lo_key = ~(uint32_t)a;
+      hi_key = (uint32_t)b;
+      linear = false;
+    }
+    // of the tokens equal to the key at the cut the i-th stays if before + i * one < limit
+    const u64 one = MASS ? mass(lo_key) : 1;
+    u64 stay = (u64)ceil(fmax(0.0, limit - (double)before) / (double)max(one, 1ull));
+    while (stay > 0 && (double)(before + (stay - 1) * one) >= limit) --stay;
+    return first_of(lo_key, cut, max(stay, 1ull));
+  }
 
-__global__ void __launch_bounds__(1024)
+  // The cut behind the stay-th token (counted from 1, in index order) with this key that `cut` lets stay.
+  __device__ __forceinline__ Cut first_of(uint32_t key_at, const Cut cut, u64 stay) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const int rows = (n + 31) / 32, r0 = (int)((long long)warp * rows / warps), r1 = (int)((long long)(warp + 1) * rows / warps);
+    u64 count = 0;
+    for (int r = r0; r < r1; ++r) {
+      const int i = r * 32 + lane;
+      count += i < n && key(i) == key_at && cut.stays(key_at, lo + i);
+    }
+    u64 total = count;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    const u64(&ex)[2][MAX_CLUSTER] = gather<false>(count, 0);
+    u64 all = 0, ahead = 0;
+    for (int c = 0; c < n_ctas; ++c) {
+      if (c < rank) ahead += ex[0][c];
+      all += ex[0][c];
+    }
+    if (stay >= all) return Cut{key_at, cut.key == key_at ? cut.index : 0x7fffffff};
+    __syncthreads();
+    if (lane == 0) sh.warp[warp][0] = total;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) ahead += sh.warp[w][0];
+    bool mine = false;
+    int index = 0;
+    if (ahead < stay && stay <= ahead + total)
+      for (int r = r0; r < r1; ++r) {
+        const int i = r * 32 + lane;
+        const unsigned hit = __ballot_sync(0xffffffffu, i < n && key(i) == key_at && cut.stays(key_at, lo + i));
+        const u64 here = __popc(hit);
+        if (ahead + here >= stay) {
+          const int nth = (int)(stay - ahead);      // the nth set bit of hit
+          mine = (hit >> lane & 1) && __popc(hit & ((2u << lane) - 1)) == nth;
+          index = lo + i;
+          break;
+        }
+        ahead += here;
+      }
+    tell(mine, (u64)index, 0);
+    return Cut{key_at, (int)sh.found[0]};
+  }
+
+  // The draw from the tokens that the cut lets stay and that weigh min_w at least.
+  __device__ __forceinline__ void draw(const Cut cut, double min_w, double u, int out) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const int rows = (n + 31) / 32, r0 = (int)((long long)warp * rows / warps), r1 = (int)((long long)(warp + 1) * rows / warps);
+    auto mass_at = [&](int r) -> u64 {
+      const int i = r * 32 + lane;
+      const uint32_t k = i < n ? key(i) : 0;
+      if (k == 0 || !cut.stays(k, lo + i)) return 0;
+      const double v = scaled_weight(k);
+      return v >= min_w ? whole(v) : 0;
+    };
+    u64 sum = 0;
+    for (int s = 0; s < SEGMENTS; ++s) {
+      u64 part = 0;
+      for (int r = r0 + (r1 - r0) * s / SEGMENTS; r < r0 + (r1 - r0) * (s + 1) / SEGMENTS; ++r) part += mass_at(r);
+      sum += part;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+      if (lane == 0) sh.segment[warp][s] = part;
+    }
+    const u64(&ex)[2][MAX_CLUSTER] = gather<false>(sum, 0);
+    u64 all = 0, at = 0;
+    for (int c = 0; c < n_ctas; ++c) {
+      if (c < rank) at += ex[0][c];
+      all += ex[0][c];
+    }
+    const double x = u > 0.0 ? u * (double)all : 0.0;
+    const u64 threshold = x >= (double)all ? all - 1 : min((u64)x, all - 1);
+    if (threshold < at || threshold >= at + ex[0][rank]) return;
+    for (int w = 0; w < warp; ++w)
+      for (int s = 0; s < SEGMENTS; ++s) at += sh.segment[w][s];
+    for (int s = 0; s < SEGMENTS; ++s) {
+      const u64 part = sh.segment[warp][s];
+      if (threshold >= at && threshold < at + part) {
+        for (int r = r0 + (r1 - r0) * s / SEGMENTS; r < r0 + (r1 - r0) * (s + 1) / SEGMENTS; ++r) {
+          const u64 own = mass_at(r);
+          u64 run = own;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const u64 v = __shfl_up_sync(0xffffffffu, run, o);
+            if (lane >= o) run += v;
+          }
+          if (threshold >= at + run - own && threshold < at + run) {
+            p.out_ids[out] = lo + r * 32 + lane;
+            if (p.also_to) p.also_to[out] = lo + r * 32 + lane;
+          }
+          at += __shfl_sync(0xffffffffu, run, 31);
+        }
+        return;
+      }
+      at += part;
+    }
+  }
+};
+
+template <bool RESIDENT>
+__global__ void __launch_bounds__(THREADS)
 sample_filtered_kernel(const FilterParams p) {
-  __shared__ u64 red[32];
-  __shared__ int s_id;
-  __shared__ u64 s_run[3];
-  pdl_launch();
+  extern __shared__ __align__(16) uint32_t slice[];
+  __shared__ Shared sh;
+  const int tid = threadIdx.x;
+  if (tid < 64) sh.powers[tid] = exp2((double)tid / 64.0);
+  // a CTA's shared memory may be written by a peer only once the CTA is known to run
+  cluster_sync();
   pdl_wait();
-  const int r = p.rows ? p.rows[blockIdx.x] : blockIdx.x, tid = threadIdx.x, V = p.V;
+  pdl_launch();
+  const int q = blockIdx.x, r = p.rows ? p.rows[q] : q, rank = blockIdx.y;
   const float* row = p.logits + (size_t)r * p.ld;
-  const float T = p.temperature[blockIdx.x], top_p = p.top_p ? p.top_p[blockIdx.x] : 1.f, min_p = p.min_p ? p.min_p[blockIdx.x] : 0.f;
-  const int top_k = p.top_k ? p.top_k[blockIdx.x] : 0;
-  auto finish = [&](int id, int code) {
-    if (tid == 0) {
-      p.out_ids[r] = id;
-      if (p.also_to) p.also_to[r] = id;
-      if (code) atomicExch(p.err, code);
+  const float T = p.temperature[q], top_p = p.top_p ? p.top_p[q] : 1.f, min_p = p.min_p ? p.min_p[q] : 0.f;
+  const int top_k = p.top_k ? p.top_k[q] : 0, lo = min(p.V, rank * p.per), n = min(p.V, lo + p.per) - lo;
+  auto refuse = [&](int code) {
+    if (tid == 0 && rank == 0) {
+      p.out_ids[r] = -1;
+      if (p.also_to) p.also_to[r] = -1;
+      atomicExch(p.err, code);
     }
   };
-  if (!(T >= 0.f) || T == INFINITY || !(top_p > 0.f) || !(min_p <= 1.f)) {      // (the same for the whole block)
-    finish(-1, 7);
+  if (!(T >= 0.f) || T == INFINITY || !(top_p > 0.f) || !(min_p <= 1.f)) {      // (the same for the whole cluster)
+    refuse(7);
     return;
   }
-  uint32_t best = 0;
-  for (int i = tid; i < V; i += blockDim.x) best = max(best, order_key(row[i]));
-  for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-  __syncthreads();
-  if ((tid & 31) == 0) red[tid >> 5] = best;
-  __syncthreads();
-  for (int i = 0; i < (int)(blockDim.x >> 5); ++i) best = max(best, (uint32_t)red[i]);
-  if (best == 0) {
-    finish(-1, 6);
+  // ---- the slice, its largest key and its smallest (of any logit, and of the finite ones)
+  uint32_t most = 0, least = ~0u, least_finite = ~0u;
+  for (int i = tid; i < n; i += blockDim.x) {
+    const uint32_t k = order_key(row[lo + i]);
+    if (RESIDENT) slice[i] = k;
+    most = max(most, k);
+    if (k) least = min(least, k);
+    if (k > 0x007fffffu) least_finite = min(least_finite, k);      // (0x007fffff: minus infinity)
+  }
+  Row<RESIDENT> w{p, sh, slice, row, rank, (int)gridDim.y, lo, n, 0, 0, 0.f, 0.0};
+  const u64(&ex)[2][MAX_CLUSTER] = w.template gather<true>(most, (uint32_t)~least_finite);
+  for (int c = 0; c < w.n_ctas; ++c) {
+    w.best = max(w.best, (uint32_t)ex[0][c]);
+    least_finite = min(least_finite, ~(uint32_t)ex[1][c]);
+  }
+  if (w.best == 0) {
+    refuse(6);
     return;
   }
-  const float top = key_value(best);
-  auto count_from = [&](uint32_t key) {
-    u64 n = 0;
-    for (int i = tid; i < V; i += blockDim.x) n += order_key(row[i]) >= key;
-    return block_sum64(n, red);
-  };
-  uint32_t t_key = 1;          // tokens above t_key stay, of those equal to it the first `ties`
-  u64 ties = ~0ull;
+  w.top = key_value(w.best);
+  Cut cut{1, 0x7fffffff};
   if (T == 0.f) {
-    t_key = best;
-    ties = 1;
-  } else if (top_k > 0 && top_k < V) {
-    uint32_t lo = 1, hi = best;      // the largest key that at least top_k tokens reach, or 1
-    while (lo < hi) {
-      const uint32_t mid = lo + (hi - lo + 1) / 2;
-      if (count_from(mid) >= (u64)top_k) lo = mid; else hi = mid - 1;
-    }
-    t_key = lo;
-    const u64 above = t_key == 0xffffffffu ? 0 : count_from(t_key + 1);
-    ties = (u64)top_k > above ? (u64)top_k - above : 0;
+    cut = w.first_of(w.best, cut, 1);
+    w.draw(Cut{w.best, cut.index}, 0.0, 0.0, r);
+    cluster_sync();
+    return;
   }
-  const float Tw = T == 0.f ? 1.f : T;
-  auto mass_above = [&](uint32_t key) {       // tokens that stay so far with a key above `key`
-    u64 m = 0, n = 0;
-    for (int i = tid; i < V; i += blockDim.x) {
-      const uint32_t k = order_key(row[i]);
-      if (k > key && k > t_key) m += mass_of(weight(k, top, Tw), p.shift);
-      if (k > key && k == t_key) ++n;
-    }
-    m = block_sum64(m, red);
-    n = block_sum64(n, red);
-    return m + min(n, ties) * mass_of(weight(t_key, top, Tw), p.shift);
-  };
-  if (T > 0.f && top_p < 1.f) {
-    const double target = (double)top_p * (double)mass_above(t_key - 1);
-    uint32_t lo = t_key, hi = best;          // the smallest key whose tokens above weigh less than the target
-    while (lo < hi) {
-      const uint32_t mid = lo + (hi - lo) / 2;
-      if ((double)mass_above(mid) < target) hi = mid; else lo = mid + 1;
-    }
-    const u64 before = mass_above(lo), each = mass_of(weight(lo, top, Tw), p.shift);
-    // of the tokens at the border the i-th stays if before + i * each < target
-    u64 stay = ~0ull;
-    if (each > 0) {
-      const double room = target - (double)before;
-      stay = (u64)ceil(room / (double)each);
-      while (stay > 0 && (double)(before + (stay - 1) * each) >= target) --stay;
-      while ((double)(before + stay * each) < target) ++stay;
-    }
-    ties = lo == t_key ? min(ties, stay) : stay;
-    t_key = lo;
+  w.inv_t = 1.0 / (double)T;
+  if (top_k > 0 && top_k < p.V) {
+    const u64(&ea)[2][MAX_CLUSTER] = w.template gather<true>((uint32_t)~least, 0);
+    for (int c = 0; c < w.n_ctas; ++c) least = min(least, ~(uint32_t)ea[0][c]);
+    cut = w.template find<false>(cut, (double)top_k, least, w.best, least_finite == ~0u ? INFINITY : w.top - key_value(least_finite));
   }
-  // the whole mass, then the draw: both in index order, a tile of blockDim tokens at a time
-  const int lane = tid & 31, warp = tid >> 5;
-  u64 threshold = 0;
-  for (int pass = 0; pass < 2; ++pass) {
-    u64 run_mass = 0, run_ties = 0;
-    if (tid == 0) s_id = V;
-    for (int base = 0; base < V; base += blockDim.x) {
-      const uint32_t k = base + tid < V ? order_key(row[base + tid]) : 0;
-      u64 t = k == t_key;
-      for (int o = 1; o < 32; o <<= 1) {
-        const u64 v = __shfl_up_sync(0xffffffffu, t, o);
-        if (lane >= o) t += v;
-      }
-      __syncthreads();
-      if (lane == 31) red[warp] = t;
-      __syncthreads();
-      u64 before = run_ties, all = run_ties;
-      for (int i = 0; i < (int)(blockDim.x >> 5); ++i) {
-        if (i < warp) before += red[i];
-        all += red[i];
-      }
-      run_ties = all;
-      const bool stays = k != 0 && (k > t_key || (k == t_key && before + t <= ties));
-      u64 m = 0;
-      if (stays) {
-        const double w = weight(k, top, Tw);
-        if (!(min_p > 0.f) || w >= (double)min_p) m = mass_of(w, p.shift);
-      }
-      const u64 mine = m;
-      for (int o = 1; o < 32; o <<= 1) {
-        const u64 v = __shfl_up_sync(0xffffffffu, m, o);
-        if (lane >= o) m += v;
-      }
-      __syncthreads();
-      if (lane == 31) red[warp] = m;
-      __syncthreads();
-      before = run_mass, all = run_mass;
-      for (int i = 0; i < (int)(blockDim.x >> 5); ++i) {
-        if (i < warp) before += red[i];
-        all += red[i];
-      }
-      run_mass = all;
-      if (pass == 1 && mine > 0 && before + m > threshold && before + m - mine <= threshold) s_id = base + tid;
+  if (top_p < 1.f) {
+    // the mass that is left, and the smallest key that has any
+    u64 sum = 0;
+    uint32_t weighs = ~0u;
+    for (int i = tid; i < n; i += blockDim.x) {
+      const uint32_t k = w.key(i);
+      if (k == 0 || !cut.stays(k, lo + i)) continue;
+      const u64 v = w.mass(k);
+      sum += v;
+      if (v) weighs = min(weighs, k);
     }
-    if (pass == 0) {
-      const double u = p.uniform ? p.uniform[blockIdx.x] : 0.0;
-      const double x = u > 0.0 ? u * (double)run_mass : 0.0;
-      threshold = x >= (double)run_mass ? run_mass - 1 : min((u64)x, run_mass - 1);
-    }
+    const u64(&ea)[2][MAX_CLUSTER] = w.template gather<false>(sum, 0);
+    sum = 0;
+    for (int c = 0; c < w.n_ctas; ++c) sum += ea[0][c];
+    const u64(&eb)[2][MAX_CLUSTER] = w.template gather<true>((u64)(uint32_t)~weighs, 0);
+    weighs = 0;
+    for (int c = 0; c < w.n_ctas; ++c) weighs = max(weighs, (uint32_t)eb[0][c]);
+    weighs = ~weighs;
+    cut = w.template find<true>(cut, (double)top_p * (double)sum, weighs, w.best, w.top - key_value(weighs));
   }
-  __syncthreads();
-  finish(s_id, 0);
+  w.draw(cut, min_p > 0.f ? (double)min_p * (double)(1ull << p.shift) : 0.0, p.uniform[q], r);
+  cluster_sync();                   // (no CTA leaves while a peer may still reach into its shared memory)
 }
+
+template <bool RESIDENT>
+int launch_sample(const FilterParams& p, int n_rows, int ctas, int threads, cudaStream_t stream) {
+  const int smem = RESIDENT ? p.per * 4 : 0;
+  static int reserved = 16 * 1024;
+  if (smem > reserved) {
+    cudaError_t e = cudaFuncSetAttribute(sample_filtered_kernel<RESIDENT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    FERRUM_CHECK_ARG(e == cudaSuccess, "sample_filtered: cannot reserve %d bytes of shared memory: %s", smem, cudaGetErrorString(e));
+    reserved = smem;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(n_rows, ctas);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 1;
+  attr[0].val.clusterDim.y = ctas;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = ferrum_dependent_launch_enabled() ? 2 : 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, sample_filtered_kernel<RESIDENT>, p);
+  FERRUM_CHECK_ARG(e == cudaSuccess, "sample_filtered: launch failed: %s", cudaGetErrorString(e));
+  FERRUM_CHECK_LAUNCH("sample_filtered");
+  return 0;
+}
+
+// The most logits that a CTA keeps in its shared memory; a row of more than MAX_CLUSTER times that is read from global memory every time.
+constexpr int MOST_RESIDENT = 45 * 1024;
 
 }  // namespace
 
@@ -204,8 +461,8 @@ FERRUM_API int ferrum_sample_filtered(const float* logits, int ld, int n_rows, i
   if (n_rows == 0) return 0;
   int bits = 0;
   while (bits < 31 && (1ll << bits) < V) ++bits;
-  FilterParams p{logits, rows, temperature, top_k, top_p, min_p, uniform, out_ids, also_to, err_flag, ld, V, 62 - bits};
-  launch_kernel(sample_filtered_kernel, dim3(n_rows), dim3(V >= 8192 ? 1024 : 256), 0, stream, p);
-  FERRUM_CHECK_LAUNCH("sample_filtered");
-  return 0;
+  const int ctas = V >= 16384 ? MAX_CLUSTER : 1;
+  FilterParams p{logits, rows, temperature, top_k, top_p, min_p, uniform, out_ids, also_to, err_flag, ld, V, (V + ctas - 1) / ctas, bits > 17 ? 62 - bits : 45};
+  if (p.per <= MOST_RESIDENT) return launch_sample<true>(p, n_rows, ctas, THREADS, stream);
+  return launch_sample<false>(p, n_rows, ctas, THREADS, stream);
 }
