@@ -156,12 +156,15 @@ struct Row {
     __syncthreads();
   }
 
-  // Where `limit` cuts: of the tokens that `cut` lets stay, ordered, a token stays while the sum of what comes before it is below the limit;
-  // a token counts 1 or (MASS) its mass.  lo_key, hi_key: the smallest and largest key that count.
+  // Where a limit cuts: of the tokens that `cut` lets stay, ordered, a token stays while the sum of what comes before it is below the limit;
+  // a token counts 1, the limit is `limit` itself, or (MASS) a token counts its mass and the limit is that part of all of it.  range: how
+  // far below the maximum the logits go that count (at least).
   template <bool MASS>
-  __device__ __forceinline__ Cut find(const Cut cut, double limit, uint32_t lo_key, uint32_t hi_key, float range) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+  __device__ __forceinline__ Cut find(const Cut cut, double limit, float range) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    uint32_t lo_key = 1, hi_key = best;
     u64 before = 0;
+    bool whole_known = !MASS;
     // the first histogram's bins are of equal width below the maximum, where that is a finite number
     bool linear = isfinite(top) && isfinite(range);
     const float scale = (float)BINS / range;
@@ -173,11 +176,20 @@ struct Row {
       };
       for (int i = tid; i < BINS; i += blockDim.x) sh.hist[i] = 0;
       __syncthreads();
+#pragma unroll 4
       for (int i = tid; i < n; i += blockDim.x) {
         const uint32_t k = key(i);
         if (k < lo_key || k > hi_key || !cut.stays(k, lo + i)) continue;
-        const u64 v = MASS ? mass(k) : 1;
-        if (v) atomicAdd(&sh.hist[bin_of(k)], v);
+        unsigned* half = reinterpret_cast<unsigned*>(&sh.hist[bin_of(k)]);      // (a 64-bit addition by two of 32 bits, the second hardly ever made)
+        if (MASS) {
+          const u64 v = mass(k);
+          const unsigned low = (unsigned)v;
+          if (v == 0) continue;
+          const unsigned old = atomicAdd(half, low), high = (unsigned)(v >> 32) + (old + low < old ? 1 : 0);
+          if (high) atomicAdd(half + 1, high);
+        } else {
+          atomicAdd(half, 1u);
+        }
       }
       cluster_sync();
       // the CTA's share of the bins, BINS / n_ctas of them in the first threads: their sums over the cluster, and how they run
@@ -201,8 +213,13 @@ struct Row {
       __syncthreads();
       if (lane == 31) sh.warp[warp][0] = run;
       __syncthreads();
-      u64 at = before + run - own;
-      for (int c = 0; c < rank; ++c) at += ex[0][c];
+      u64 at = before + run - own, all = 0;
+      for (int c = 0; c < n_ctas; ++c) {
+        if (c < rank) at += ex[0][c];
+        all += ex[0][c];
+      }
+      if (!whole_known) limit *= (double)all;
+      whole_known = true;
       for (int w = 0; w < warp; ++w) at += sh.warp[w][0];
       // the last bin with something in it whose predecessors stay below the limit
       u64 best_bin = 0, best_at = 0;
@@ -218,6 +235,7 @@ struct Row {
       for (int c = 0; c < n_ctas; ++c) bin = max(bin, e2[0][c]), before = max(before, e2[1][c]);
       // the keys in that bin: their range, for the next histogram
       u64 a = 0, b = 0;             // maximum of ~key and of key
+#pragma unroll 4
       for (int i = tid; i < n; i += blockDim.x) {
         const uint32_t k = key(i);
         if (k < lo_key || k > hi_key || bin_of(k) != (int)bin - 1 || !cut.stays(k, lo + i)) continue;
@@ -244,6 +262,7 @@ struct Row {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const int rows = (n + 31) / 32, r0 = (int)((long long)warp * rows / warps), r1 = (int)((long long)(warp + 1) * rows / warps);
     u64 count = 0;
+#pragma unroll 4
     for (int r = r0; r < r1; ++r) {
       const int i = r * 32 + lane;
       count += i < n && key(i) == key_at && cut.stays(key_at, lo + i);
@@ -362,13 +381,13 @@ sample_filtered_kernel(const FilterParams p) {
     refuse(7);
     return;
   }
-  // ---- the slice, its largest key and its smallest (of any logit, and of the finite ones)
-  uint32_t most = 0, least = ~0u, least_finite = ~0u;
+  // ---- the slice, its largest key and its smallest of a finite logit
+  uint32_t most = 0, least_finite = ~0u;
+#pragma unroll 8
   for (int i = tid; i < n; i += blockDim.x) {
     const uint32_t k = order_key(row[lo + i]);
     if (RESIDENT) slice[i] = k;
     most = max(most, k);
-    if (k) least = min(least, k);
     if (k > 0x007fffffu) least_finite = min(least_finite, k);      // (0x007fffff: minus infinity)
   }
   Row<RESIDENT> w{p, sh, slice, row, rank, (int)gridDim.y, lo, n, 0, 0, 0.f, 0.0};
@@ -390,31 +409,10 @@ sample_filtered_kernel(const FilterParams p) {
     return;
   }
   w.inv_t = 1.0 / (double)T;
-  if (top_k > 0 && top_k < p.V) {
-    const u64(&ea)[2][MAX_CLUSTER] = w.template gather<true>((uint32_t)~least, 0);
-    for (int c = 0; c < w.n_ctas; ++c) least = min(least, ~(uint32_t)ea[0][c]);
-    cut = w.template find<false>(cut, (double)top_k, least, w.best, least_finite == ~0u ? INFINITY : w.top - key_value(least_finite));
-  }
-  if (top_p < 1.f) {
-    // the mass that is left, and the smallest key that has any
-    u64 sum = 0;
-    uint32_t weighs = ~0u;
-    for (int i = tid; i < n; i += blockDim.x) {
-      const uint32_t k = w.key(i);
-      if (k == 0 || !cut.stays(k, lo + i)) continue;
-      const u64 v = w.mass(k);
-      sum += v;
-      if (v) weighs = min(weighs, k);
-    }
-    const u64(&ea)[2][MAX_CLUSTER] = w.template gather<false>(sum, 0);
-    sum = 0;
-    for (int c = 0; c < w.n_ctas; ++c) sum += ea[0][c];
-    const u64(&eb)[2][MAX_CLUSTER] = w.template gather<true>((u64)(uint32_t)~weighs, 0);
-    weighs = 0;
-    for (int c = 0; c < w.n_ctas; ++c) weighs = max(weighs, (uint32_t)eb[0][c]);
-    weighs = ~weighs;
-    cut = w.template find<true>(cut, (double)top_p * (double)sum, weighs, w.best, w.top - key_value(weighs));
-  }
+  const float range = least_finite == ~0u ? INFINITY : w.top - key_value(least_finite);
+  if (top_k > 0 && top_k < p.V) cut = w.template find<false>(cut, (double)top_k, range);
+  // (a token further below the maximum than (shift + 1) ln 2 temperatures has no mass)
+  if (top_p < 1.f) cut = w.template find<true>(cut, (double)top_p, fminf(range, (float)(p.shift + 1) * 0.6931472f * T));
   w.draw(cut, min_p > 0.f ? (double)min_p * (double)(1ull << p.shift) : 0.0, p.uniform[q], r);
   cluster_sync();                   // (no CTA leaves while a peer may still reach into its shared memory)
 }
