@@ -8,11 +8,12 @@
 // T = 0 takes the largest logit.  Masses are whole numbers, w_i rounded to 2^-s with s = min(45, 62 - ceil(log2 V)): their sums are exact
 // whatever their order, and 2^-45 is far below what a row's sum of 32-bit weights could tell apart.
 //
-// A cluster of CTAs holds a row's logits in its shared memory, as integers of the same order, and reads them from there as often as it
-// takes.  Where top-k or top-p cuts is found by histograms: 2,048 bins of equal width below the maximum, then the range of keys in the
-// bin that holds the cut, cut into 2,048 again, until that bin holds a single key (one or two histograms for logits of any real
-// model, four at most).  Each CTA counts its slice; of the bins' sums over the cluster each CTA makes its share.  Of equal keys at the
-// cut the first in index order stay: a threshold is a key and an index.
+// A cluster of CTAs holds a row's logits in its shared memory, as integers of the same order; a warp owns a run of them.  Where top-k or
+// top-p cuts is found by histograms: 2,048 bins of equal width below the maximum, then the range of keys in the bin that holds the
+// cut, cut into 2,048 again, until that bin holds a single key (one or two histograms for logits of any real model, four at
+// most).  Each CTA counts its slice; of the bins' sums over the cluster each CTA makes its share.  What lies in the bin of the cut or
+// above it is listed on the way, in index order, and all that follows reads the lists (where a warp's share outgrows its list,
+// the slice again).  Of equal keys at the cut the first in index order stay: a threshold is a key and an index.
 //
 // The reference samples greedily only (crates/core-types/src/model.rs:44-62).
 #include "common.cuh"
@@ -22,9 +23,10 @@ namespace {
 typedef unsigned long long u64;
 
 constexpr int BINS = 2048;
-constexpr int MAX_CLUSTER = 8;
-constexpr int THREADS = 512;
-constexpr int SEGMENTS = 8;         // parts of a warp's range whose masses are kept for the draw
+constexpr int MAX_CLUSTER = 16;
+constexpr int MAX_WARPS = 32;
+constexpr int SEGMENTS = 4;         // parts of a warp's run whose masses are kept for the draw
+constexpr int LIST = 1024;          // listed tokens of a CTA, LIST / warps of a warp
 
 // Order-preserving integer of a logit; 0 stands for NaN, which comes after everything and is never kept.
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -74,9 +76,11 @@ __device__ __forceinline__ void cluster_sync() {
 struct Shared {
   u64 hist[BINS];
   u64 exchange[4][2][MAX_CLUSTER];
-  u64 warp[THREADS / 32][2];
-  u64 segment[THREADS / 32][SEGMENTS];
+  u64 warp[MAX_WARPS][2];
+  u64 segment[MAX_WARPS][SEGMENTS];
   u64 found[2];
+  uint32_t list_key[LIST];
+  int list_index[LIST];
   double powers[64];                // 2^(j / 64)
 };
 
@@ -87,13 +91,16 @@ struct Row {
   Shared& sh;
   const uint32_t* keys;             // the slice in shared memory, or
   const float* row;                 // in global memory
-  int rank, n_ctas, lo, n;          // the slice: logits lo .. lo + n - 1
+  int rank, n_ctas, lo;             // the slice's first logit
+  int e0, e1;                       // the warp's run: entries e0 .. e1 - 1 of the slice, or of the lists
+  bool listed;
   int turn;                         // exchanges so far
   uint32_t best;
   float top;
   double inv_t;
 
-  __device__ __forceinline__ uint32_t key(int i) const { return RESIDENT ? keys[i] : order_key(row[lo + i]); }
+  __device__ __forceinline__ uint32_t key(int e) const { return listed ? sh.list_key[e] : RESIDENT ? keys[e] : order_key(row[lo + e]); }
+  __device__ __forceinline__ int index(int e) const { return listed ? sh.list_index[e] : lo + e; }
 
   // w * 2^shift of a key, not rounded.  exp by 2^(n / 64) from a table and the series of the rest (below 2^-7 in size: the sixth term is
   // 3e-17 of the sum); what is below 2^-1 after the scaling rounds to 0 whatever its value.
@@ -177,9 +184,9 @@ struct Row {
       for (int i = tid; i < BINS; i += blockDim.x) sh.hist[i] = 0;
       __syncthreads();
 #pragma unroll 4
-      for (int i = tid; i < n; i += blockDim.x) {
-        const uint32_t k = key(i);
-        if (k < lo_key || k > hi_key || !cut.stays(k, lo + i)) continue;
+      for (int e = e0 + lane; e < e1; e += 32) {
+        const uint32_t k = key(e);
+        if (k < lo_key || k > hi_key || !cut.stays(k, index(e))) continue;
         unsigned* half = reinterpret_cast<unsigned*>(&sh.hist[bin_of(k)]);      // (a 64-bit addition by two of 32 bits, the second hardly ever made)
         if (MASS) {
           const u64 v = mass(k);
@@ -194,14 +201,19 @@ struct Row {
       cluster_sync();
       // the CTA's share of the bins, BINS / n_ctas of them in the first threads: their sums over the cluster, and how they run
       const int share = BINS / n_ctas;
-      u64 mine[BINS / THREADS] = {}, run = 0;
+      constexpr int MOST = 4;
+      u64 mine[MOST] = {}, run = 0;
       const int each = max(1, share / (int)blockDim.x), b0 = rank * share + tid * each;
       const bool has = tid * each < share;
       if (has)
-        for (int j = 0; j < each; ++j) {
-          for (int c = 0; c < n_ctas; ++c) mine[j] += load_peer(peer((uint32_t)__cvta_generic_to_shared(&sh.hist[b0 + j]), c));
-          run += mine[j];
-        }
+#pragma unroll
+        for (int j = 0; j < MOST; ++j)
+          if (j < each) {
+            const uint32_t at = (uint32_t)__cvta_generic_to_shared(&sh.hist[b0 + j]);
+#pragma unroll 8
+            for (int c = 0; c < n_ctas; ++c) mine[j] += load_peer(peer(at, c));
+            run += mine[j];
+          }
       const u64 own = run;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -220,12 +232,14 @@ struct Row {
       }
       if (!whole_known) limit *= (double)all;
       whole_known = true;
-      for (int w = 0; w < warp; ++w) at += sh.warp[w][0];
+      if (has)
+        for (int w = 0; w < warp; ++w) at += sh.warp[w][0];
       // the last bin with something in it whose predecessors stay below the limit
       u64 best_bin = 0, best_at = 0;
       if (has)
-        for (int j = 0; j < each; ++j) {
-          if (mine[j] && (double)at < limit) best_bin = b0 + j + 1, best_at = at;
+#pragma unroll
+        for (int j = 0; j < MOST; ++j) {
+          if (j < each && mine[j] && (double)at < limit) best_bin = b0 + j + 1, best_at = at;
           at += mine[j];
         }
       // bins and their sums rise together: the largest of each belong together
@@ -233,21 +247,57 @@ struct Row {
       u64 bin = 0;
       before = 0;
       for (int c = 0; c < n_ctas; ++c) bin = max(bin, e2[0][c]), before = max(before, e2[1][c]);
-      // the keys in that bin: their range, for the next histogram
-      u64 a = 0, b = 0;             // maximum of ~key and of key
+      // the range of the keys in that bin, for the next histogram; and the lists of what lies in it or above
+      uint32_t a = 0, b = 0;        // maximum of ~key and of key
+      const int border = (int)bin - 1, most = LIST / (int)(blockDim.x >> 5);
+      int count = 0;
 #pragma unroll 4
-      for (int i = tid; i < n; i += blockDim.x) {
-        const uint32_t k = key(i);
-        if (k < lo_key || k > hi_key || bin_of(k) != (int)bin - 1 || !cut.stays(k, lo + i)) continue;
-        if (MASS && !mass(k)) continue;
-        a = max(a, (u64)(uint32_t)~k);
-        b = max(b, (u64)k);
+      for (int e = e0 + lane; e - lane < e1; e += 32) {
+        const uint32_t k = e < e1 ? key(e) : 0;
+        const bool fits = k >= lo_key && cut.stays(k, e < e1 ? index(e) : 0);
+        const int its = fits && k <= hi_key ? bin_of(k) : -1;
+        if (its == border && !(MASS && mass(k) == 0)) {
+          a = max(a, ~k);
+          b = max(b, k);
+        }
+        if (!listed) {
+          const unsigned hit = __ballot_sync(0xffffffffu, fits && its <= border);
+          if (hit) {
+            const int slot = count + __popc(hit & ((1u << lane) - 1));
+            if ((hit >> lane & 1) && slot < most) {
+              sh.list_key[warp * most + slot] = k;
+              sh.list_index[warp * most + slot] = index(e);
+            }
+            count += __popc(hit);
+          }
+        }
       }
-      const u64(&e3)[2][MAX_CLUSTER] = gather<true>(a, b);
+      const u64(&e3)[2][MAX_CLUSTER] = gather<true>((u64)(count > most) << 32 | a, b);
       a = b = 0;
-      for (int c = 0; c < n_ctas; ++c) a = max(a, e3[0][c]), b = max(b, e3[1][c]);
-      lo_key = ~(uint32_t)a;
-      hi_key = (uint32_t)b;
+      bool fit = !listed;
+      for (int c = 0; c < n_ctas; ++c) {
+        a = max(a, (uint32_t)e3[0][c]);
+        b = max(b, (uint32_t)e3[1][c]);
+        fit &= e3[0][c] >> 32 == 0;
+      }
+      if (!fit && !listed) {        // (the flag hid a CTA's range: once more without it)
+        uint32_t a2 = 0;
+        for (int e = e0 + lane; e < e1; e += 32) {
+          const uint32_t k = key(e);
+          if (k >= lo_key && k <= hi_key && cut.stays(k, index(e)) && bin_of(k) == border && !(MASS && mass(k) == 0)) a2 = max(a2, ~k);
+        }
+        const u64(&e4)[2][MAX_CLUSTER] = gather<true>(a2, 0);
+        a = 0;
+        for (int c = 0; c < n_ctas; ++c) a = max(a, (uint32_t)e4[0][c]);
+      }
+      if (fit) {
+        __syncwarp();
+        listed = true;
+        e0 = warp * most;
+        e1 = e0 + count;
+      }
+      lo_key = ~a;
+      hi_key = b;
       linear = false;
     }
     // of the tokens equal to the key at the cut the i-th stays if before + i * one < limit
@@ -259,17 +309,11 @@ struct Row {
 
   // The cut behind the stay-th token (counted from 1, in index order) with this key that `cut` lets stay.
   __device__ __forceinline__ Cut first_of(uint32_t key_at, const Cut cut, u64 stay) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    const int rows = (n + 31) / 32, r0 = (int)((long long)warp * rows / warps), r1 = (int)((long long)(warp + 1) * rows / warps);
-    u64 count = 0;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    unsigned count = 0;
 #pragma unroll 4
-    for (int r = r0; r < r1; ++r) {
-      const int i = r * 32 + lane;
-      count += i < n && key(i) == key_at && cut.stays(key_at, lo + i);
-    }
-    u64 total = count;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    for (int e = e0 + lane; e < e1; e += 32) count += key(e) == key_at && cut.stays(key_at, index(e));
+    const unsigned total = __reduce_add_sync(0xffffffffu, count);
     const u64(&ex)[2][MAX_CLUSTER] = gather<false>(count, 0);
     u64 all = 0, ahead = 0;
     for (int c = 0; c < n_ctas; ++c) {
@@ -282,39 +326,39 @@ struct Row {
     __syncthreads();
     for (int w = 0; w < warp; ++w) ahead += sh.warp[w][0];
     bool mine = false;
-    int index = 0;
+    int found = 0;
     if (ahead < stay && stay <= ahead + total)
-      for (int r = r0; r < r1; ++r) {
-        const int i = r * 32 + lane;
-        const unsigned hit = __ballot_sync(0xffffffffu, i < n && key(i) == key_at && cut.stays(key_at, lo + i));
+      for (int e = e0 + lane; e - lane < e1; e += 32) {
+        const unsigned hit = __ballot_sync(0xffffffffu, e < e1 && key(e) == key_at && cut.stays(key_at, index(e)));
         const u64 here = __popc(hit);
         if (ahead + here >= stay) {
           const int nth = (int)(stay - ahead);      // the nth set bit of hit
           mine = (hit >> lane & 1) && __popc(hit & ((2u << lane) - 1)) == nth;
-          index = lo + i;
+          if (mine) found = index(e);
           break;
         }
         ahead += here;
       }
-    tell(mine, (u64)index, 0);
+    tell(mine, (u64)found, 0);
     return Cut{key_at, (int)sh.found[0]};
   }
 
   // The draw from the tokens that the cut lets stay and that weigh min_w at least.
   __device__ __forceinline__ void draw(const Cut cut, double min_w, double u, int out) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    const int rows = (n + 31) / 32, r0 = (int)((long long)warp * rows / warps), r1 = (int)((long long)(warp + 1) * rows / warps);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int rows = (e1 - e0 + 31) / 32;
     auto mass_at = [&](int r) -> u64 {
-      const int i = r * 32 + lane;
-      const uint32_t k = i < n ? key(i) : 0;
-      if (k == 0 || !cut.stays(k, lo + i)) return 0;
+      const int e = e0 + r * 32 + lane;
+      const uint32_t k = e < e1 ? key(e) : 0;
+      if (k == 0 || !cut.stays(k, index(e))) return 0;
       const double v = scaled_weight(k);
       return v >= min_w ? whole(v) : 0;
     };
     u64 sum = 0;
     for (int s = 0; s < SEGMENTS; ++s) {
       u64 part = 0;
-      for (int r = r0 + (r1 - r0) * s / SEGMENTS; r < r0 + (r1 - r0) * (s + 1) / SEGMENTS; ++r) part += mass_at(r);
+#pragma unroll 4
+      for (int r = rows * s / SEGMENTS; r < rows * (s + 1) / SEGMENTS; ++r) part += mass_at(r);
       sum += part;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
@@ -334,7 +378,7 @@ struct Row {
     for (int s = 0; s < SEGMENTS; ++s) {
       const u64 part = sh.segment[warp][s];
       if (threshold >= at && threshold < at + part) {
-        for (int r = r0 + (r1 - r0) * s / SEGMENTS; r < r0 + (r1 - r0) * (s + 1) / SEGMENTS; ++r) {
+        for (int r = rows * s / SEGMENTS; r < rows * (s + 1) / SEGMENTS; ++r) {
           const u64 own = mass_at(r);
           u64 run = own;
 #pragma unroll
@@ -343,8 +387,9 @@ struct Row {
             if (lane >= o) run += v;
           }
           if (threshold >= at + run - own && threshold < at + run) {
-            p.out_ids[out] = lo + r * 32 + lane;
-            if (p.also_to) p.also_to[out] = lo + r * 32 + lane;
+            const int id = index(e0 + r * 32 + lane);
+            p.out_ids[out] = id;
+            if (p.also_to) p.also_to[out] = id;
           }
           at += __shfl_sync(0xffffffffu, run, 31);
         }
@@ -356,7 +401,7 @@ struct Row {
 };
 
 template <bool RESIDENT>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(32 * MAX_WARPS)
 sample_filtered_kernel(const FilterParams p) {
   extern __shared__ __align__(16) uint32_t slice[];
   __shared__ Shared sh;
@@ -390,7 +435,9 @@ sample_filtered_kernel(const FilterParams p) {
     most = max(most, k);
     if (k > 0x007fffffu) least_finite = min(least_finite, k);      // (0x007fffff: minus infinity)
   }
-  Row<RESIDENT> w{p, sh, slice, row, rank, (int)gridDim.y, lo, n, 0, 0, 0.f, 0.0};
+  const int warps = blockDim.x >> 5, lines = (n + 31) / 32;
+  Row<RESIDENT> w{p, sh, slice, row, rank, (int)gridDim.y, lo, (int)((long long)(tid >> 5) * lines / warps) * 32,
+                  min(n, (int)((long long)((tid >> 5) + 1) * lines / warps) * 32), false, 0, 0, 0.f, 0.0};
   const u64(&ex)[2][MAX_CLUSTER] = w.template gather<true>(most, (uint32_t)~least_finite);
   for (int c = 0; c < w.n_ctas; ++c) {
     w.best = max(w.best, (uint32_t)ex[0][c]);
@@ -420,11 +467,12 @@ sample_filtered_kernel(const FilterParams p) {
 template <bool RESIDENT>
 int launch_sample(const FilterParams& p, int n_rows, int ctas, int threads, cudaStream_t stream) {
   const int smem = RESIDENT ? p.per * 4 : 0;
-  static int reserved = 16 * 1024;
-  if (smem > reserved) {
-    cudaError_t e = cudaFuncSetAttribute(sample_filtered_kernel<RESIDENT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static int reserved = 0;
+  if (smem > reserved || reserved == 0) {
+    cudaError_t e = cudaFuncSetAttribute(sample_filtered_kernel<RESIDENT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(sample_filtered_kernel<RESIDENT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     FERRUM_CHECK_ARG(e == cudaSuccess, "sample_filtered: cannot reserve %d bytes of shared memory: %s", smem, cudaGetErrorString(e));
-    reserved = smem;
+    reserved = max(smem, 1);
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(n_rows, ctas);
@@ -459,8 +507,10 @@ FERRUM_API int ferrum_sample_filtered(const float* logits, int ld, int n_rows, i
   if (n_rows == 0) return 0;
   int bits = 0;
   while (bits < 31 && (1ll << bits) < V) ++bits;
-  const int ctas = V >= 16384 ? MAX_CLUSTER : 1;
+  // A few rows: clusters of 16 CTAs of 1,024 threads, so that the whole GPU reads them; more: 8 CTAs of 512.  Small vocabularies: one CTA.
+  const int sms = ferrum_sm_count(), ctas = V < 16384 ? 1 : n_rows * MAX_CLUSTER <= sms && V >= 65536 ? MAX_CLUSTER : 8;
+  const int threads = n_rows * ctas <= sms && V >= 8192 ? 1024 : 512;
   FilterParams p{logits, rows, temperature, top_k, top_p, min_p, uniform, out_ids, also_to, err_flag, ld, V, (V + ctas - 1) / ctas, bits > 17 ? 62 - bits : 45};
-  if (p.per <= MOST_RESIDENT) return launch_sample<true>(p, n_rows, ctas, THREADS, stream);
-  return launch_sample<false>(p, n_rows, ctas, THREADS, stream);
+  if (p.per <= MOST_RESIDENT) return launch_sample<true>(p, n_rows, ctas, threads, stream);
+  return launch_sample<false>(p, n_rows, ctas, threads, stream);
 }

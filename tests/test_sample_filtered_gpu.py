@@ -72,6 +72,18 @@ def test_draws(cuda, V, kind):
           some(rng.uniform(0, 0.3, n), 0.0), rng.random(n))
 
 
+@pytest.mark.parametrize("n,V", [(1, 128256), (9, 70000), (10, 70000), (19, 65536), (3, 400001), (2, 760000), (150, 900)])
+def test_launch_shapes(cuda, n, V):
+    """Clusters of every size, rows that outgrow the shared memory, cuts that outgrow the lists of what lies above them."""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    rng = np.random.default_rng(n)
+    for kind in ("plain", "ties"):
+        x = rows_of(kind, n, V, g)
+        some = lambda v, off: np.where(rng.random(n) < 0.6, v, off)
+        check(x, rng.uniform(0.7, 1.5, n), some(np.exp(rng.uniform(0, np.log(V + 1), n)).astype(int), 0), some(rng.uniform(0.5, 0.999, n), 1.0),
+              some(rng.uniform(0, 0.05, n), 0.0), rng.random(n))
+
+
 @pytest.mark.parametrize("V", [700, 50000])
 def test_edges_of_the_filters(cuda, V):
     """k of 1, V and beyond; p next to 0 and 1; min_p of 1; random numbers 0 and next to 1; a temperature next to 0 and a large one."""
