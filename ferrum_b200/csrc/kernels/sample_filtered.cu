@@ -13,7 +13,7 @@
 // cut, cut into 2,048 again, until that bin holds a single key (one or two histograms for logits of any real model, four at
 // most).  Each CTA counts its slice; of the bins' sums over the cluster each CTA makes its share.  What lies in the bin of the cut or
 // above it is listed on the way, in index order, and all that follows reads the lists (where a warp's share outgrows its list,
-// the slice again).  Of equal keys at the cut the first in index order stay: a threshold is a key and an index.
+// the slice again).  Where the first histogram leaves no more than 1,024 tokens, the usual case, one CTA sorts those and does the rest alone.  Of equal keys at the cut the first in index order stay: a threshold is a key and an index.
 //
 // The reference samples greedily only (crates/core-types/src/model.rs:44-62).
 #include "common.cuh"
@@ -27,6 +27,8 @@ constexpr int MAX_CLUSTER = 16;
 constexpr int MAX_WARPS = 32;
 constexpr int SEGMENTS = 4;         // parts of a warp's run whose masses are kept for the draw
 constexpr int LIST = 1024;          // listed tokens of a CTA, LIST / warps of a warp
+constexpr int MOST_BINS = 4;        // bins of a thread's share: BINS / 512
+constexpr int FEW = 1024;           // tokens that one CTA sorts
 
 // Order-preserving integer of a logit; 0 stands for NaN, which comes after everything and is never kept.
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -74,7 +76,13 @@ __device__ __forceinline__ void cluster_sync() {
 }
 
 struct Shared {
-  u64 hist[BINS];
+  union {
+    u64 hist[BINS];
+    struct {
+      u64 order[FEW], mass[FEW];    // the first CTA's: (key, ~index) of the tokens at or above the cut, and their masses
+    };
+  };
+  unsigned few;                     // how many there are
   u64 exchange[4][2][MAX_CLUSTER];
   u64 warp[MAX_WARPS][2];
   u64 segment[MAX_WARPS][SEGMENTS];
@@ -163,6 +171,197 @@ struct Row {
     __syncthreads();
   }
 
+  // Running sums of mass[0 .. size - 1] in place (size a power of two, at least 32 and at most 2 * blockDim).
+  __device__ __forceinline__ void run_sums(int size) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, chunks = size / 32;
+    __syncthreads();
+    for (int w = warp; w < chunks; w += blockDim.x >> 5) {
+      u64 v = sh.mass[w * 32 + lane];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const u64 x = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += x;
+      }
+      sh.mass[w * 32 + lane] = v;
+    }
+    __syncthreads();
+    if (warp == 0) {                // the chunks' totals, one a lane
+      u64 v = lane < chunks ? sh.mass[lane * 32 + 31] : 0;
+      const u64 own = v;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const u64 x = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += x;
+      }
+      sh.warp[lane][0] = v - own;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < size; i += blockDim.x) sh.mass[i] += sh.warp[i >> 5][0];
+    __syncthreads();
+  }
+  // order[0 .. size - 1], the largest first.
+  __device__ __forceinline__ void sort_down(int size) {
+    for (int k = 2; k <= size; k <<= 1)
+      for (int j = k >> 1; j > 0; j >>= 1) {
+        __syncthreads();
+        for (int t = threadIdx.x; t < size / 2; t += blockDim.x) {
+          const int i = 2 * t - (t & (j - 1));      // the lower of the pair (i, i + j)
+          const u64 a = sh.order[i], b = sh.order[i + j];
+          if ((a < b) == ((i & k) == 0)) sh.order[i] = b, sh.order[i + j] = a;
+        }
+      }
+    __syncthreads();
+  }
+
+  // Rows whose cut leaves few tokens: one histogram, and the tokens of the bins down to the one that holds the cut go to the first CTA, which sorts
+  // them and does the rest.  BY_MASS: no top-k, so that the cut is top-p's.  False (for all CTAs alike): there are more than FEW of them.
+  template <bool BY_MASS>
+  __device__ __forceinline__ bool draw_of_few(int top_k, float top_p, double min_w, double u, float range, int out) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (!(isfinite(top) && isfinite(range))) return false;
+    const float scale = (float)BINS / range;
+    auto bin_of = [&](uint32_t k) { return min(BINS - 1, (int)((top - key_value(k)) * scale)); };
+    for (int i = tid; i < BINS; i += blockDim.x) sh.hist[i] = 0;
+    __syncthreads();
+#pragma unroll 4
+    for (int e = e0 + lane; e < e1; e += 32) {
+      const uint32_t k = key(e);
+      if (k == 0) continue;
+      unsigned* half = reinterpret_cast<unsigned*>(&sh.hist[bin_of(k)]);
+      if (BY_MASS) {
+        const u64 v = mass(k);
+        const unsigned low = (unsigned)v;
+        if (v == 0) continue;
+        const unsigned old = atomicAdd(half, low), high = (unsigned)(v >> 32) + (old + low < old ? 1 : 0);
+        if (high) atomicAdd(half + 1, high);
+      } else {
+        atomicAdd(half, 1u);
+      }
+    }
+    cluster_sync();
+    u64 mine[MOST_BINS], own, all, at;
+    int b0, each;
+    bins_of_cluster(mine, own, all, at, b0, each);
+    const double limit = BY_MASS ? (double)top_p * (double)all : (double)top_k;
+    u64 best_bin = 0;
+#pragma unroll
+    for (int j = 0; j < MOST_BINS; ++j) {
+      if (j < each && mine[j] && (double)at < limit) best_bin = b0 + j + 1;
+      at += mine[j];
+    }
+    const u64(&e2)[2][MAX_CLUSTER] = gather<true>(best_bin, 0);
+    int border = 0;
+    for (int c = 0; c < n_ctas; ++c) border = max(border, (int)e2[0][c]);
+    // (the bins are read: their place is free)
+    unsigned count = 0;
+#pragma unroll 4
+    for (int e = e0 + lane; e < e1; e += 32) {
+      const uint32_t k = key(e);
+      count += k != 0 && bin_of(k) < border;
+    }
+    const unsigned total = __reduce_add_sync(0xffffffffu, count);
+    if (total) {
+      unsigned base = 0;
+      if (lane == 0)
+        asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], %2;"
+                     : "=r"(base) : "r"(peer((uint32_t)__cvta_generic_to_shared(&sh.few), 0)), "r"(total) : "memory");
+      base = __shfl_sync(0xffffffffu, base, 0);
+      if (base + total <= FEW)
+        for (int e = e0 + lane; e - lane < e1; e += 32) {
+          const uint32_t k = e < e1 ? key(e) : 0;
+          const bool goes = k != 0 && bin_of(k) < border;
+          const unsigned hit = __ballot_sync(0xffffffffu, goes);
+          if (goes)
+            store_peer(peer((uint32_t)__cvta_generic_to_shared(&sh.order[base + __popc(hit & ((1u << lane) - 1))]), 0), (u64)k << 32 | (uint32_t)~index(e));
+          base += __popc(hit);
+        }
+    }
+    cluster_sync();
+    unsigned n;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(n) : "r"(peer((uint32_t)__cvta_generic_to_shared(&sh.few), 0)) : "memory");
+    cluster_sync();                 // (read before the first CTA goes on, or leaves)
+    if (n > FEW) return false;
+    if (rank != 0) return true;
+    int size = 32;
+    while (size < (int)n) size <<= 1;
+    for (int i = tid; i < size; i += blockDim.x)
+      if (i >= (int)n) sh.order[i] = 0;
+    sort_down(size);
+    auto weigh = [&](int i) { return i < (int)n ? scaled_weight((uint32_t)(sh.order[i] >> 32)) : 0.0; };
+    for (int i = tid; i < size; i += blockDim.x) sh.mass[i] = whole(weigh(i));
+    run_sums(size);
+    const int n_k = BY_MASS ? (int)n : min((int)n, top_k);
+    const double part = BY_MASS ? limit : top_p < 1.f ? (double)top_p * (double)sh.mass[n_k - 1] : INFINITY;
+    // what stays are the first so many
+    int stays = 0;
+    for (int i = tid; i < n_k; i += blockDim.x)
+      if ((i == 0 || (double)sh.mass[i - 1] < part) && weigh(i) >= min_w) stays = i + 1;
+    stays = __reduce_max_sync(0xffffffffu, stays);
+    __syncthreads();
+    if (lane == 0) sh.warp[warp][1] = stays;
+    __syncthreads();
+    for (int w = 0; w < (int)(blockDim.x >> 5); ++w) stays = max(stays, (int)sh.warp[w][1]);
+    const u64 sum = sh.mass[stays - 1];
+    const double x = u > 0.0 ? u * (double)sum : 0.0;
+    const u64 threshold = x >= (double)sum ? sum - 1 : min((u64)x, sum - 1);
+    // in index order: (~index, key) from the largest down
+    size = 32;
+    while (size < stays) size <<= 1;
+    for (int i = tid; i < size; i += blockDim.x) {
+      const u64 v = sh.order[i];
+      sh.order[i] = i < stays ? v << 32 | v >> 32 : 0;
+    }
+    sort_down(size);
+    for (int i = tid; i < size; i += blockDim.x) sh.mass[i] = i < stays ? mass((uint32_t)sh.order[i]) : 0;
+    run_sums(size);
+    for (int i = tid; i < stays; i += blockDim.x)
+      if (threshold < sh.mass[i] && (i == 0 || threshold >= sh.mass[i - 1])) {
+        const int id = (int)~(uint32_t)(sh.order[i] >> 32);
+        p.out_ids[out] = id;
+        if (p.also_to) p.also_to[out] = id;
+      }
+    return true;
+  }
+
+  // The CTA's share of the histogram's bins, `each` from b0 on for the first threads: their sums over the cluster (mine, zeros beyond), what lies in the
+  // bins before them (at) and in all (all).  All threads of the cluster call it behind the barrier that ends the counting.
+  __device__ __forceinline__ void bins_of_cluster(u64 (&mine)[MOST_BINS], u64& own, u64& all, u64& at, int& b0, int& each) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, share = BINS / n_ctas;
+    each = max(1, share / (int)blockDim.x);
+    b0 = rank * share + tid * each;
+    const bool has = tid * each < share;
+    u64 run = 0;
+#pragma unroll
+    for (int j = 0; j < MOST_BINS; ++j) {
+      mine[j] = 0;
+      if (has && j < each) {
+        const uint32_t a = (uint32_t)__cvta_generic_to_shared(&sh.hist[b0 + j]);
+#pragma unroll 8
+        for (int c = 0; c < n_ctas; ++c) mine[j] += load_peer(peer(a, c));
+      }
+      run += mine[j];
+    }
+    own = run;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const u64 v = __shfl_up_sync(0xffffffffu, run, o);
+      if (lane >= o) run += v;
+    }
+    const u64(&ex)[2][MAX_CLUSTER] = gather<false>(own, 0);
+    // (gather's sums went over sh.warp; the warps' own totals for the running sums follow in it)
+    __syncthreads();
+    if (lane == 31) sh.warp[warp][0] = run;
+    __syncthreads();
+    at = run - own;
+    all = 0;
+    for (int c = 0; c < n_ctas; ++c) {
+      if (c < rank) at += ex[0][c];
+      all += ex[0][c];
+    }
+    if (has)
+      for (int w = 0; w < warp; ++w) at += sh.warp[w][0];
+  }
+
   // Where a limit cuts: of the tokens that `cut` lets stay, ordered, a token stays while the sum of what comes before it is below the limit;
   // a token counts 1, the limit is `limit` itself, or (MASS) a token counts its mass and the limit is that part of all of it.  range: how
   // far below the maximum the logits go that count (at least).
@@ -199,49 +398,19 @@ struct Row {
         }
       }
       cluster_sync();
-      // the CTA's share of the bins, BINS / n_ctas of them in the first threads: their sums over the cluster, and how they run
-      const int share = BINS / n_ctas;
-      constexpr int MOST = 4;
-      u64 mine[MOST] = {}, run = 0;
-      const int each = max(1, share / (int)blockDim.x), b0 = rank * share + tid * each;
-      const bool has = tid * each < share;
-      if (has)
-#pragma unroll
-        for (int j = 0; j < MOST; ++j)
-          if (j < each) {
-            const uint32_t at = (uint32_t)__cvta_generic_to_shared(&sh.hist[b0 + j]);
-#pragma unroll 8
-            for (int c = 0; c < n_ctas; ++c) mine[j] += load_peer(peer(at, c));
-            run += mine[j];
-          }
-      const u64 own = run;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const u64 v = __shfl_up_sync(0xffffffffu, run, o);
-        if (lane >= o) run += v;
-      }
-      const u64(&ex)[2][MAX_CLUSTER] = gather<false>(own, 0);
-      // (gather's sums went over sh.warp; the warps' own totals for the running sums follow in it)
-      __syncthreads();
-      if (lane == 31) sh.warp[warp][0] = run;
-      __syncthreads();
-      u64 at = before + run - own, all = 0;
-      for (int c = 0; c < n_ctas; ++c) {
-        if (c < rank) at += ex[0][c];
-        all += ex[0][c];
-      }
+      u64 mine[MOST_BINS], own, all, at;
+      int b0, each;
+      bins_of_cluster(mine, own, all, at, b0, each);
+      at += before;
       if (!whole_known) limit *= (double)all;
       whole_known = true;
-      if (has)
-        for (int w = 0; w < warp; ++w) at += sh.warp[w][0];
       // the last bin with something in it whose predecessors stay below the limit
       u64 best_bin = 0, best_at = 0;
-      if (has)
 #pragma unroll
-        for (int j = 0; j < MOST; ++j) {
-          if (j < each && mine[j] && (double)at < limit) best_bin = b0 + j + 1, best_at = at;
-          at += mine[j];
-        }
+      for (int j = 0; j < MOST_BINS; ++j) {
+        if (j < each && mine[j] && (double)at < limit) best_bin = b0 + j + 1, best_at = at;
+        at += mine[j];
+      }
       // bins and their sums rise together: the largest of each belong together
       const u64(&e2)[2][MAX_CLUSTER] = gather<true>(best_bin, best_at);
       u64 bin = 0;
@@ -406,6 +575,7 @@ sample_filtered_kernel(const FilterParams p) {
   extern __shared__ __align__(16) uint32_t slice[];
   __shared__ Shared sh;
   const int tid = threadIdx.x;
+  if (tid == 0) sh.few = 0;
   if (tid < 64) sh.powers[tid] = exp2((double)tid / 64.0);
   // a CTA's shared memory may be written by a peer only once the CTA is known to run
   cluster_sync();
@@ -457,10 +627,16 @@ sample_filtered_kernel(const FilterParams p) {
   }
   w.inv_t = 1.0 / (double)T;
   const float range = least_finite == ~0u ? INFINITY : w.top - key_value(least_finite);
-  if (top_k > 0 && top_k < p.V) cut = w.template find<false>(cut, (double)top_k, range);
   // (a token further below the maximum than (shift + 1) ln 2 temperatures has no mass)
-  if (top_p < 1.f) cut = w.template find<true>(cut, (double)top_p, fminf(range, (float)(p.shift + 1) * 0.6931472f * T));
-  w.draw(cut, min_p > 0.f ? (double)min_p * (double)(1ull << p.shift) : 0.0, p.uniform[q], r);
+  const float mass_range = fminf(range, (float)(p.shift + 1) * 0.6931472f * T);
+  const double min_w = min_p > 0.f ? (double)min_p * (double)(1ull << p.shift) : 0.0, u = p.uniform[q];
+  const bool by_k = top_k > 0 && top_k < p.V, by_p = top_p < 1.f;
+  if (by_k ? top_k <= FEW && w.template draw_of_few<false>(top_k, top_p, min_w, u, range, r)
+           : by_p && w.template draw_of_few<true>(top_k, top_p, min_w, u, mass_range, r))
+    return;
+  if (by_k) cut = w.template find<false>(cut, (double)top_k, range);
+  if (by_p) cut = w.template find<true>(cut, (double)top_p, mass_range);
+  w.draw(cut, min_w, u, r);
   cluster_sync();                   // (no CTA leaves while a peer may still reach into its shared memory)
 }
 
