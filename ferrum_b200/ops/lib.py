@@ -30,6 +30,16 @@ _lock = threading.Lock()
 ABI = 25
 
 
+# Entry points whose arguments ctypes converts itself, so that addresses and 64-bit sizes travel as plain integers (p: address or None, i: int,
+# l: long long, f: float).
+_KINDS = {"p": c_void_p, "i": c_int, "l": c_longlong, "f": c_float}
+_ARGUMENTS = {
+    "ferrum_rope_cache_write_packed": "piiipipppipipliiiiiiiipp",
+    "ferrum_unpack_cache": "pliipipipiiipp",
+    "ferrum_attention_packed": "pipiipliipippiiplpiiiifipp",
+    "ferrum_sample_filtered": "piiipppppppppp",
+}
+
 _CTYPES = (ctypes._SimpleCData, ctypes.Array, type(ctypes.byref(c_int())))
 
 
@@ -48,7 +58,7 @@ class _Library:
             try:
                 return fn(*args)
             except ctypes.ArgumentError:
-                return fn(*[a if a is None or isinstance(a, _CTYPES) else operator.index(a) for a in args])
+                return fn(*[a if a is None or isinstance(a, _CTYPES) or (fn.argtypes and isinstance(a, float)) else operator.index(a) for a in args])
         setattr(self, name, entry)
         return entry
 
@@ -67,6 +77,8 @@ def lib():
                 handle.ferrum_gemm_tc_workspace.restype = c_longlong
                 handle.ferrum_attention_packed_workspace.restype = c_longlong
                 handle.ferrum_matrix_memory_state_floats.restype = c_longlong
+                for name, kinds in _ARGUMENTS.items():
+                    getattr(handle, name).argtypes = [_KINDS[k] for k in kinds]
                 if handle.ferrum_kernels_abi() != ABI:
                     raise KernelError(f"{path} is a stale build; delete it and call again")
                 if os.environ.get("FERRUM_DEPENDENT_LAUNCH", "1") == "0":
@@ -212,6 +224,15 @@ def _ptr(t):
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _device_index = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def _at(t):
+    """A tensor's address for an entry point of `_ARGUMENTS`."""
+    return t.data_ptr() if t is not None else None
+
+
+def _stream_at():
+    return _raw_stream(_device_index()) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
 
 
 def _stream():
@@ -802,10 +823,10 @@ def rope_cache_write_packed(qkv, n_tokens, positions, req_of_token, block_table,
     global _work
     if _profile is not None:
         _work = (n_tokens * (2 * (2 * Hq + (2 * Hkv if write_kv else 0)) * D + (Hkv * 9 * D // 8 if write_kv else 0)), 0.0)
-    _check(lib().ferrum_rope_cache_write_packed(_ptr(qkv), dtype_code(qkv.dtype), n_tokens, qkv.stride(0), _ptr(q), q.stride(0), _ptr(positions),
-                                                _ptr(req_of_token), _ptr(block_table), block_table.shape[1], _ptr(cos_sin if R else None),
-                                                cos_sin.shape[0] if R else 0, _ptr(plane), c_longlong(page_stride), plane.shape[0], page_size,
-                                                Hq, Hkv, D, R, pairing, 1 if write_kv else 0, _ptr(err), _stream()), "rope_cache_write_packed")
+    _check(lib().ferrum_rope_cache_write_packed(_at(qkv), dtype_code(qkv.dtype), n_tokens, qkv.stride(0), _at(q), q.stride(0), _at(positions),
+                                                _at(req_of_token), _at(block_table), block_table.shape[1], _at(cos_sin if R else None),
+                                                cos_sin.shape[0] if R else 0, _at(plane), page_stride, plane.shape[0], page_size,
+                                                Hq, Hkv, D, R, pairing, 1 if write_kv else 0, _at(err), _stream_at()), "rope_cache_write_packed")
 
 
 def unpack_cache(plane, page_stride, page_size, block_table, items, out, err):
@@ -820,8 +841,8 @@ def unpack_cache(plane, page_stride, page_size, block_table, items, out, err):
     global _work
     if _profile is not None:
         _work = (n * Hkv * page_size * D * (9 / 8 + 4), 0.0)
-    _check(lib().ferrum_unpack_cache(_ptr(plane), c_longlong(page_stride), plane.shape[0], page_size, _ptr(block_table), block_table.shape[1],
-                                     _ptr(items), n, _ptr(out), dtype_code(out.dtype), Hkv, D, _ptr(err), _stream()), "unpack_cache")
+    _check(lib().ferrum_unpack_cache(_at(plane), page_stride, plane.shape[0], page_size, _at(block_table), block_table.shape[1],
+                                     _at(items), n, _at(out), dtype_code(out.dtype), Hkv, D, _at(err), _stream_at()), "unpack_cache")
 
 
 @functools.lru_cache(maxsize=None)
@@ -850,10 +871,10 @@ def attention_packed(q, out, n_tokens, block_table, q_start, pos0, plane, page_s
         raise KernelError("attention_packed: q_start, pos0, block_table and the rows do not agree")
     if not (q_start.is_contiguous() and pos0.is_contiguous() and part.is_contiguous() and counters.is_contiguous()):
         raise KernelError("attention_packed: q_start, pos0, part and counters must be contiguous")
-    _check(lib().ferrum_attention_packed(_ptr(q), q.stride(0), _ptr(out), out.stride(0), dtype_code(q.dtype), _ptr(plane), c_longlong(page_stride),
-                                         plane.shape[0], page_size, _ptr(block_table), block_table.shape[1], _ptr(q_start), _ptr(pos0), n_reqs,
-                                         n_tokens, _ptr(part), c_longlong(part.numel()), _ptr(counters), counters.numel(), Hq, Hkv, D, c_float(scale),
-                                         window, _ptr(err), _stream()),
+    _check(lib().ferrum_attention_packed(_at(q), q.stride(0), _at(out), out.stride(0), dtype_code(q.dtype), _at(plane), page_stride,
+                                         plane.shape[0], page_size, _at(block_table), block_table.shape[1], _at(q_start), _at(pos0), n_reqs,
+                                         n_tokens, _at(part), part.numel(), _at(counters), counters.numel(), Hq, Hkv, D, float(scale),
+                                         window, _at(err), _stream_at()),
            "attention_packed")
 
 
@@ -899,8 +920,8 @@ def sample_filtered(logits, n_rows, out_ids, err, temperature, top_k, top_p, min
     global _work
     if _profile is not None:
         _work = (n_rows * logits.shape[1] * 4, 0.0)
-    _check(lib().ferrum_sample_filtered(_ptr(logits), logits.stride(0), n_rows, logits.shape[1], _ptr(rows), _ptr(temperature), _ptr(top_k),
-                                        _ptr(top_p), _ptr(min_p), _ptr(uniform), _ptr(out_ids), _ptr(also_to), _ptr(err), _stream()),
+    _check(lib().ferrum_sample_filtered(_at(logits), logits.stride(0), n_rows, logits.shape[1], _at(rows), _at(temperature), _at(top_k),
+                                        _at(top_p), _at(min_p), _at(uniform), _at(out_ids), _at(also_to), _at(err), _stream_at()),
            "sample_filtered")
 
 
