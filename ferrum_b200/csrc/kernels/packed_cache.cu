@@ -1,9 +1,9 @@
 // Writing a cache held in 4 bits (packed_cache.cuh has the layout), and bringing pages back to 16 bits.
 //
 // The write turns the queries and keys by the rotary table and quantises keys and values group by group of 64 elements:
-//   lo, hi = min, max;   step = r16(hi / 15 - lo / 15);   middle = r16(lo + 8 step);   code = clamp(rint((x - middle) / step) + 8, 0, 15)
-// with r16 the rounding to the cache's 16-bit type: codes are made against the pair that is stored.  (hi / 15 - lo / 15 and not
-// (hi - lo) / 15: the range of a bfloat16 row may not fit a float32.)  step 0: code 8, the middle itself.  A group that holds a NaN
+//   lo, hi = min, max;   step = r16(hi f - lo f), f = 1/15 in float32;   middle = r16(lo + 8 step);   code = clamp(rint((x - middle) / step) + 8, 0, 15)
+// with r16 the rounding to the cache's 16-bit type: codes are made against the pair that is stored.  (hi f - lo f and not
+// (hi - lo) f: the range of a bfloat16 row may not fit a float32.)  step 0: code 8, the middle itself.  A group that holds a NaN
 // or an infinity gets a NaN for both, as such an element would poison its row of a 16-bit cache.  Every operation is a single
 // float32 one, rounded on its own: the codes of a key follow from the definition alone.  (lo + 8 step is one fused operation: 8 step is exact, but
 // for the largest bfloat16 values it is beyond float32.)
@@ -16,43 +16,65 @@ namespace {
 template <typename T>
 __device__ __forceinline__ float r16(float v) { return to_f32<T>(from_f32<T>(v)); }
 
-// One warp per (token, head slot); slots are Hq query heads, Hkv key heads, Hkv value heads.  Lane l owns elements l*E .. l*E + E - 1.
-template <typename T, int D>
+template <typename T, int N> struct Elements { T v[N]; };
+
+// One warp per (token, head slot); slots are Hq query heads, Hkv key heads, Hkv value heads.  Lane l owns elements l*E .. l*E + E - 1.  WIDE:
+// it reads them, and those that they are turned with, in one piece (rows and halves aligned to E elements).
+template <typename T, int D, bool WIDE>
 __global__ void __launch_bounds__(256)
 packed_write_kernel(const T* __restrict__ qkv, int ld, T* __restrict__ q_out, int ldq, const int* __restrict__ positions,
                     const int* __restrict__ req_of_token, const int* __restrict__ block_table, int table_width,
                     const float* __restrict__ cos_sin, int n_pos, uint8_t* __restrict__ plane, long long page_stride, int n_pages,
-                    int page_size, int Hq, int Hkv, int R, int pairing, int write_kv, int n_tokens, int* __restrict__ err) {
+                    int page_size, int Hq, int Hkv, int R, int pairing, int write_kv, int* __restrict__ err) {
   constexpr int E = D / 32;
   using B = PackedBlock<D>;
-  pdl_launch();
+  using Piece = Elements<T, E>;
   pdl_wait();
+  pdl_launch();
   const int slots = Hq + (write_kv ? 2 * Hkv : 0);
-  const long long w = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (w >= (long long)n_tokens * slots) return;
-  const int t = (int)(w / slots), slot = (int)(w % slots), lane = threadIdx.x & 31;
+  const int t = blockIdx.x, slot = blockIdx.y * (blockDim.x >> 5) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (slot >= slots) return;
   const T* src = qkv + (size_t)t * ld + (size_t)slot * D;
+  float x[E];
+  if (WIDE) {
+    alignas(8) Piece p = *reinterpret_cast<const Piece*>(__builtin_assume_aligned(src + lane * E, 2 * E));
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = to_f32<T>(p.v[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = to_f32<T>(src[lane * E + e]);
+  }
   const int pos = positions[t], half = R >> 1;
   if (pos < 0 || (half > 0 && pos >= n_pos)) {
     if (lane == 0) atomicExch(err, 2);
     return;
   }
-  float x[E];
+  if (slot < Hq + Hkv && half > 0) {
+    const float2* cs = reinterpret_cast<const float2*>(cos_sin) + (size_t)pos * half;
+    float y[E], other[E];
+    const int d0 = lane * E;
+    if (pairing == 0) {
 #pragma unroll
-  for (int e = 0; e < E; ++e) x[e] = to_f32<T>(src[lane * E + e]);
-  if (slot < Hq + Hkv) {
-    const float* cs = cos_sin + (size_t)pos * R;
-    float y[E];
+      for (int e = 0; e < E; ++e) other[e] = x[e ^ 1];
+    } else if (WIDE) {
+      alignas(8) Piece p = *reinterpret_cast<const Piece*>(__builtin_assume_aligned(src + (d0 < half ? d0 + half : d0 < R ? d0 - half : d0), 2 * E));
+#pragma unroll
+      for (int e = 0; e < E; ++e) other[e] = to_f32<T>(p.v[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int d = d0 + e;
+        other[e] = to_f32<T>(src[d < half ? d + half : d < R ? d - half : d]);
+      }
+    }
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int d = lane * E + e;
+      const int d = d0 + e;
       y[e] = x[e];
       if (d < R) {
         const bool first = pairing == 0 ? (d & 1) == 0 : d < half;
-        const int i = pairing == 0 ? d >> 1 : (first ? d : d - half);
-        const float other = to_f32<T>(src[pairing == 0 ? d ^ 1 : (first ? d + half : d - half)]);
-        const float c = cs[2 * i], s = cs[2 * i + 1];
-        y[e] = first ? __fsub_rn(__fmul_rn(x[e], c), __fmul_rn(other, s)) : __fadd_rn(__fmul_rn(other, s), __fmul_rn(x[e], c));
+        const float2 c = cs[pairing == 0 ? d >> 1 : (first ? d : d - half)];
+        y[e] = first ? __fsub_rn(__fmul_rn(x[e], c.x), __fmul_rn(other[e], c.y)) : __fadd_rn(__fmul_rn(other[e], c.y), __fmul_rn(x[e], c.x));
       }
     }
     __syncwarp();      // q_out may be the row that the other lanes just read
@@ -61,8 +83,15 @@ packed_write_kernel(const T* __restrict__ qkv, int ld, T* __restrict__ q_out, in
   }
   if (slot < Hq) {
     T* dst = q_out + (size_t)t * ldq + (size_t)slot * D + lane * E;
+    if (WIDE) {
+      alignas(8) Piece p;
 #pragma unroll
-    for (int e = 0; e < E; ++e) dst[e] = from_f32<T>(x[e]);
+      for (int e = 0; e < E; ++e) p.v[e] = from_f32<T>(x[e]);
+      *reinterpret_cast<Piece*>(__builtin_assume_aligned(dst, 2 * E)) = p;
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) dst[e] = from_f32<T>(x[e]);
+    }
     return;
   }
   const int lp = pos / page_size;
@@ -91,7 +120,7 @@ packed_write_kernel(const T* __restrict__ qkv, int ld, T* __restrict__ q_out, in
     hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     wrong |= (bool)__shfl_xor_sync(0xffffffffu, (int)wrong, o);
   }
-  float step = r16<T>(__fsub_rn(__fdiv_rn(hi, 15.f), __fdiv_rn(lo, 15.f)));
+  float step = r16<T>(__fsub_rn(__fmul_rn(hi, 1.f / 15.f), __fmul_rn(lo, 1.f / 15.f)));
   float middle = r16<T>(fmaf(8.f, step, lo));
   if (wrong) step = middle = __int_as_float(0x7fc00000);
   unsigned codes = 0;
@@ -121,8 +150,8 @@ __global__ void __launch_bounds__(256)
 unpack_kernel(const uint8_t* __restrict__ plane, long long page_stride, int n_pages, int page_size, const int* __restrict__ block_table,
               int table_width, const int* __restrict__ items, T* __restrict__ out, int Hkv, int* __restrict__ err) {
   using B = PackedBlock<D>;
-  pdl_launch();
   pdl_wait();
+  pdl_launch();
   const int item = blockIdx.x, h = blockIdx.y;
   const int req = items[2 * item], lp = items[2 * item + 1];
   const int page = lp >= 0 && lp < table_width ? block_table[(size_t)req * table_width + lp] : -1;
@@ -168,16 +197,17 @@ FERRUM_API int ferrum_rope_cache_write_packed(const void* qkv, int dtype, int n_
                    "rope_packed: page size %d must be a multiple of %d, and the cache given", page_size, PACKED_POS);
   FERRUM_CHECK_ARG(((uintptr_t)plane & 15) == 0 && page_stride % 16 == 0, "rope_packed: pages must be 16-byte aligned");
   if (n_tokens == 0) return 0;
-  const long long warps = (long long)n_tokens * (Hq + (write_kv ? 2 * Hkv : 0));
-  const long long blocks = (warps + 7) / 8;
-  FERRUM_CHECK_ARG(blocks <= 0x7fffffffLL, "rope_packed: too many tokens");
+  const int slots = Hq + (write_kv ? 2 * Hkv : 0), E = D / 32;
+  const dim3 grid(n_tokens, (slots + 7) / 8);
+  FERRUM_CHECK_ARG(grid.y <= 65535, "rope_packed: too many heads");
+  const bool wide = ld % E == 0 && ldq % E == 0 && (((uintptr_t)qkv | (uintptr_t)q_out) & (2 * E - 1)) == 0 && (pairing == 0 || R / 2 % E == 0);
   auto launch = [&](auto kernel, auto* x, auto* q) {
-    launch_kernel(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, x, ld, q, ldq, positions, req_of_token, block_table, table_width, cos_sin,
-                  n_pos, (uint8_t*)plane, page_stride, n_pages, page_size, Hq, Hkv, R, pairing, write_kv, n_tokens, err_flag);
+    launch_kernel(kernel, grid, dim3(256), 0, stream, x, ld, q, ldq, positions, req_of_token, block_table, table_width, cos_sin, n_pos, (uint8_t*)plane,
+                  page_stride, n_pages, page_size, Hq, Hkv, R, pairing, write_kv, err_flag);
   };
   FERRUM_DISPATCH_16BIT(dtype, T, {
-    if (D == 64) launch(packed_write_kernel<T, 64>, (const T*)qkv, (T*)q_out);
-    else launch(packed_write_kernel<T, 128>, (const T*)qkv, (T*)q_out);
+    if (D == 64) wide ? launch(packed_write_kernel<T, 64, true>, (const T*)qkv, (T*)q_out) : launch(packed_write_kernel<T, 64, false>, (const T*)qkv, (T*)q_out);
+    else wide ? launch(packed_write_kernel<T, 128, true>, (const T*)qkv, (T*)q_out) : launch(packed_write_kernel<T, 128, false>, (const T*)qkv, (T*)q_out);
   });
   FERRUM_CHECK_LAUNCH("rope_cache_write_packed");
   return 0;

@@ -11,7 +11,8 @@ def quantise(x, dtype):
     """x float32 [..., D] -> (codes int64 [..., D], step, middle of the 16-bit type [..., D / 64]) by the definition, a float32 operation at a time."""
     g = x.unflatten(-1, (-1, 64))
     lo, hi = g.min(-1).values, g.max(-1).values
-    step = (hi / 15 - lo / 15).to(dtype)
+    f = torch.tensor(1 / 15, dtype=torch.float32, device=x.device)
+    step = (hi * f - lo * f).to(dtype)
     mid = (lo + 8 * step.float()).to(dtype)
     bad = ~torch.isfinite(g).all(-1)
     step[bad], mid[bad] = math.nan, math.nan
