@@ -15,10 +15,11 @@
 // 2^-30 below the largest); p step, times a power of two that follows the largest step seen, is rounded to float16: a weight's half
 // step of 2^-12, and the result's own.  All sums are float32.
 //
-// The work is handed out on the device: all (request, KV head, rows of 8 NT, 64 keys) units form one line, and CTA c of P takes the units
-// [c U / P, (c + 1) U / P): the launch does not depend on the lengths, so that a captured one serves any.  A CTA's four warps take every
-// fourth block of 16 positions; a block is one bulk copy into the warp's own ring of stages, and no warp waits for another until
-// its part of a (request, head) is done.  Of the CTAs that share a (request, head) the one that comes last adds up the parts, in a fixed order.
+// The work is handed out on the device, so that the launch does not depend on the lengths and a captured one serves any.  A (request, KV head,
+// rows of 8 NT) is a pair.  Few pairs (at most half the CTAs): each gets a number of CTAs of its own by its length, one part a CTA, as a
+// part costs some 4 us beside its keys.  Many: their units of 64 keys form one line, and CTA c of P takes the units [c U / P, (c + 1) U / P).
+// A CTA's four warps take every fourth block of 16 positions; a block is one bulk copy into the warp's own ring of stages, and no
+// warp waits for another until its part is done; the first copies of the next part are on their way by then.  Of the CTAs that share a (request, head) the one that comes last adds up the parts, in a fixed order.
 #include "packed_cache.cuh"
 #include "ptx_sm100.cuh"
 
@@ -137,25 +138,23 @@ __device__ __forceinline__ void write_row4(const PackedParams& p, int token, int
   *reinterpret_cast<uint2*>((T*)p.out + (size_t)token * p.ldo + (size_t)head * D + d) = r;
 }
 
-// One CTA's share of the units of (request r, KV head kvh, row tile rt): tiles [t0, t1).
-template <typename T, int D, int NT>
-__device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kvh, int rt, int key_lo, int t0, int t1, const Parts parts, uint8_t* ring,
-                                            uint32_t bars, uint32_t& turn, float* merge, bool& failed) {
-  using B = PackedBlock<D>;
-  constexpr int GN = B::GROUPS;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tig = lane & 3;
-  const int qs = p.q_start[r], n_rows = (p.q_start[r + 1] - qs) * p.G, pos0 = p.pos0[r];
-  const int row0 = rt * 8 * NT;
-  const int hi = pos0 + p.q_start[r + 1] - qs;                       // one past the last key
-  const int b_end = min((hi - key_lo + PACKED_POS - 1) / PACKED_POS, t1 * WARPS);
-  const int b0 = t0 * WARPS + warp;                                   // the warp's blocks: b0, b0 + WARPS, ... below b_end
-  const int n_blocks = b0 < b_end ? (b_end - b0 + WARPS - 1) / WARPS : 0;
-  const int* bt = p.block_table + (size_t)r * p.table_width;
-  const uint8_t* head = p.plane + (size_t)kvh * (p.page_size / PACKED_POS) * B::BYTES;
+// A CTA's part of a pair: blocks [q0, q1) of 16 positions from key_lo on.
+struct Item {
+  int r, kvh, rt, key_lo, q0, q1;
+  Parts parts;
+};
 
-  // ---- where the warp's next 32 blocks lie, one a lane, which also asks for its copy when the step's turn comes
-  const uint8_t* my_src = head;
-  auto find_blocks = [&](int i) {      // blocks i .. i + 31 of the warp
+// A warp's way through the blocks of an item: b0, b0 + WARPS, ..., n_blocks of them.  Where the next 32 of them lie is kept one a lane, which also asks
+// for its copy when its step's turn comes.
+template <int D>
+struct Flow {
+  using B = PackedBlock<D>;
+  const int* bt;
+  const uint8_t* head;
+  const uint8_t* my_src;
+  int key_lo, b0, n_blocks;
+
+  __device__ __forceinline__ void find(const PackedParams& p, int i, int lane) {      // blocks i .. i + 31 of the warp
     const int k = i + lane;
     if (k < n_blocks) {
       const int key = key_lo + (b0 + k * WARPS) * PACKED_POS, lp = key / p.page_size;
@@ -166,16 +165,41 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
       }
       my_src = head + (size_t)page * p.page_stride + (size_t)((key - lp * p.page_size) / PACKED_POS) * B::BYTES;
     }
-  };
-  auto request = [&](int j) {          // the copies of step j: blocks NB j .. NB j + NB - 1, those that there are
-    if ((NB * j & 31) == 0) find_blocks(NB * j);
-    const uint32_t half = (turn + j) % HALVES, bar = bars + 8 * half;
+  }
+  // the copies of step j (blocks NB j .. NB j + NB - 1, those that there are), the warp's step number `turn`
+  __device__ __forceinline__ void request(const PackedParams& p, int j, uint32_t turn, uint8_t* ring, uint32_t bars, int lane) {
+    if ((NB * j & 31) == 0) find(p, NB * j, lane);
+    const uint32_t half = turn % HALVES, bar = bars + 8 * half;
     const int b = lane - (NB * j & 31), n = min(NB, n_blocks - NB * j);
     if (b == 0) sm100::mbar_expect_tx(bar, n * B::BYTES);
     if (b >= 0 && b < n) bulk_load(sm100::smem_u32(ring + (half * NB + b) * B::BYTES), my_src, B::BYTES, bar);
-  };
-  const int n_steps = (n_blocks + NB - 1) / NB;
-  for (int j = 0; j < min(HALVES, n_steps); ++j) request(j);
+  }
+  __device__ __forceinline__ int steps() const { return (n_blocks + NB - 1) / NB; }
+  __device__ __forceinline__ void begin(const PackedParams& p, const Item& it, uint32_t turn, uint8_t* ring, uint32_t bars) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    bt = p.block_table + (size_t)it.r * p.table_width;
+    head = p.plane + (size_t)it.kvh * (p.page_size / PACKED_POS) * B::BYTES;
+    my_src = head;
+    key_lo = it.key_lo;
+    b0 = it.q0 + warp;
+    n_blocks = b0 < it.q1 ? (it.q1 - b0 + WARPS - 1) / WARPS : 0;
+    for (int j = 0; j < min(HALVES, steps()); ++j) request(p, j, turn + j, ring, bars, lane);
+  }
+};
+
+// One item, whose first copies are on their way; next() sends the next item's.
+template <typename T, int D, int NT, typename Next>
+__device__ __forceinline__ void packed_item(const PackedParams& p, const Item it, Flow<D>& flow, uint8_t* ring, uint32_t bars, uint32_t& turn, float* merge,
+                                            bool& failed, Next next) {
+  using B = PackedBlock<D>;
+  constexpr int GN = B::GROUPS;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tig = lane & 3;
+  const int r = it.r, kvh = it.kvh, rt = it.rt;
+  const Parts parts = it.parts;
+  const int qs = p.q_start[r], n_rows = (p.q_start[r + 1] - qs) * p.G, pos0 = p.pos0[r];
+  const int row0 = rt * 8 * NT;
+  const int hi = pos0 + p.q_start[r + 1] - qs;                       // one past the last key
+  const int n_blocks = flow.n_blocks, n_steps = flow.steps();
 
   // ---- the rows' queries as float16 operands, their sums per group and their scale
   unsigned qf[NT][GN][4][2];
@@ -470,7 +494,7 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
         }
   };
   // whole blocks, by their number in the warp: [k_lo, k_hi) hide no key from any row
-  const int base = key_lo + b0 * PACKED_POS;
+  const int base = flow.key_lo + flow.b0 * PACKED_POS;
   const int k_lo = all_lo > base ? (all_lo - base + TILE - 1) / TILE : 0, k_hi = all_hi - PACKED_POS + 1 >= base ? (all_hi - PACKED_POS + 1 - base) / TILE + 1 : 0;
   for (int j = 0; j < n_steps; ++j) {
     const uint32_t half = (turn + j) % HALVES;
@@ -480,11 +504,12 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
     else step_of(std::true_type{}, first, base + NB * j * TILE, n_blocks - NB * j);
     if (j % SETTLE == SETTLE - 1) settle();
     __syncwarp();                      // the half is free
-    if (j + HALVES < n_steps) request(j + HALVES);
+    if (j + HALVES < n_steps) flow.request(p, j + HALVES, turn + j + HALVES, ring, bars, lane);
   }
   settle();
   turn += n_steps;
   if (failed) atomicExch(p.err, 29);
+  next();
 
   // ---- the warps' parts meet, eight rows at a time
   const float down = 1.f / v_up;
@@ -543,47 +568,75 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, int r, int kv
   if (parts.n == 1) return;
   // ---- the last CTA to come adds the parts up
   __shared__ int s_last;
-  __threadfence();
   __syncthreads();
   if (tid == 0) {
     int* count = p.counters + ((size_t)r * p.Hkv + kvh) * 2 + rt;
+    __threadfence();                   // (the block's stores lie before it by the barrier)
     s_last = atomicAdd(count, 1) == parts.n - 1;
     if (s_last) *count = 0;
     __threadfence();
   }
   __syncthreads();
   if (!s_last) return;
-  constexpr int GROUP = 16;            // parts whose loads are in flight together
-  for (int idx = tid; idx < min(8 * NT, n_rows - row0) * (D / 4); idx += WARPS * 32) {
-    const int rr = idx / (D / 4), d = idx % (D / 4) * 4, row = row0 + rr;
-    float M = -INFINITY, L = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i0 = 0; i0 < parts.n; i0 += GROUP) {
-      float2 ml[GROUP];
-      float4 v[GROUP];
+  // CHUNK parts at a time: a warp a row forms the parts' factors, then a thread adds four elements of a row over the parts, all loads in flight
+  constexpr int CHUNK = 64, ITEMS = 8 * NT * (D / 4) / (WARPS * 32), GROUP = 16;
+  const int rows = min(8 * NT, n_rows - row0);
+  float* factor = merge;               // [8 NT][CHUNK]
+  float* state = merge + 8 * NT * CHUNK;      // [8 NT][3]: maximum, sum, what becomes of the sums so far
+  float4 acc[ITEMS];
 #pragma unroll
-      for (int i = 0; i < GROUP; ++i) {
-        const bool have = i0 + i < parts.n;
-        const size_t at = (size_t)parts.slot(have ? i0 + i : 0) * PART_ROWS + rr;
-        ml[i] = have ? __ldcg(reinterpret_cast<const float2*>(p.part_ml + at * 2)) : make_float2(-INFINITY, 0.f);
-        v[i] = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * D + d));
+  for (int i = 0; i < ITEMS; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int first = 0; first < parts.n; first += CHUNK) {
+    const int n = min(CHUNK, parts.n - first);
+    for (int rr = warp; rr < rows; rr += WARPS) {
+      float2 ml[CHUNK / 32];
+      float m_run = first ? state[rr * 3] : -INFINITY, m_new = m_run;
+#pragma unroll
+      for (int k = 0; k < CHUNK / 32; ++k) {
+        const int i = lane + 32 * k;
+        ml[k] = i < n ? __ldcg(reinterpret_cast<const float2*>(p.part_ml + ((size_t)parts.slot(first + i) * PART_ROWS + rr) * 2)) : make_float2(-INFINITY, 0.f);
+        m_new = fmaxf(m_new, ml[k].x);
       }
-      float m_new = M;
+      m_new = warp_max(m_new);
+      float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < GROUP; ++i) m_new = fmaxf(m_new, ml[i].x);
-      const float keep = M == -INFINITY ? 0.f : exp2f(M - m_new);
-      L *= keep;
-      acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
-#pragma unroll
-      for (int i = 0; i < GROUP; ++i) {
-        if (ml[i].x == -INFINITY && ml[i].y == 0.f) continue;      // (no key of the part was seen by the row)
-        const float f = exp2f(ml[i].x - m_new);
-        L += ml[i].y * f;
-        acc.x += v[i].x * f; acc.y += v[i].y * f; acc.z += v[i].z * f; acc.w += v[i].w * f;
+      for (int k = 0; k < CHUNK / 32; ++k) {
+        const float f = ml[k].x == -INFINITY && ml[k].y == 0.f ? 0.f : exp2f(ml[k].x - m_new);      // (a part of which the row sees no key: zeros)
+        sum += ml[k].y * f;
+        factor[rr * CHUNK + lane + 32 * k] = f;
       }
-      M = m_new;
+      sum = warp_sum(sum);
+      if (lane == 0) {
+        const float keep = m_run == -INFINITY ? 0.f : exp2f(m_run - m_new);
+        state[rr * 3 + 1] = first ? state[rr * 3 + 1] * keep + sum : sum;
+        state[rr * 3 + 2] = keep;
+        state[rr * 3] = m_new;
+      }
     }
-    write_row4<T>(p, qs + row / p.G, kvh * p.G + row % p.G, D, d, acc, L);
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+      const int idx = tid + k * WARPS * 32, rr = idx / (D / 4), d = idx % (D / 4) * 4;
+      if (rr >= rows) continue;
+      const float keep = state[rr * 3 + 2];
+      acc[k].x *= keep; acc[k].y *= keep; acc[k].z *= keep; acc[k].w *= keep;
+      for (int i0 = 0; i0 < n; i0 += GROUP) {
+        float4 v[GROUP];
+#pragma unroll
+        for (int i = 0; i < GROUP; ++i) v[i] = __ldcg(reinterpret_cast<const float4*>(p.part_o + ((size_t)parts.slot(first + min(i0 + i, n - 1)) * PART_ROWS + rr) * D + d));
+#pragma unroll
+        for (int i = 0; i < GROUP; ++i) {
+          const float f = factor[rr * CHUNK + i0 + i];      // (0 behind the last part)
+          acc[k].x += v[i].x * f; acc[k].y += v[i].y * f; acc[k].z += v[i].z * f; acc[k].w += v[i].w * f;
+        }
+      }
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    const int idx = tid + k * WARPS * 32, rr = idx / (D / 4), d = idx % (D / 4) * 4, row = row0 + rr;
+    if (rr < rows) write_row4<T>(p, qs + row / p.G, kvh * p.G + row % p.G, D, d, acc[k], state[rr * 3 + 1]);
   }
 }
 
@@ -605,12 +658,12 @@ attention_packed_kernel(const PackedParams p) {
   sm100::fence_proxy_async();
   pdl_wait();
   pdl_launch();
-  // ---- the line's length, then the request in which the CTA's share begins (up to 128 requests: one look at their lengths)
-  long long U = 0, mine = 0, at = 0;
-  auto scan = [&](int base) {          // requests base .. base + 127, one a thread: mine, and the units before it in `at`; their sum is added to U
+  // ---- the CTA's first item.  count(r, span): what request r adds to a line; the sums before each thread's request, 128 requests at a time.
+  const long long c = blockIdx.x;
+  long long mine = 0, at = 0, line = 0;
+  auto scan = [&](int base, auto count) {
     const int r = base + tid;
-    const Span sp = r < p.n_reqs ? span_of<NT>(p, r) : Span{0, 0, 0};
-    mine = (long long)sp.tiles * sp.row_tiles * p.Hkv;
+    mine = r < p.n_reqs ? count(span_of<NT>(p, r)) : 0;
     long long u = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -620,51 +673,85 @@ attention_packed_kernel(const PackedParams p) {
     __syncthreads();
     if (lane == 31) s_scan[warp] = u;
     __syncthreads();
-    at = U + u - mine;
+    at = line + u - mine;
     for (int w = 0; w < WARPS; ++w) {
       if (w < warp) at += s_scan[w];
-      U += s_scan[w];
+      line += s_scan[w];
     }
   };
-  for (int base = 0; base < p.n_reqs; base += WARPS * 32) scan(base);
-  const long long P = min((long long)gridDim.x, U), all_units = U;
-  const long long c = blockIdx.x;
-  if (c >= P) return;
-  const long long first = c * all_units / P, last = (c + 1) * all_units / P;
-  if (p.n_reqs > WARPS * 32) U = 0;
+  // units in the low 40 bits, pairs above
+  for (int base = 0; base < p.n_reqs; base += WARPS * 32)
+    scan(base, [&](const Span sp) { return (long long)sp.tiles * sp.row_tiles * p.Hkv + ((long long)(sp.tiles ? sp.row_tiles * p.Hkv : 0) << 40); });
+  const long long U = line & ((1ll << 40) - 1), N = line >> 40;
+  if (U == 0) return;
+  const bool own = 2 * N <= gridDim.x;
+  const long long P = min((long long)gridDim.x, U);
+  // CTAs that a pair of its own gets: their sum over all pairs is at most N + (P - N)
+  auto ctas_of = [&](const Span sp) { return sp.tiles ? (int)min((long long)sp.tiles, 1 + (long long)sp.tiles * max(0ll, P - N) / U) : 0; };
+  const long long first = own ? c : c * U / P, last = own ? c + 1 : (c + 1) * U / P;
+  if (!own && c >= P) return;
+  if (tid == 0) s_req = -1;
+  line = 0;
   for (int base = 0; base < p.n_reqs; base += WARPS * 32) {
-    if (p.n_reqs > WARPS * 32) scan(base);
+    scan(base, [&](const Span sp) { return (long long)(own ? ctas_of(sp) : sp.tiles) * sp.row_tiles * p.Hkv; });
     if (first >= at && first < at + mine) {
       s_req = base + tid;
       s_start = at;
     }
+    if (line > first) break;
   }
-  U = all_units;
   __syncthreads();
+  if (s_req < 0) return;
+  int r = s_req;
+  long long u = first, start = s_start;
+  auto next_item = [&](Item& it) {
+    if (u >= last) return false;
+    Span sp = span_of<NT>(p, r);
+    while (u >= start + (long long)(own ? ctas_of(sp) : sp.tiles) * sp.row_tiles * p.Hkv) {
+      start += (long long)(own ? ctas_of(sp) : sp.tiles) * sp.row_tiles * p.Hkv;
+      sp = span_of<NT>(p, ++r);
+    }
+    const int each = own ? ctas_of(sp) : sp.tiles, pair = (int)((u - start) / each), i = (int)((u - start) % each);
+    const int blocks = (p.pos0[r] + p.q_start[r + 1] - p.q_start[r] - sp.lo + PACKED_POS - 1) / PACKED_POS;
+    it.r = r;
+    it.kvh = pair / sp.row_tiles;
+    it.rt = pair % sp.row_tiles;
+    it.key_lo = sp.lo;
+    if (own) {
+      it.q0 = (int)((long long)i * blocks / each);
+      it.q1 = (int)((long long)(i + 1) * blocks / each);
+      it.parts = Parts{(int)c - i, each, 0};
+      u = last;
+      return true;
+    }
+    const long long pair_start = start + (long long)pair * each, pair_end = pair_start + each, until = min(pair_end, last);
+    it.q0 = i * WARPS;
+    it.q1 = min(blocks, (int)(until - pair_start) * WARPS);
+    // the CTAs of the pair's first and last units: the largest k with k U / P <= that unit
+    const int k0 = (int)(((pair_start + 1) * P - 1) / U), k1 = (int)((pair_end * P - 1) / U);
+    it.parts = Parts{k0, k1 - k0 + 1, k0 * U / P == pair_start ? 0 : 1};
+    u = until;
+    return true;
+  };
   // ---- walk the share
   uint32_t turn = 0;      // steps that the warp has run: a step's half of the ring and its barrier's phase follow from its number
   bool failed = false;
-  long long u = first, start = s_start;
-  for (int r = s_req; u < last; ++r) {
-    const Span sp = span_of<NT>(p, r);
-    const long long all = (long long)sp.tiles * sp.row_tiles * p.Hkv;
-    while (u < last && u < start + all) {
-      const int pair = (int)((u - start) / sp.tiles), t0 = (int)((u - start) % sp.tiles);
-      const long long pair_start = start + (long long)pair * sp.tiles, pair_end = pair_start + sp.tiles;
-      const int t1 = (int)(min(pair_end, last) - pair_start);
-      const int kvh = pair / sp.row_tiles, rt = pair % sp.row_tiles;
-      // the CTAs of the pair's first and last units: the largest k with k U / P <= that unit
-      const int k0 = (int)(((pair_start + 1) * P - 1) / U), k1 = (int)((pair_end * P - 1) / U);
-      const Parts parts{k0, k1 - k0 + 1, k0 * U / P == pair_start ? 0 : 1};
-      packed_item<T, D, NT>(p, r, kvh, rt, sp.lo, t0, t1, parts, ring, bars, turn, merge, failed);
-      u = pair_start + t1;
-    }
-    start += all;
+  Flow<D> flow;
+  Item it, following;
+  bool more = next_item(it);
+  flow.begin(p, it, turn, ring, bars);
+  while (more) {
+    packed_item<T, D, NT>(p, it, flow, ring, bars, turn, merge, failed, [&]() {
+      more = next_item(following);
+      if (more) flow.begin(p, following, turn, ring, bars);
+    });
+    it = following;
   }
 }
 
 template <typename T, int D, int NT>
 int launch_packed(const PackedParams& p, cudaStream_t stream) {
+  static_assert(8 * NT * (64 + 3) <= WARPS * 8 * (D + 2), "the parts' factors lie where the warps' sums did");
   constexpr int smem = WARPS * HALVES * NB * PackedBlock<D>::BYTES + WARPS * 8 * (D + 2) * 4;
   static bool configured = false;
   if (!configured) {

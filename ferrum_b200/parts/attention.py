@@ -119,7 +119,7 @@ class PagedAttention(Mixer):
         into a scratch plane, which the kernels of prompt portions then read in the cache's place."""
         Hq, Hkv, D = self.Hq, self.Hkv, self.D
         few, G = ops.attention_packed_rows(), Hq // Hkv
-        if min(ctx.h_q_len) * G <= few:
+        if any(0 < n * G <= few for n in ctx.h_q_len):
             part = ctx.buf("attn_packed_part", (ops.attention_packed_workspace(D),), torch.float32)
             if ops.profiling():      # (a step with prompt portions counts the whole step's work for each kernel)
                 ops.set_work(ops.attention_work(ctx, Hq, Hkv, D, self.window, 9 / 16))

@@ -126,6 +126,8 @@ class Step:
     def check(self, out, what=""):
         row, D = 0, self.cache.D
         for r, (p, n) in enumerate(zip(self.past, self.new)):
+            if n == 0:
+                continue
             q = self.qkv[row:row + n, :self.Hq * D].view(n, self.Hq, D)
             few = n * (self.Hq // self.cache.Hkv) <= 16
             want, bound = attention(q, self.cache.keys[r], self.cache.vals[r], self.cache.mids[r], p, self.mixer.scale, self.window,

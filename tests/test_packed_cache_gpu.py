@@ -148,7 +148,11 @@ DECODE = [([1], [1], 4, 2, 64, 16, 0), ([16, 17, 15, 1, 2], [1] * 5, 8, 1, 128, 
           ([700], [1], 32, 8, 128, 16, 0), ([300, 5, 2049], [1] * 3, 16, 1, 64, 64, 0), ([40, 333], [1, 3], 4, 1, 128, 48, 0),
           ([90, 200, 16], [16, 5, 16], 2, 2, 64, 16, 0), ([90, 200, 31], [2, 1, 2], 14, 2, 128, 32, 0), ([500, 20, 77], [1] * 3, 8, 4, 128, 16, 30),
           ([500, 20, 77, 600], [4] * 4, 8, 4, 64, 16, 1), ([900, 3, 128], [3, 3, 1], 5, 1, 128, 16, 100), ([5000, 40], [1] * 2, 4, 4, 128, 32, 3000),
-          ([20000], [1], 8, 2, 128, 64, 0), ([260] * 40, [1] * 40, 8, 8, 64, 16, 0)]
+          ([20000], [1], 8, 2, 128, 64, 0), ([260] * 40, [1] * 40, 8, 8, 64, 16, 0),
+          # more requests than a block has threads, with fewer and with more (request, head) pairs than CTAs; a long context among short ones;
+          # rows in two tiles of eight
+          ([1 + 7 * i % 90 for i in range(200)], [1] * 200, 4, 1, 64, 16, 0), ([1 + 13 * i % 200 for i in range(300)], [1] * 300, 6, 3, 128, 16, 0),
+          ([30000] + [50] * 30, [1] * 31, 8, 2, 64, 64, 0), ([9000] + [70] * 100, [1] * 101, 8, 8, 128, 32, 0), ([4000, 3, 50, 900], [2, 0, 0, 1], 8, 1, 64, 16, 0)]
 
 
 @pytest.mark.parametrize("dtype", H.DTYPES)
@@ -159,7 +163,7 @@ def test_decoded_tokens(cuda, dtype, case):
     out = s.attend()
     assert s.ctx.err.item() == 0
     s.check(out, f"case {case}")
-    assert torch.equal(out, s.attend())                       # the same twice
+    assert torch.equal(out, s.attend()) and not any(t.any() for t in s.ctx._zeros.values())        # the same twice, the counters left as they were
 
 
 PROMPT = [([40], [40], 8, 2, 64, 16, 0), ([300], [300], 4, 4, 128, 16, 0), ([700, 90, 33], [200, 90, 17], 8, 8, 128, 32, 0),
