@@ -138,6 +138,12 @@ __device__ __forceinline__ void write_row4(const PackedParams& p, int token, int
   *reinterpret_cast<uint2*>((T*)p.out + (size_t)token * p.ldo + (size_t)head * D + d) = r;
 }
 
+// How the work is shared out: units and pairs in all, CTAs, the CTA's own stretch of the line (of units, or of parts where pairs have CTAs of their own).
+struct Way {
+  long long U, P, N, first, last;
+  bool own;
+};
+
 // A CTA's part of a pair: blocks [q0, q1) of 16 positions from key_lo on.
 struct Item {
   int r, kvh, rt, key_lo, q0, q1;
@@ -646,8 +652,9 @@ attention_packed_kernel(const PackedParams p) {
   using B = PackedBlock<D>;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) unsigned long long bars_mem[WARPS * HALVES];
-  __shared__ long long s_scan[WARPS], s_start;
-  __shared__ int s_req;
+  __shared__ long long s_scan[WARPS];
+  __shared__ int s_req, s_begin;
+  __shared__ Way way;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint8_t* ring = smem + warp * HALVES * NB * B::BYTES;
   float* merge = reinterpret_cast<float*>(smem + WARPS * HALVES * NB * B::BYTES);
@@ -658,79 +665,98 @@ attention_packed_kernel(const PackedParams p) {
   sm100::fence_proxy_async();
   pdl_wait();
   pdl_launch();
-  // ---- the CTA's first item.  count(r, span): what request r adds to a line; the sums before each thread's request, 128 requests at a time.
-  const long long c = blockIdx.x;
-  long long mine = 0, at = 0, line = 0;
-  auto scan = [&](int base, auto count) {
-    const int r = base + tid;
-    mine = r < p.n_reqs ? count(span_of<NT>(p, r)) : 0;
-    long long u = mine;
+  // ---- the CTA's first item
+  // CTAs that a pair of its own gets: their sum over all pairs is at most N + (P - N)
+  auto ctas_of = [&](const Span sp) { return sp.tiles ? (int)min((long long)sp.tiles, 1 + (long long)sp.tiles * max(0ll, way.P - way.N) / way.U) : 0; };
+  auto pairs_of = [&](const Span sp) { return sp.row_tiles * p.Hkv; };
+  // units in the low 40 bits, pairs above
+  auto load_of = [&](const Span sp) { return sp.tiles ? (long long)sp.tiles * pairs_of(sp) + ((long long)pairs_of(sp) << 40) : 0ll; };
+  auto line_of = [&](const Span sp) { return (long long)(way.own ? ctas_of(sp) : sp.tiles) * pairs_of(sp); };
+  auto decide = [&](long long load) {      // the same in every thread
+    const long long c = blockIdx.x, U = load & ((1ll << 40) - 1), N = load >> 40, P = min((long long)gridDim.x, U);
+    const bool own = 2 * N <= gridDim.x;
+    if (tid == 0 && U) way = Way{U, P, N, own ? c : c * U / P, own ? c + 1 : (c + 1) * U / P, own};
+    return U > 0 && (own || c < P);
+  };
+  auto run_in_warp = [&](long long v) {
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const long long v = __shfl_up_sync(0xffffffffu, u, d);
-      if (lane >= d) u += v;
+      const long long x = __shfl_up_sync(0xffffffffu, v, d);
+      if (lane >= d) v += x;
     }
-    __syncthreads();
-    if (lane == 31) s_scan[warp] = u;
-    __syncthreads();
-    at = line + u - mine;
-    for (int w = 0; w < WARPS; ++w) {
-      if (w < warp) at += s_scan[w];
-      line += s_scan[w];
-    }
+    return v;
   };
-  // units in the low 40 bits, pairs above
-  for (int base = 0; base < p.n_reqs; base += WARPS * 32)
-    scan(base, [&](const Span sp) { return (long long)sp.tiles * sp.row_tiles * p.Hkv + ((long long)(sp.tiles ? sp.row_tiles * p.Hkv : 0) << 40); });
-  const long long U = line & ((1ll << 40) - 1), N = line >> 40;
-  if (U == 0) return;
-  const bool own = 2 * N <= gridDim.x;
-  const long long P = min((long long)gridDim.x, U);
-  // CTAs that a pair of its own gets: their sum over all pairs is at most N + (P - N)
-  auto ctas_of = [&](const Span sp) { return sp.tiles ? (int)min((long long)sp.tiles, 1 + (long long)sp.tiles * max(0ll, P - N) / U) : 0; };
-  const long long first = own ? c : c * U / P, last = own ? c + 1 : (c + 1) * U / P;
-  if (!own && c >= P) return;
-  if (tid == 0) s_req = -1;
-  line = 0;
-  for (int base = 0; base < p.n_reqs; base += WARPS * 32) {
-    scan(base, [&](const Span sp) { return (long long)(own ? ctas_of(sp) : sp.tiles) * sp.row_tiles * p.Hkv; });
-    if (first >= at && first < at + mine) {
-      s_req = base + tid;
-      s_start = at;
+  int r = -1, begin = 0;               // the item's request, and where its line begins, counted from the CTA's share
+  if (p.n_reqs <= 32) {                // every warp looks at all of them
+    const Span sp = lane < p.n_reqs ? span_of<NT>(p, lane) : Span{0, 0, 0};
+    if (!decide(__shfl_sync(0xffffffffu, run_in_warp(load_of(sp)), 31))) return;
+    __syncthreads();
+    const long long mine = line_of(sp), at = run_in_warp(mine) - mine;
+    const unsigned here = __ballot_sync(0xffffffffu, way.first >= at && way.first < at + mine);
+    if (here == 0) return;
+    r = __ffs(here) - 1;
+    begin = (int)(__shfl_sync(0xffffffffu, at, r) - way.first);
+  } else {                             // 128 at a time, one a thread
+    long long mine = 0, at = 0, line = 0;
+    auto scan = [&](int base, auto count) {
+      mine = base + tid < p.n_reqs ? count(span_of<NT>(p, base + tid)) : 0;
+      const long long u = run_in_warp(mine);
+      __syncthreads();
+      if (lane == 31) s_scan[warp] = u;
+      __syncthreads();
+      at = line + u - mine;
+      for (int w = 0; w < WARPS; ++w) {
+        if (w < warp) at += s_scan[w];
+        line += s_scan[w];
+      }
+    };
+    for (int base = 0; base < p.n_reqs; base += WARPS * 32) scan(base, load_of);
+    if (!decide(line)) return;
+    if (tid == 0) s_req = -1;
+    line = 0;
+    __syncthreads();
+    for (int base = 0; base < p.n_reqs; base += WARPS * 32) {
+      scan(base, line_of);
+      if (way.first >= at && way.first < at + mine) {
+        s_req = base + tid;
+        s_begin = (int)(at - way.first);
+      }
+      if (line > way.first) break;
     }
-    if (line > first) break;
+    __syncthreads();
+    r = s_req;
+    begin = s_begin;
+    if (r < 0) return;
   }
-  __syncthreads();
-  if (s_req < 0) return;
-  int r = s_req;
-  long long u = first, start = s_start;
+  int done = 0;                        // of the CTA's share
   auto next_item = [&](Item& it) {
-    if (u >= last) return false;
+    if (done >= way.last - way.first) return false;
     Span sp = span_of<NT>(p, r);
-    while (u >= start + (long long)(own ? ctas_of(sp) : sp.tiles) * sp.row_tiles * p.Hkv) {
-      start += (long long)(own ? ctas_of(sp) : sp.tiles) * sp.row_tiles * p.Hkv;
+    while (done >= begin + line_of(sp)) {
+      begin += (int)line_of(sp);
       sp = span_of<NT>(p, ++r);
     }
-    const int each = own ? ctas_of(sp) : sp.tiles, pair = (int)((u - start) / each), i = (int)((u - start) % each);
+    const int each = way.own ? ctas_of(sp) : sp.tiles, pair = (done - begin) / each, i = (done - begin) % each;
     const int blocks = (p.pos0[r] + p.q_start[r + 1] - p.q_start[r] - sp.lo + PACKED_POS - 1) / PACKED_POS;
     it.r = r;
     it.kvh = pair / sp.row_tiles;
     it.rt = pair % sp.row_tiles;
     it.key_lo = sp.lo;
-    if (own) {
+    if (way.own) {
       it.q0 = (int)((long long)i * blocks / each);
       it.q1 = (int)((long long)(i + 1) * blocks / each);
-      it.parts = Parts{(int)c - i, each, 0};
-      u = last;
+      it.parts = Parts{(int)blockIdx.x - i, each, 0};
+      done = 1;
       return true;
     }
-    const long long pair_start = start + (long long)pair * each, pair_end = pair_start + each, until = min(pair_end, last);
+    const long long U = way.U, P = way.P, pair_start = way.first + begin + (long long)pair * each, pair_end = pair_start + each;
+    const int until = (int)(min(pair_end, way.last) - way.first);
     it.q0 = i * WARPS;
-    it.q1 = min(blocks, (int)(until - pair_start) * WARPS);
+    it.q1 = min(blocks, (i + until - done) * WARPS);
     // the CTAs of the pair's first and last units: the largest k with k U / P <= that unit
     const int k0 = (int)(((pair_start + 1) * P - 1) / U), k1 = (int)((pair_end * P - 1) / U);
     it.parts = Parts{k0, k1 - k0 + 1, k0 * U / P == pair_start ? 0 : 1};
-    u = until;
+    done = until;
     return true;
   };
   // ---- walk the share
