@@ -577,10 +577,10 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, const Item it
   __syncthreads();
   if (tid == 0) {
     int* count = p.counters + ((size_t)r * p.Hkv + kvh) * 2 + rt;
-    __threadfence();                   // (the block's stores lie before it by the barrier)
-    s_last = atomicAdd(count, 1) == parts.n - 1;
+    int before;                        // (the block's stores come before it by the barrier, what the others stored before theirs by theirs)
+    asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(count) : "memory");
+    s_last = before == parts.n - 1;
     if (s_last) *count = 0;
-    __threadfence();
   }
   __syncthreads();
   if (!s_last) return;
@@ -592,8 +592,14 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, const Item it
   float4 acc[ITEMS];
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto load_parts = [&](float4 (&v)[GROUP], int i0, int n, int rr, int d) {      // parts i0 .., of which the last is n - 1
+#pragma unroll
+    for (int i = 0; i < GROUP; ++i) v[i] = __ldcg(reinterpret_cast<const float4*>(p.part_o + ((size_t)parts.slot(min(i0 + i, n - 1)) * PART_ROWS + rr) * D + d));
+  };
   for (int first = 0; first < parts.n; first += CHUNK) {
     const int n = min(CHUNK, parts.n - first);
+    float4 ahead[GROUP];               // (the first loads go out before the factors are known)
+    load_parts(ahead, first, first + n, min(tid / (D / 4), rows - 1), tid % (D / 4) * 4);
     for (int rr = warp; rr < rows; rr += WARPS) {
       float2 ml[CHUNK / 32];
       float m_run = first ? state[rr * 3] : -INFINITY, m_new = m_run;
@@ -628,8 +634,12 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, const Item it
       acc[k].x *= keep; acc[k].y *= keep; acc[k].z *= keep; acc[k].w *= keep;
       for (int i0 = 0; i0 < n; i0 += GROUP) {
         float4 v[GROUP];
+        if (k == 0 && i0 == 0) {
 #pragma unroll
-        for (int i = 0; i < GROUP; ++i) v[i] = __ldcg(reinterpret_cast<const float4*>(p.part_o + ((size_t)parts.slot(first + min(i0 + i, n - 1)) * PART_ROWS + rr) * D + d));
+          for (int i = 0; i < GROUP; ++i) v[i] = ahead[i];
+        } else {
+          load_parts(v, first + i0, first + n, rr, d);
+        }
 #pragma unroll
         for (int i = 0; i < GROUP; ++i) {
           const float f = factor[rr * CHUNK + i0 + i];      // (0 behind the last part)
