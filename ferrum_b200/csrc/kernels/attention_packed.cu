@@ -17,7 +17,9 @@
 //
 // The work is handed out on the device, so that the launch does not depend on the lengths and a captured one serves any.  A (request, KV head,
 // rows of 8 NT) is a pair.  Few pairs (at most half the CTAs): each gets a number of CTAs of its own by its length, one part a CTA, as a
-// part costs some 4 us beside its keys.  Many: their units of 64 keys form one line, and CTA c of P takes the units [c U / P, (c + 1) U / P).
+// part costs some 4 us beside its keys.  Many: they form one line, a pair as long as its units of 64 keys and EXTRA for that cost, and CTA c of
+// P takes the stretch [c L / P, (c + 1) L / P); pairs of up to WHOLE units (and of no more than a stretch) are not cut but belong to the CTA in whose
+// stretch they begin.
 // A CTA's four warps take every fourth block of 16 positions; a block is one bulk copy into the warp's own ring of stages, and no
 // warp waits for another until its part is done; the first copies of the next part are on their way by then.  Of the CTAs that share a (request, head) the one that comes last adds up the parts, in a fixed order.
 #include "packed_cache.cuh"
@@ -36,6 +38,8 @@ constexpr int HEAD = 15 - (int)SLACK;        // p step times its power of two is
 constexpr int SETTLE = 16;                   // steps after which the sums of codes are centred
 constexpr int HALVES = 2;                    // steps in a warp's ring: one is read while the next arrives
 static_assert(32 % NB == 0, "the blocks of a step lie in one window of 32 blocks, one a lane");
+constexpr int EXTRA = 6;                     // what a part costs beside its keys, in units
+constexpr int WHOLE = 16;                    // units up to which a pair is not cut
 constexpr int PART_ROWS = 16;                // rows of a partial's slot
 
 struct PackedParams {
@@ -122,11 +126,11 @@ __device__ __forceinline__ Span span_of(const PackedParams& p, int r) {
   return Span{lo, (pos + n - lo + TILE - 1) / TILE, (rows + 8 * NT - 1) / (8 * NT)};
 }
 
-// Where the parts of a (request, head, row tile) lie: n CTAs from `cta` on; the first one's is in slot 2 cta + odd, the others' in the even slots
-// of theirs.  n = 1: not cut.
+// Where the parts of a pair lie: n CTAs from `cta` on; the first one's is in the odd slot of its two (the pair ends beyond that CTA's stretch), the others'
+// in the even slots of theirs.  n = 1: not cut.
 struct Parts {
-  int cta, n, odd;
-  __device__ __forceinline__ int slot(int i) const { return i == 0 ? 2 * cta + odd : 2 * (cta + i); }
+  int cta, n;
+  __device__ __forceinline__ int slot(int i) const { return 2 * (cta + i) + (i == 0); }
 };
 
 template <typename T>
@@ -138,9 +142,11 @@ __device__ __forceinline__ void write_row4(const PackedParams& p, int token, int
   *reinterpret_cast<uint2*>((T*)p.out + (size_t)token * p.ldo + (size_t)head * D + d) = r;
 }
 
-// How the work is shared out: units and pairs in all, CTAs, the CTA's own stretch of the line (of units, or of parts where pairs have CTAs of their own).
+// How the work is shared out: the line's length, units and pairs in all, CTAs, the CTA's own stretch of the line (or its own part, where pairs have
+// CTAs of their own).
 struct Way {
-  long long U, P, N, first, last;
+  long long L, U, P, N, first, last;
+  int whole;              // pairs of up to so many units are not cut
   bool own;
 };
 
@@ -681,11 +687,13 @@ attention_packed_kernel(const PackedParams p) {
   auto pairs_of = [&](const Span sp) { return sp.row_tiles * p.Hkv; };
   // units in the low 40 bits, pairs above
   auto load_of = [&](const Span sp) { return sp.tiles ? (long long)sp.tiles * pairs_of(sp) + ((long long)pairs_of(sp) << 40) : 0ll; };
-  auto line_of = [&](const Span sp) { return (long long)(way.own ? ctas_of(sp) : sp.tiles) * pairs_of(sp); };
+  auto length_of = [&](const Span sp) { return way.own ? ctas_of(sp) : sp.tiles ? sp.tiles + EXTRA : 0; };
+  auto line_of = [&](const Span sp) { return (long long)length_of(sp) * pairs_of(sp); };
   auto decide = [&](long long load) {      // the same in every thread
-    const long long c = blockIdx.x, U = load & ((1ll << 40) - 1), N = load >> 40, P = min((long long)gridDim.x, U);
+    const long long c = blockIdx.x, U = load & ((1ll << 40) - 1), N = load >> 40, L = U + EXTRA * N;
     const bool own = 2 * N <= gridDim.x;
-    if (tid == 0 && U) way = Way{U, P, N, own ? c : c * U / P, own ? c + 1 : (c + 1) * U / P, own};
+    const long long P = min((long long)gridDim.x, own ? U : L);
+    if (tid == 0 && U) way = Way{L, U, P, N, own ? c : c * L / P, own ? c + 1 : (c + 1) * L / P, (int)min((long long)WHOLE, L / P), own};
     return U > 0 && (own || c < P);
   };
   auto run_in_warp = [&](long long v) {
@@ -740,34 +748,48 @@ attention_packed_kernel(const PackedParams p) {
   }
   int done = 0;                        // of the CTA's share
   auto next_item = [&](Item& it) {
-    if (done >= way.last - way.first) return false;
-    Span sp = span_of<NT>(p, r);
-    while (done >= begin + line_of(sp)) {
-      begin += (int)line_of(sp);
-      sp = span_of<NT>(p, ++r);
-    }
-    const int each = way.own ? ctas_of(sp) : sp.tiles, pair = (done - begin) / each, i = (done - begin) % each;
-    const int blocks = (p.pos0[r] + p.q_start[r + 1] - p.q_start[r] - sp.lo + PACKED_POS - 1) / PACKED_POS;
-    it.r = r;
-    it.kvh = pair / sp.row_tiles;
-    it.rt = pair % sp.row_tiles;
-    it.key_lo = sp.lo;
-    if (way.own) {
-      it.q0 = (int)((long long)i * blocks / each);
-      it.q1 = (int)((long long)(i + 1) * blocks / each);
-      it.parts = Parts{(int)blockIdx.x - i, each, 0};
-      done = 1;
+    const long long P = way.P, L = way.L;
+    while (done < way.last - way.first) {
+      const Span sp = span_of<NT>(p, r);
+      if (done >= begin + line_of(sp)) {
+        begin += (int)line_of(sp);
+        ++r;
+        continue;
+      }
+      const int each = length_of(sp), pair = (done - begin) / each, i = (done - begin) % each;
+      const int blocks = (p.pos0[r] + p.q_start[r + 1] - p.q_start[r] - sp.lo + PACKED_POS - 1) / PACKED_POS;
+      it.r = r;
+      it.kvh = pair / sp.row_tiles;
+      it.rt = pair % sp.row_tiles;
+      it.key_lo = sp.lo;
+      if (way.own) {
+        it.q0 = (int)((long long)i * blocks / each);
+        it.q1 = (int)((long long)(i + 1) * blocks / each);
+        it.parts = Parts{(int)blockIdx.x - i, each};
+        done = 1;
+        return true;
+      }
+      const int after = done - i + each;      // where the pair ends
+      if (sp.tiles <= way.whole) {
+        done = after;
+        if (i > 0) continue;                  // it begins in another CTA's stretch
+        it.q0 = 0;
+        it.q1 = blocks;
+        it.parts = Parts{0, 1};
+        return true;
+      }
+      const long long pair_start = way.first + begin + (long long)pair * each;
+      const int t0 = max(0, i - EXTRA), t1 = (int)min((long long)sp.tiles, way.last - pair_start - EXTRA);
+      done = min(after, (int)(way.last - way.first));
+      if (t0 >= t1) continue;                 // the stretch ends within the pair's EXTRA
+      it.q0 = t0 * WARPS;
+      it.q1 = min(blocks, t1 * WARPS);
+      // the CTAs of the pair's first and last units: the largest k with k L / P <= that unit's place
+      const int k0 = (int)(((pair_start + EXTRA + 1) * P - 1) / L), k1 = (int)(((pair_start + each) * P - 1) / L);
+      it.parts = Parts{k0, k1 - k0 + 1};
       return true;
     }
-    const long long U = way.U, P = way.P, pair_start = way.first + begin + (long long)pair * each, pair_end = pair_start + each;
-    const int until = (int)(min(pair_end, way.last) - way.first);
-    it.q0 = i * WARPS;
-    it.q1 = min(blocks, (i + until - done) * WARPS);
-    // the CTAs of the pair's first and last units: the largest k with k U / P <= that unit
-    const int k0 = (int)(((pair_start + 1) * P - 1) / U), k1 = (int)((pair_end * P - 1) / U);
-    it.parts = Parts{k0, k1 - k0 + 1, k0 * U / P == pair_start ? 0 : 1};
-    done = until;
-    return true;
+    return false;
   };
   // ---- walk the share
   uint32_t turn = 0;      // steps that the warp has run: a step's half of the ring and its barrier's phase follow from its number
@@ -775,7 +797,7 @@ attention_packed_kernel(const PackedParams p) {
   Flow<D> flow;
   Item it, following;
   bool more = next_item(it);
-  flow.begin(p, it, turn, ring, bars);
+  if (more) flow.begin(p, it, turn, ring, bars);
   while (more) {
     packed_item<T, D, NT>(p, it, flow, ring, bars, turn, merge, failed, [&]() {
       more = next_item(following);
