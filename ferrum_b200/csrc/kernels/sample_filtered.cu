@@ -92,6 +92,13 @@ struct Shared {
   double powers[64];                // 2^(j / 64)
 };
 
+// What a first histogram has told: the bin of the cut (none: -1), the sum of what lies above it, and the limit.
+struct Border {
+  int bin;
+  u64 before;
+  double limit;
+};
+
 // The CTA's view of its row.
 template <bool RESIDENT>
 struct Row {
@@ -214,9 +221,10 @@ struct Row {
   }
 
   // Rows whose cut leaves few tokens: one histogram, and the tokens of the bins down to the one that holds the cut go to the first CTA, which sorts
-  // them and does the rest.  BY_MASS: no top-k, so that the cut is top-p's.  False (for all CTAs alike): there are more than FEW of them.
+  // them and does the rest.  BY_MASS: no top-k, so that the cut is top-p's.  False (for all CTAs alike): there are more than FEW of them; `known` is what
+  // the histogram told then.
   template <bool BY_MASS>
-  __device__ __forceinline__ bool draw_of_few(int top_k, float top_p, double min_w, double u, float range, int out) {
+  __device__ __forceinline__ bool draw_of_few(int top_k, float top_p, double min_w, double u, float range, int out, Border& known) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (!(isfinite(top) && isfinite(range))) return false;
     const float scale = (float)BINS / range;
@@ -243,15 +251,17 @@ struct Row {
     int b0, each;
     bins_of_cluster(mine, own, all, at, b0, each);
     const double limit = BY_MASS ? (double)top_p * (double)all : (double)top_k;
-    u64 best_bin = 0;
+    u64 best_bin = 0, best_at = 0;
 #pragma unroll
     for (int j = 0; j < MOST_BINS; ++j) {
-      if (j < each && mine[j] && (double)at < limit) best_bin = b0 + j + 1;
+      if (j < each && mine[j] && (double)at < limit) best_bin = b0 + j + 1, best_at = at;
       at += mine[j];
     }
-    const u64(&e2)[2][MAX_CLUSTER] = gather<true>(best_bin, 0);
+    const u64(&e2)[2][MAX_CLUSTER] = gather<true>(best_bin, best_at);
     int border = 0;
-    for (int c = 0; c < n_ctas; ++c) border = max(border, (int)e2[0][c]);
+    u64 before = 0;
+    for (int c = 0; c < n_ctas; ++c) border = max(border, (int)e2[0][c]), before = max(before, e2[1][c]);
+    known = Border{border - 1, before, limit};
     // (the bins are read: their place is free)
     unsigned count = 0;
 #pragma unroll 4
@@ -366,7 +376,7 @@ struct Row {
   // a token counts 1, the limit is `limit` itself, or (MASS) a token counts its mass and the limit is that part of all of it.  range: how
   // far below the maximum the logits go that count (at least).
   template <bool MASS>
-  __device__ __forceinline__ Cut find(const Cut cut, double limit, float range) {
+  __device__ __forceinline__ Cut find(const Cut cut, double limit, float range, Border known = Border{-1, 0, 0.0}) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     uint32_t lo_key = 1, hi_key = best;
     u64 before = 0;
@@ -380,45 +390,55 @@ struct Row {
         if (!linear) return (int)((hi_key - k) >> down);
         return min(BINS - 1, (int)((top - key_value(k)) * scale));
       };
-      for (int i = tid; i < BINS; i += blockDim.x) sh.hist[i] = 0;
-      __syncthreads();
+      int border;
+      if (known.bin >= 0) {         // (a first histogram was made before)
+        border = known.bin;
+        before = known.before;
+        limit = known.limit;
+        whole_known = true;
+        known.bin = -1;
+      } else {
+        for (int i = tid; i < BINS; i += blockDim.x) sh.hist[i] = 0;
+        __syncthreads();
 #pragma unroll 4
-      for (int e = e0 + lane; e < e1; e += 32) {
-        const uint32_t k = key(e);
-        if (k < lo_key || k > hi_key || !cut.stays(k, index(e))) continue;
-        unsigned* half = reinterpret_cast<unsigned*>(&sh.hist[bin_of(k)]);      // (a 64-bit addition by two of 32 bits, the second hardly ever made)
-        if (MASS) {
-          const u64 v = mass(k);
-          const unsigned low = (unsigned)v;
-          if (v == 0) continue;
-          const unsigned old = atomicAdd(half, low), high = (unsigned)(v >> 32) + (old + low < old ? 1 : 0);
-          if (high) atomicAdd(half + 1, high);
-        } else {
-          atomicAdd(half, 1u);
+        for (int e = e0 + lane; e < e1; e += 32) {
+          const uint32_t k = key(e);
+          if (k < lo_key || k > hi_key || !cut.stays(k, index(e))) continue;
+          unsigned* half = reinterpret_cast<unsigned*>(&sh.hist[bin_of(k)]);      // (a 64-bit addition by two of 32 bits, the second hardly ever made)
+          if (MASS) {
+            const u64 v = mass(k);
+            const unsigned low = (unsigned)v;
+            if (v == 0) continue;
+            const unsigned old = atomicAdd(half, low), high = (unsigned)(v >> 32) + (old + low < old ? 1 : 0);
+            if (high) atomicAdd(half + 1, high);
+          } else {
+            atomicAdd(half, 1u);
+          }
         }
-      }
-      cluster_sync();
-      u64 mine[MOST_BINS], own, all, at;
-      int b0, each;
-      bins_of_cluster(mine, own, all, at, b0, each);
-      at += before;
-      if (!whole_known) limit *= (double)all;
-      whole_known = true;
-      // the last bin with something in it whose predecessors stay below the limit
-      u64 best_bin = 0, best_at = 0;
+        cluster_sync();
+        u64 mine[MOST_BINS], own, all, at;
+        int b0, each;
+        bins_of_cluster(mine, own, all, at, b0, each);
+        at += before;
+        if (!whole_known) limit *= (double)all;
+        whole_known = true;
+        // the last bin with something in it whose predecessors stay below the limit
+        u64 best_bin = 0, best_at = 0;
 #pragma unroll
-      for (int j = 0; j < MOST_BINS; ++j) {
-        if (j < each && mine[j] && (double)at < limit) best_bin = b0 + j + 1, best_at = at;
-        at += mine[j];
+        for (int j = 0; j < MOST_BINS; ++j) {
+          if (j < each && mine[j] && (double)at < limit) best_bin = b0 + j + 1, best_at = at;
+          at += mine[j];
+        }
+        // bins and their sums rise together: the largest of each belong together
+        const u64(&e2)[2][MAX_CLUSTER] = gather<true>(best_bin, best_at);
+        u64 bin = 0;
+        before = 0;
+        for (int c = 0; c < n_ctas; ++c) bin = max(bin, e2[0][c]), before = max(before, e2[1][c]);
+        border = (int)bin - 1;
       }
-      // bins and their sums rise together: the largest of each belong together
-      const u64(&e2)[2][MAX_CLUSTER] = gather<true>(best_bin, best_at);
-      u64 bin = 0;
-      before = 0;
-      for (int c = 0; c < n_ctas; ++c) bin = max(bin, e2[0][c]), before = max(before, e2[1][c]);
       // the range of the keys in that bin, for the next histogram; and the lists of what lies in it or above
       uint32_t a = 0, b = 0;        // maximum of ~key and of key
-      const int border = (int)bin - 1, most = LIST / (int)(blockDim.x >> 5);
+      const int most = LIST / (int)(blockDim.x >> 5);
       int count = 0;
 #pragma unroll 4
       for (int e = e0 + lane; e - lane < e1; e += 32) {
@@ -631,11 +651,12 @@ sample_filtered_kernel(const FilterParams p) {
   const float mass_range = fminf(range, (float)(p.shift + 1) * 0.6931472f * T);
   const double min_w = min_p > 0.f ? (double)min_p * (double)(1ull << p.shift) : 0.0, u = p.uniform[q];
   const bool by_k = top_k > 0 && top_k < p.V, by_p = top_p < 1.f;
-  if (by_k ? top_k <= FEW && w.template draw_of_few<false>(top_k, top_p, min_w, u, range, r)
-           : by_p && w.template draw_of_few<true>(top_k, top_p, min_w, u, mass_range, r))
+  Border known{-1, 0, 0.0};
+  if (by_k ? top_k <= FEW && w.template draw_of_few<false>(top_k, top_p, min_w, u, range, r, known)
+           : by_p && w.template draw_of_few<true>(top_k, top_p, min_w, u, mass_range, r, known))
     return;
-  if (by_k) cut = w.template find<false>(cut, (double)top_k, range);
-  if (by_p) cut = w.template find<true>(cut, (double)top_p, mass_range);
+  if (by_k) cut = w.template find<false>(cut, (double)top_k, range, known);
+  if (by_p) cut = w.template find<true>(cut, (double)top_p, mass_range, by_k ? Border{-1, 0, 0.0} : known);
   w.draw(cut, min_w, u, r);
   cluster_sync();                   // (no CTA leaves while a peer may still reach into its shared memory)
 }
