@@ -231,6 +231,22 @@ def _at(t):
     return t.data_ptr() if t is not None else None
 
 
+def _dense(t, dtype, name, ndim):
+    """The address of a contiguous CUDA tensor of this type (for the wrappers whose share of a short call counts)."""
+    if type(t) is torch.Tensor and t.is_cuda and t.dtype is dtype and t.ndim == ndim and t.is_contiguous():
+        return t.data_ptr()
+    _need(t, dtype, name, ndim)
+    raise KernelError(f"{name} must be contiguous")
+
+
+def _rows(t, dtype, name):
+    """(address, elements from a row to the next) of a CUDA matrix of this type with dense rows."""
+    if not (type(t) is torch.Tensor and t.is_cuda and t.dtype is dtype and t.ndim == 2 and t.is_contiguous()):
+        _need(t, dtype, name, 2)
+        return t.data_ptr(), t.stride(0)
+    return t.data_ptr(), t.shape[1]
+
+
 def _stream_at():
     return _raw_stream(_device_index()) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
 
@@ -789,60 +805,57 @@ def packed_block_bytes(D):
 
 
 def _need_packed(plane, page_stride, page_size, Hkv, D, name):
-    """The checks of a plane of packed pages, uint8 [pages, Hkv, page_size / 16, bytes of a block]."""
-    _need(plane, torch.uint8, "plane", 4)
+    """The checks of a plane of packed pages, uint8 [pages, Hkv, page_size / 16, bytes of a block]; (address, pages)."""
     block = packed_block_bytes(D)
     if page_size <= 0 or page_size % 16 or block == 0:
         raise KernelError(f"{name}: a cache in 4 bits has pages of a multiple of 16 positions and heads of 64 or 128 elements, found {page_size} and {D}")
-    if plane.shape[1:] != (Hkv, page_size // 16, block) or page_stride != plane.stride(0) or not (plane.is_contiguous() or plane[0].is_contiguous()):
+    _need(plane, torch.uint8, "plane", 4)
+    n_pages, heads, blocks, found = plane.shape
+    if heads != Hkv or blocks * 16 != page_size or found != block or page_stride != plane.stride(0) or not (plane.is_contiguous() or plane[0].is_contiguous()):
         raise KernelError(f"{name}: the plane must be [pages, {Hkv}, {page_size // 16}, {block}] with dense pages {page_stride} bytes apart")
-
-
-def _need_table(block_table, name):
-    _need(block_table, torch.int32, "block_table", 2)
-    if not block_table.is_contiguous():
-        raise KernelError(f"{name}: block_table must be contiguous")
+    return plane.data_ptr(), n_pages
 
 
 def rope_cache_write_packed(qkv, n_tokens, positions, req_of_token, block_table, cos_sin, plane, page_stride, page_size, Hq, Hkv, D, R, pairing,
                             err, q_out=None, write_kv=True):
     """Rotate q and k and store k and v in the pages of a cache held in 4 bits, quantised by groups of 64 elements.  The turned
     q goes to `q_out` ([>= n_tokens, >= Hq * D]; None: in place).  plane: uint8 [pages, Hkv, page_size / 16, `packed_block_bytes(D)`]."""
-    _need16(qkv, "qkv", 2); _need(positions, torch.int32, "positions", 1); _need(req_of_token, torch.int32, "req_of_token", 1)
-    _need_table(block_table, "rope_cache_write_packed")
-    if q_out is not None:
-        _need16(q_out, "q_out", 2, like=qkv)
-    q = qkv if q_out is None else q_out
+    dt = dtype_code(qkv.dtype) if isinstance(qkv, torch.Tensor) and qkv.dtype in SIXTEEN_BIT else _need16(qkv, "qkv", 2)
+    at, ld = _rows(qkv, qkv.dtype, "qkv")
+    q_at, ldq = (at, ld) if q_out is None else _rows(q_out, qkv.dtype, "q_out")
+    cs_at = n_pos = 0
     if R:
-        _need(cos_sin, torch.float32, "cos_sin", 3)
-        if cos_sin.shape[1] != R // 2 or cos_sin.shape[2] != 2 or not cos_sin.is_contiguous():
+        cs_at = _dense(cos_sin, torch.float32, "cos_sin", 3)
+        n_pos, half, two = cos_sin.shape
+        if half != R // 2 or two != 2:
             raise KernelError("rope_cache_write_packed: cos_sin must be contiguous [positions, rope_dim/2, 2]")
-    _need_packed(plane, page_stride, page_size, Hkv, D, "rope_cache_write_packed")
-    if min(qkv.shape[0], q.shape[0], positions.shape[0], req_of_token.shape[0]) < n_tokens:
+    plane_at, n_pages = _need_packed(plane, page_stride, page_size, Hkv, D, "rope_cache_write_packed")
+    pos_at, req_at, table_at = _dense(positions, torch.int32, "positions", 1), _dense(req_of_token, torch.int32, "req_of_token", 1), _dense(block_table, torch.int32, "block_table", 2)
+    if min(qkv.shape[0], positions.shape[0], req_of_token.shape[0]) < n_tokens or (q_out is not None and q_out.shape[0] < n_tokens):
         raise KernelError(f"rope_cache_write_packed: fewer rows than {n_tokens} tokens")
     global _work
     if _profile is not None:
         _work = (n_tokens * (2 * (2 * Hq + (2 * Hkv if write_kv else 0)) * D + (Hkv * 9 * D // 8 if write_kv else 0)), 0.0)
-    _check(lib().ferrum_rope_cache_write_packed(_at(qkv), dtype_code(qkv.dtype), n_tokens, qkv.stride(0), _at(q), q.stride(0), _at(positions),
-                                                _at(req_of_token), _at(block_table), block_table.shape[1], _at(cos_sin if R else None),
-                                                cos_sin.shape[0] if R else 0, _at(plane), page_stride, plane.shape[0], page_size,
-                                                Hq, Hkv, D, R, pairing, 1 if write_kv else 0, _at(err), _stream_at()), "rope_cache_write_packed")
+    _check(lib().ferrum_rope_cache_write_packed(at, dt, n_tokens, ld, q_at, ldq, pos_at, req_at, table_at, block_table.shape[1], cs_at or None, n_pos,
+                                                plane_at, page_stride, n_pages, page_size, Hq, Hkv, D, R, pairing, 1 if write_kv else 0, _at(err),
+                                                _stream_at()), "rope_cache_write_packed")
 
 
 def unpack_cache(plane, page_stride, page_size, block_table, items, out, err):
     """out[i] = the 16-bit keys and values of page items[i, 1] of request items[i, 0] (int32 [n, 2]); out: [>= n, 2, Hkv, page_size, D] of
     the cache's 16-bit type.  A page that the request does not hold arrives as zeros and raises the error flag."""
-    _need16(out, "out", 5); _need(items, torch.int32, "items", 2); _need_table(block_table, "unpack_cache")
-    Hkv, D = out.shape[2], out.shape[4]
-    _need_packed(plane, page_stride, page_size, Hkv, D, "unpack_cache")
-    n = items.shape[0]
-    if items.shape[1] != 2 or not items.is_contiguous() or out.shape[0] < n or out.shape[1] != 2 or out.shape[3] != page_size or not out.is_contiguous():
+    dt = dtype_code(out.dtype) if isinstance(out, torch.Tensor) and out.dtype in SIXTEEN_BIT else _need16(out, "out", 5)
+    out_at, items_at, table_at = _dense(out, out.dtype, "out", 5), _dense(items, torch.int32, "items", 2), _dense(block_table, torch.int32, "block_table", 2)
+    held, two, Hkv, page, D = out.shape
+    plane_at, n_pages = _need_packed(plane, page_stride, page_size, Hkv, D, "unpack_cache")
+    n, pair = items.shape
+    if pair != 2 or held < n or two != 2 or page != page_size:
         raise KernelError("unpack_cache: items must be [n, 2] and out contiguous [>= n, 2, Hkv, page_size, D]")
     global _work
     if _profile is not None:
         _work = (n * Hkv * page_size * D * (9 / 8 + 4), 0.0)
-    _check(lib().ferrum_unpack_cache(_at(plane), page_stride, plane.shape[0], page_size, _at(block_table), block_table.shape[1],
-                                     _at(items), n, _at(out), dtype_code(out.dtype), Hkv, D, _at(err), _stream_at()), "unpack_cache")
+    _check(lib().ferrum_unpack_cache(plane_at, page_stride, n_pages, page_size, table_at, block_table.shape[1], items_at, n, out_at, dt, Hkv, D, _at(err),
+                                     _stream_at()), "unpack_cache")
 
 
 @functools.lru_cache(maxsize=None)
@@ -863,19 +876,17 @@ def attention_packed(q, out, n_tokens, block_table, q_start, pos0, plane, page_s
     each request; pos0 (int32 [requests]): positions cached before the step, whose own keys must be in the pages already.  part:
     float32 workspace of `attention_packed_workspace(D)` elements; counters: int32, requests x Hkv x 2 zeros, which the call leaves
     zeros.  Calls that may run at the same time need one of each for themselves."""
-    _need16(q, "q", 2); _need16(out, "out", 2, like=q); _need(q_start, torch.int32, "q_start", 1); _need(pos0, torch.int32, "pos0", 1)
-    _need_table(block_table, "attention_packed"); _need_packed(plane, page_stride, page_size, Hkv, D, "attention_packed")
-    _need(part, torch.float32, "part", 1); _need(counters, torch.int32, "counters", 1)
-    n_reqs = pos0.shape[0]
-    if q_start.shape[0] != n_reqs + 1 or block_table.shape[0] < n_reqs or min(q.shape[0], out.shape[0]) < n_tokens:
+    dt = dtype_code(q.dtype) if isinstance(q, torch.Tensor) and q.dtype in SIXTEEN_BIT else _need16(q, "q", 2)
+    (q_at, ldq), (out_at, ldo) = _rows(q, q.dtype, "q"), _rows(out, q.dtype, "out")
+    start_at, pos_at, table_at = _dense(q_start, torch.int32, "q_start", 1), _dense(pos0, torch.int32, "pos0", 1), _dense(block_table, torch.int32, "block_table", 2)
+    plane_at, n_pages = _need_packed(plane, page_stride, page_size, Hkv, D, "attention_packed")
+    part_at, counters_at = _dense(part, torch.float32, "part", 1), _dense(counters, torch.int32, "counters", 1)
+    n_reqs, (held, width) = pos0.shape[0], block_table.shape
+    if q_start.shape[0] != n_reqs + 1 or held < n_reqs or min(q.shape[0], out.shape[0]) < n_tokens:
         raise KernelError("attention_packed: q_start, pos0, block_table and the rows do not agree")
-    if not (q_start.is_contiguous() and pos0.is_contiguous() and part.is_contiguous() and counters.is_contiguous()):
-        raise KernelError("attention_packed: q_start, pos0, part and counters must be contiguous")
-    _check(lib().ferrum_attention_packed(_at(q), q.stride(0), _at(out), out.stride(0), dtype_code(q.dtype), _at(plane), page_stride,
-                                         plane.shape[0], page_size, _at(block_table), block_table.shape[1], _at(q_start), _at(pos0), n_reqs,
-                                         n_tokens, _at(part), part.numel(), _at(counters), counters.numel(), Hq, Hkv, D, float(scale),
-                                         window, _at(err), _stream_at()),
-           "attention_packed")
+    _check(lib().ferrum_attention_packed(q_at, ldq, out_at, ldo, dt, plane_at, page_stride, n_pages, page_size, table_at, width, start_at, pos_at, n_reqs,
+                                         n_tokens, part_at, part.shape[0], counters_at, counters.shape[0], Hq, Hkv, D, float(scale), window, _at(err),
+                                         _stream_at()), "attention_packed")
 
 
 def swiglu(gu, act, n_tokens, F):
@@ -905,24 +916,24 @@ def sample_filtered(logits, n_rows, out_ids, err, temperature, top_k, top_p, min
     top_p of their mass before them; of these, those with at least min_p times the largest one's probability.  The draw is the first
     of them in index order at which their running mass exceeds uniform times their whole mass.  NaN logits are never drawn.  A row of NaN
     raises error 6, a temperature, top_p or min_p out of range error 7 (id -1 each).  `also_to` (int32) receives the ids as well."""
-    _need(logits, torch.float32, "logits", 2); _need(out_ids, torch.int32, "out_ids", 1); _need(err, torch.int32, "err")
-    for t, dt, name in ((temperature, torch.float32, "temperature"), (top_k, torch.int32, "top_k"), (top_p, torch.float32, "top_p"),
-                        (min_p, torch.float32, "min_p"), (uniform, torch.float64, "uniform"), (rows, torch.int32, "rows")):
-        if t is None and name in ("top_k", "top_p", "min_p", "rows"):
-            continue
-        _need(t, dt, name, 1)
-        if t.shape[0] < n_rows or not t.is_contiguous():
-            raise KernelError(f"sample_filtered: {name} must be contiguous with {n_rows} elements")
-    if rows is None and min(logits.shape[0], out_ids.shape[0]) < n_rows:
+    at, ld = _rows(logits, torch.float32, "logits")
+    _need(err, torch.int32, "err")
+    t_at, u_at = _dense(temperature, torch.float32, "temperature", 1), _dense(uniform, torch.float64, "uniform", 1)
+    k_at = _dense(top_k, torch.int32, "top_k", 1) if top_k is not None else None
+    p_at = _dense(top_p, torch.float32, "top_p", 1) if top_p is not None else None
+    m_at = _dense(min_p, torch.float32, "min_p", 1) if min_p is not None else None
+    r_at = _dense(rows, torch.int32, "rows", 1) if rows is not None else None
+    ids_at, also_at = _dense(out_ids, torch.int32, "out_ids", 1), _dense(also_to, torch.int32, "also_to", 1) if also_to is not None else None
+    for t in (temperature, top_k, top_p, min_p, uniform, rows):
+        if t is not None and t.shape[0] < n_rows:
+            raise KernelError(f"sample_filtered: a parameter has fewer than {n_rows} elements")
+    held, V = logits.shape
+    if rows is None and min(held, out_ids.shape[0], n_rows if also_to is None else also_to.shape[0]) < n_rows:
         raise KernelError(f"sample_filtered: fewer logits or ids than {n_rows} rows")
-    if also_to is not None:
-        _need(also_to, torch.int32, "also_to", 1)
     global _work
     if _profile is not None:
-        _work = (n_rows * logits.shape[1] * 4, 0.0)
-    _check(lib().ferrum_sample_filtered(_at(logits), logits.stride(0), n_rows, logits.shape[1], _at(rows), _at(temperature), _at(top_k),
-                                        _at(top_p), _at(min_p), _at(uniform), _at(out_ids), _at(also_to), _at(err), _stream_at()),
-           "sample_filtered")
+        _work = (n_rows * V * 4, 0.0)
+    _check(lib().ferrum_sample_filtered(at, ld, n_rows, V, r_at, t_at, k_at, p_at, m_at, u_at, ids_at, also_at, _at(err), _stream_at()), "sample_filtered")
 
 
 # ----------------------------------------------------------------------------- parallel gated block

@@ -119,13 +119,16 @@ class PagedAttention(Mixer):
         into a scratch plane, which the kernels of prompt portions then read in the cache's place."""
         Hq, Hkv, D = self.Hq, self.Hkv, self.D
         few, G = ops.attention_packed_rows(), Hq // Hkv
-        if any(0 < n * G <= few for n in ctx.h_q_len):
+        kinds = ctx.step_cache.get(("packed", G))
+        if kinds is None:            # whether the step brings decoded tokens, and portions of prompts
+            kinds = ctx.step_cache[("packed", G)] = (any(0 < n * G <= few for n in ctx.h_q_len), ctx.max_q_len * G > few)
+        if kinds[0]:
             part = ctx.buf("attn_packed_part", (ops.attention_packed_workspace(D),), torch.float32)
             if ops.profiling():      # (a step with prompt portions counts the whole step's work for each kernel)
                 ops.set_work(ops.attention_work(ctx, Hq, Hkv, D, self.window, 9 / 16))
             ops.attention_packed(qkv, out, ctx.n_tokens, table, ctx.q_start, ctx.pos0, cache.plane, cache.page_stride, cache.page_size,
                                  Hq, Hkv, D, self.scale, self.window, ctx.err, part, ctx.zeros("attn_packed_counters", 2 * ctx.n_reqs * Hkv))
-        if ctx.max_q_len * G <= few:
+        if not kinds[1]:
             return
         items, pages = attention_plan.unpack_plan(ctx, cache.group, G, self.window, cache.page_size, few)
         n, whole = items.shape[0], cache.plane.shape[0]
