@@ -12,7 +12,7 @@
 //                weights comes from a product with a constant and goes off every 512 keys, so that the sums do not outgrow what they
 //                stand for; the middles' sum on the CUDA cores in float32.
 // Roundings: q, a power of two times itself that puts a row's largest element at 2^14 to 2^15, is a float16 (exactly, from bfloat16 also, but for what is
-// 2^-30 below the largest); p step, times a power of two that follows the largest step seen, is rounded to float16: a weight's half
+// 2^-30 below the largest); p step, times a power of two that follows the largest one seen, is rounded to float16: a weight's half
 // step of 2^-12, and the result's own.  All sums are float32.
 //
 // The work is handed out on the device, so that the launch does not depend on the lengths and a captured one serves any.  A (request, KV head,
@@ -34,7 +34,7 @@ constexpr int WARPS = 4;
 constexpr int TILE = WARPS * PACKED_POS;     // keys of a unit
 constexpr int NB = 2;                        // blocks of a step: one running maximum for 32 keys
 constexpr float SLACK = 6.f;                 // a weight is at most 2^SLACK times that of the maximum in use
-constexpr int HEAD = 15 - (int)SLACK;        // p step times its power of two is at most 2^(HEAD + SLACK), within float16
+constexpr int HEAD = 12;                     // the largest p step so far is brought to 2^(HEAD - 1) to 2^HEAD: room for one of up to 2^15, within float16
 constexpr int SETTLE = 16;                   // steps after which the sums of codes are centred
 constexpr int HALVES = 2;                    // steps in a warp's ring: one is read while the next arrives
 static_assert(32 % NB == 0, "the blocks of a step lie in one window of 32 blocks, one a lane");
@@ -287,7 +287,7 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, const Item it
         for (int j = 0; j < 4; ++j) o[nt][g][j][c] = o[nt][g][j][2 + c] = 0.f;
       }
     }
-  float step_limit = 0x1p-100f, v_up = __uint_as_float((unsigned)(127 + 100 + HEAD) << 23);       // the largest step seen is at most step_limit = 2^HEAD / v_up
+  float most_allowed = 0x1p-100f, v_up = __uint_as_float((unsigned)(127 + 100 + 15) << 23);      // p step is at most most_allowed = 2^15 / v_up
 
   // (m_run: the maximum in use, a score times f_row.)
   // The step's blocks, the first at key0.  MASKED: some key of theirs is hidden from some row or lies behind the last key.
@@ -344,7 +344,7 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, const Item it
       }
     }
     // ---- the values' steps and middles
-    float step[NB][GN][2], mid[NB][GN][2], most = 0.f;
+    float step[NB][GN][2], mid[NB][GN][2];
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -357,11 +357,9 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, const Item it
           if (MASKED && (b >= n || key0 + b * TILE + gid + 8 * k >= hi)) v = make_float2(0.f, 0.f);      // (what lies behind the last key may be a NaN)
           step[b][g][k] = v.x;
           mid[b][g][k] = v.y;
-          most = fmaxf(most, v.x);
         }
       }
-    // ---- exponents against the maximum in use, which moves only when a score leaves it 2^SLACK behind: a vote in its place
-    // otherwise.  The largest step in use likewise.
+    // ---- exponents against the maximum in use, which moves only when a score leaves it 2^SLACK behind: a vote in its place otherwise
     float x[NB][NT][4], far = -INFINITY;
     auto exponents = [&]() {
 #pragma unroll
@@ -375,7 +373,7 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, const Item it
           }
     };
     if (!MASKED) exponents();
-    if (MASKED || __any_sync(0xffffffffu, far > SLACK || most > step_limit)) {
+    if (MASKED || __any_sync(0xffffffffu, far > SLACK)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -402,23 +400,7 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, const Item it
             }
           }
         }
-      const unsigned top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
-      if (__uint_as_float(top) > step_limit) {
-        const int e = min(127, (int)(top >> 23) - 126);              // top < 2^e
-        const float up = __uint_as_float((unsigned)(127 + HEAD - e) << 23), ratio = up / v_up;
-        step_limit = __uint_as_float(min((unsigned)(127 + e), 254u) << 23);
-        v_up = up;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int g = 0; g < GN; ++g)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              eights[nt][g][c] *= ratio;
-#pragma unroll
-              for (int j = 0; j < 4; ++j) o[nt][g][j][c] *= ratio;
-            }
-      }
+      most_allowed = 0.f;            // (what was the largest product may have shrunk to nothing: found anew below)
       if (MASKED) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -431,32 +413,63 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, const Item it
         exponents();
       }
     }
+    // ---- weights; times a step they are float16 operands, whose power of two follows the largest product (and not the largest step: a key that
+    // nobody looks at must not push the others' weights into the subnormals)
+    float w[NB][NT][4], most = 0.f;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float of_key = 0.f;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float y = exp2_fast(x[b][nt][2 * k + c]);
+            w[b][nt][2 * k + c] = y;
+            l_run[nt][c] += y;
+            of_key = fmaxf(of_key, y);
+          }
+#pragma unroll
+        for (int g = 0; g < GN; ++g) most = fmaxf(most, of_key * step[b][g][k]);
+      }
+    if (__any_sync(0xffffffffu, most > most_allowed)) {
+      const unsigned top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
+      const int e = min(127, (int)(top >> 23) - 126);              // top < 2^e
+      const float up = __uint_as_float((unsigned)(127 + HEAD - e) << 23), ratio = up / v_up;
+      most_allowed = __uint_as_float(min((unsigned)(127 + e + 15 - HEAD), 254u) << 23);
+      v_up = up;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int g = 0; g < GN; ++g)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            eights[nt][g][c] *= ratio;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[nt][g][j][c] *= ratio;
+          }
+    }
     // ---- values
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       unsigned pf[NT][GN][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          w[e] = exp2_fast(x[b][nt][e]);
-          l_run[nt][e & 1] += w[e];
-        }
 #pragma unroll
         for (int g = 0; g < GN; ++g) {
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             const float up = step[b][g][k] * v_up;
-            float y0 = w[2 * k] * up, y1 = w[2 * k + 1] * up;
+            float y0 = w[b][nt][2 * k] * up, y1 = w[b][nt][2 * k + 1] * up;
             if (MASKED) {              // a key that a row does not see counts for nothing, whatever it holds
-              if (w[2 * k] == 0.f) y0 = 0.f;
-              if (w[2 * k + 1] == 0.f) y1 = 0.f;
-              if (w[2 * k] != 0.f) mid_acc[nt][g][0] = fmaf(w[2 * k], mid[b][g][k], mid_acc[nt][g][0]);
-              if (w[2 * k + 1] != 0.f) mid_acc[nt][g][1] = fmaf(w[2 * k + 1], mid[b][g][k], mid_acc[nt][g][1]);
+              if (w[b][nt][2 * k] == 0.f) y0 = 0.f;
+              if (w[b][nt][2 * k + 1] == 0.f) y1 = 0.f;
+              if (w[b][nt][2 * k] != 0.f) mid_acc[nt][g][0] = fmaf(w[b][nt][2 * k], mid[b][g][k], mid_acc[nt][g][0]);
+              if (w[b][nt][2 * k + 1] != 0.f) mid_acc[nt][g][1] = fmaf(w[b][nt][2 * k + 1], mid[b][g][k], mid_acc[nt][g][1]);
             } else {
-              mid_acc[nt][g][0] = fmaf(w[2 * k], mid[b][g][k], mid_acc[nt][g][0]);
-              mid_acc[nt][g][1] = fmaf(w[2 * k + 1], mid[b][g][k], mid_acc[nt][g][1]);
+              mid_acc[nt][g][0] = fmaf(w[b][nt][2 * k], mid[b][g][k], mid_acc[nt][g][0]);
+              mid_acc[nt][g][1] = fmaf(w[b][nt][2 * k + 1], mid[b][g][k], mid_acc[nt][g][1]);
             }
             pf[nt][g][k] = transpose8(pack2<__half>(y0, y1));
           }

@@ -182,14 +182,14 @@ template <> __device__ __forceinline__ float largest<__half>() { return 65504.f;
 template <typename T, int D>
 __global__ void __launch_bounds__(256)
 unpack_kernel(const uint8_t* __restrict__ plane, long long page_stride, int n_pages, int page_size, const int* __restrict__ block_table,
-              int table_width, const int* __restrict__ items, T* __restrict__ out, int Hkv, int* __restrict__ err) {
+              int table_rows, int table_width, const int* __restrict__ items, T* __restrict__ out, int Hkv, int* __restrict__ err) {
   using B = PackedBlock<D>;
   constexpr int WORDS = D / 8, AT_ONCE = 256 / WORDS, ROUNDS = (2 * PACKED_POS + AT_ONCE - 1) / AT_ONCE;      // rows of keys and values of a block
   pdl_wait();
   pdl_launch();
   const int item = blockIdx.x, h = blockIdx.y;
   const int req = items[2 * item], lp = items[2 * item + 1];
-  const int page = lp >= 0 && lp < table_width ? block_table[(size_t)req * table_width + lp] : -1;
+  const int page = req >= 0 && req < table_rows && lp >= 0 && lp < table_width ? block_table[(size_t)req * table_width + lp] : -1;
   const bool missing = page < 0 || page >= n_pages;
   if (missing && threadIdx.x == 0) atomicExch(err, 5);
   const uint8_t* head = plane + (size_t)(missing ? 0 : page) * page_stride + (size_t)h * (page_size / PACKED_POS) * B::BYTES;
@@ -270,7 +270,7 @@ FERRUM_API int ferrum_rope_cache_write_packed(const void* qkv, int dtype, int n_
 }
 
 // items: [n_items][2] int32 (request, page of the request); out: [n_items][2][Hkv][page_size][D].
-FERRUM_API int ferrum_unpack_cache(const void* plane, long long page_stride, int n_pages, int page_size, const int* block_table, int table_width,
+FERRUM_API int ferrum_unpack_cache(const void* plane, long long page_stride, int n_pages, int page_size, const int* block_table, int table_rows, int table_width,
                                    const int* items, int n_items, void* out, int dtype, int Hkv, int D, int* err_flag, cudaStream_t stream) {
   FERRUM_CHECK_ARG(D == 64 || D == 128, "unpack_cache: a cache in 4 bits has heads of 64 or 128 elements, found %d", D);
   FERRUM_CHECK_ARG(packed_page_ok(page_size) && table_width > 0 && n_pages > 0 && Hkv > 0 && Hkv <= 65535 && n_items >= 0,
@@ -279,8 +279,8 @@ FERRUM_API int ferrum_unpack_cache(const void* plane, long long page_stride, int
   if (n_items == 0) return 0;
   const dim3 grid(n_items, Hkv);
   FERRUM_DISPATCH_16BIT(dtype, T, {
-    if (D == 64) launch_kernel(unpack_kernel<T, 64>, grid, dim3(256), 0, stream, (const uint8_t*)plane, page_stride, n_pages, page_size, block_table, table_width, items, (T*)out, Hkv, err_flag);
-    else launch_kernel(unpack_kernel<T, 128>, grid, dim3(256), 0, stream, (const uint8_t*)plane, page_stride, n_pages, page_size, block_table, table_width, items, (T*)out, Hkv, err_flag);
+    if (D == 64) launch_kernel(unpack_kernel<T, 64>, grid, dim3(256), 0, stream, (const uint8_t*)plane, page_stride, n_pages, page_size, block_table, table_rows, table_width, items, (T*)out, Hkv, err_flag);
+    else launch_kernel(unpack_kernel<T, 128>, grid, dim3(256), 0, stream, (const uint8_t*)plane, page_stride, n_pages, page_size, block_table, table_rows, table_width, items, (T*)out, Hkv, err_flag);
   });
   FERRUM_CHECK_LAUNCH("unpack_cache");
   return 0;

@@ -49,7 +49,7 @@ struct FilterParams {
   int* out_ids;
   int* also_to;
   int* err;
-  int ld, V, per, shift;            // per: logits of a CTA's slice
+  int ld, V, per, shift, held;      // per: logits of a CTA's slice; held: rows that there are
 };
 
 // A token stays while (key, index) comes no later than the threshold: larger keys first, then lower indices.
@@ -602,6 +602,10 @@ sample_filtered_kernel(const FilterParams p) {
   pdl_wait();
   pdl_launch();
   const int q = blockIdx.x, r = p.rows ? p.rows[q] : q, rank = blockIdx.y;
+  if (r < 0 || r >= p.held) {       // (the same for the whole cluster)
+    if (tid == 0 && rank == 0) atomicExch(p.err, 7);
+    return;
+  }
   const float* row = p.logits + (size_t)r * p.ld;
   const float T = p.temperature[q], top_p = p.top_p ? p.top_p[q] : 1.f, min_p = p.min_p ? p.min_p[q] : 0.f;
   const int top_k = p.top_k ? p.top_k[q] : 0, lo = min(p.V, rank * p.per), n = min(p.V, lo + p.per) - lo;
@@ -696,10 +700,11 @@ constexpr int MOST_RESIDENT = 45 * 1024;
 
 }  // namespace
 
-FERRUM_API int ferrum_sample_filtered(const float* logits, int ld, int n_rows, int V, const int* rows, const float* temperature, const int* top_k,
+// held: rows of the logits, of out_ids and of also_to; a row named in `rows` beyond them is left out and raises error 7.
+FERRUM_API int ferrum_sample_filtered(const float* logits, int ld, int held, int n_rows, int V, const int* rows, const float* temperature, const int* top_k,
                                       const float* top_p, const float* min_p, const double* uniform, int* out_ids, int* also_to, int* err_flag,
                                       cudaStream_t stream) {
-  FERRUM_CHECK_ARG(n_rows >= 0 && V > 0 && ld >= V, "sample_filtered: bad sizes rows=%d V=%d ld=%d", n_rows, V, ld);
+  FERRUM_CHECK_ARG(n_rows >= 0 && V > 0 && ld >= V && held >= 0, "sample_filtered: bad sizes rows=%d V=%d ld=%d", n_rows, V, ld);
   FERRUM_CHECK_ARG(temperature && uniform && out_ids && err_flag, "sample_filtered: temperature, uniform, out_ids and the error flag are required");
   if (n_rows == 0) return 0;
   int bits = 0;
@@ -707,7 +712,7 @@ FERRUM_API int ferrum_sample_filtered(const float* logits, int ld, int n_rows, i
   // A few rows: clusters of 16 CTAs of 1,024 threads, so that the whole GPU reads them; more: 8 CTAs of 512.  Small vocabularies: one CTA.
   const int sms = ferrum_sm_count(), ctas = V < 16384 ? 1 : n_rows * MAX_CLUSTER <= sms && V >= 65536 ? MAX_CLUSTER : 8;
   const int threads = n_rows * ctas <= sms && V >= 8192 ? 1024 : 512;
-  FilterParams p{logits, rows, temperature, top_k, top_p, min_p, uniform, out_ids, also_to, err_flag, ld, V, (V + ctas - 1) / ctas, bits > 17 ? 62 - bits : 45};
+  FilterParams p{logits, rows, temperature, top_k, top_p, min_p, uniform, out_ids, also_to, err_flag, ld, V, (V + ctas - 1) / ctas, bits > 17 ? 62 - bits : 45, held};
   if (p.per <= MOST_RESIDENT) return launch_sample<true>(p, n_rows, ctas, threads, stream);
   return launch_sample<false>(p, n_rows, ctas, threads, stream);
 }

@@ -35,9 +35,9 @@ ABI = 25
 _KINDS = {"p": c_void_p, "i": c_int, "l": c_longlong, "f": c_float}
 _ARGUMENTS = {
     "ferrum_rope_cache_write_packed": "piiipipppipipliiiiiiiipp",
-    "ferrum_unpack_cache": "pliipipipiiipp",
+    "ferrum_unpack_cache": "pliipiipipiiipp",
     "ferrum_attention_packed": "pipiipliipippiiplpiiiifipp",
-    "ferrum_sample_filtered": "piiipppppppppp",
+    "ferrum_sample_filtered": "piiiipppppppppp",
 }
 
 _CTYPES = (ctypes._SimpleCData, ctypes.Array, type(ctypes.byref(c_int())))
@@ -843,7 +843,8 @@ def rope_cache_write_packed(qkv, n_tokens, positions, req_of_token, block_table,
 
 def unpack_cache(plane, page_stride, page_size, block_table, items, out, err):
     """out[i] = the 16-bit keys and values of page items[i, 1] of request items[i, 0] (int32 [n, 2]); out: [>= n, 2, Hkv, page_size, D] of
-    the cache's 16-bit type.  A page that the request does not hold arrives as zeros and raises the error flag."""
+    the cache's 16-bit type.  A page that the request does not hold (or a request that the table does not) arrives as zeros and
+    raises the error flag."""
     dt = dtype_code(out.dtype) if isinstance(out, torch.Tensor) and out.dtype in SIXTEEN_BIT else _need16(out, "out", 5)
     out_at, items_at, table_at = _dense(out, out.dtype, "out", 5), _dense(items, torch.int32, "items", 2), _dense(block_table, torch.int32, "block_table", 2)
     held, two, Hkv, page, D = out.shape
@@ -854,7 +855,7 @@ def unpack_cache(plane, page_stride, page_size, block_table, items, out, err):
     global _work
     if _profile is not None:
         _work = (n * Hkv * page_size * D * (9 / 8 + 4), 0.0)
-    _check(lib().ferrum_unpack_cache(plane_at, page_stride, n_pages, page_size, table_at, block_table.shape[1], items_at, n, out_at, dt, Hkv, D, _at(err),
+    _check(lib().ferrum_unpack_cache(plane_at, page_stride, n_pages, page_size, table_at, *block_table.shape, items_at, n, out_at, dt, Hkv, D, _at(err),
                                      _stream_at()), "unpack_cache")
 
 
@@ -915,7 +916,8 @@ def sample_filtered(logits, n_rows, out_ids, err, temperature, top_k, top_p, min
     min_p may be None.  The filters work in this order: the top_k largest logits (of equal ones the lower index); of these, by descending logit, those with less than
     top_p of their mass before them; of these, those with at least min_p times the largest one's probability.  The draw is the first
     of them in index order at which their running mass exceeds uniform times their whole mass.  NaN logits are never drawn.  A row of NaN
-    raises error 6, a temperature, top_p or min_p out of range error 7 (id -1 each).  `also_to` (int32) receives the ids as well."""
+    raises error 6, a temperature, top_p or min_p out of range error 7 (id -1 each), as does a row that the logits or the ids do not
+    have (left out).  `also_to` (int32) receives the ids as well."""
     at, ld = _rows(logits, torch.float32, "logits")
     _need(err, torch.int32, "err")
     t_at, u_at = _dense(temperature, torch.float32, "temperature", 1), _dense(uniform, torch.float64, "uniform", 1)
@@ -928,12 +930,13 @@ def sample_filtered(logits, n_rows, out_ids, err, temperature, top_k, top_p, min
         if t is not None and t.shape[0] < n_rows:
             raise KernelError(f"sample_filtered: a parameter has fewer than {n_rows} elements")
     held, V = logits.shape
-    if rows is None and min(held, out_ids.shape[0], n_rows if also_to is None else also_to.shape[0]) < n_rows:
+    held = min(held, out_ids.shape[0]) if also_to is None else min(held, out_ids.shape[0], also_to.shape[0])
+    if rows is None and held < n_rows:
         raise KernelError(f"sample_filtered: fewer logits or ids than {n_rows} rows")
     global _work
     if _profile is not None:
         _work = (n_rows * V * 4, 0.0)
-    _check(lib().ferrum_sample_filtered(at, ld, n_rows, V, r_at, t_at, k_at, p_at, m_at, u_at, ids_at, also_at, _at(err), _stream_at()), "sample_filtered")
+    _check(lib().ferrum_sample_filtered(at, ld, held, n_rows, V, r_at, t_at, k_at, p_at, m_at, u_at, ids_at, also_at, _at(err), _stream_at()), "sample_filtered")
 
 
 # ----------------------------------------------------------------------------- parallel gated block

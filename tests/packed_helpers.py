@@ -40,7 +40,7 @@ def block_bytes(k, v, dtype):
 class Cache:
     """Random keys and values of some requests in packed pages, in a scattered order, with bytes of 0xff (NaN pairs) wherever no position lies."""
 
-    def __init__(self, lengths, Hkv, D, page, dtype, seed, spread=1.0, offset=1.0, spare=3, width=None, fill=255):
+    def __init__(self, lengths, Hkv, D, page, dtype, seed, spread=1.0, offset=1.0, spare=3, width=None, fill=255, size=None):
         g = torch.Generator(device="cuda").manual_seed(seed)
         n_pages = [-(-n // page) for n in lengths]
         total = sum(n_pages) + spare
@@ -54,6 +54,8 @@ class Cache:
             table[r, :m] = torch.tensor(mine, dtype=torch.int32)
             kv = spread * torch.randn(2, Hkv, m * page, D, device="cuda", generator=g)
             kv = kv + offset * torch.randn(2, Hkv, 1, D, device="cuda", generator=g)
+            if size is not None and m:                      # a factor per position
+                kv = kv * size(m * page)[:, None]
             c, s, z = quantise(kv, dtype)
             vals = values(c, s, z)
             self.keys.append(vals[0, :, :n]); self.vals.append(vals[1, :, :n])
@@ -86,7 +88,7 @@ def attention(q, keys, vals, mids, pos0, scale, window, dtype, unpacked=False):
     s = s.masked_fill(~seen, -math.inf)
     p = torch.softmax(s, -1)
     out = torch.einsum("hgnl,hld->nhgd", p, vals)
-    size = torch.einsum("nhgd,hld->hgnl", qg.abs(), keys.abs()).masked_fill(~seen, 0) * scale
+    size = torch.einsum("nhgd,hld->hgnl", qg.abs(), keys.abs()).masked_fill(~seen, 0) * abs(scale)
     if unpacked:
         weight = p * (2 * h + 2 * (size * (h + 2.0 ** -20)).amax(-1, keepdim=True) + 2.0 ** -20)
         off = torch.einsum("hgnl,hld->nhgd", weight, vals.abs())

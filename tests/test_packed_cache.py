@@ -97,7 +97,7 @@ def test_wrappers_refuse_what_the_kernels_are_not_built_for():
     assert lib.ferrum_attention_packed(null, 512, null, 512, ops.BF16, null, 1152, 2, 16, null, 4, null, null, 1, 1, null, ops.c_longlong(1 << 40), null, 99, 2, 1, 96,
                                        ops.c_float(1.0), 0, ops.c_void_p(16), null) == 1
     assert b"64 or 128" in lib.ferrum_last_error()
-    assert lib.ferrum_unpack_cache(null, 1152, 2, 16, null, 4, null, 1, null, ops.F32, 1, 64, ops.c_void_p(16), null) == 1
+    assert lib.ferrum_unpack_cache(null, 1152, 2, 16, null, 1, 4, null, 1, null, ops.F32, 1, 64, ops.c_void_p(16), null) == 1
     assert b"16-bit" in lib.ferrum_last_error()
     assert lib.ferrum_rope_cache_write_packed(null, ops.BF16, 1, 100, null, 512, null, null, null, 4, null, 0, null, 1152, 2, 16, 2, 1, 64, 0, 0, 1,
                                               ops.c_void_p(16), null) == 1

@@ -137,7 +137,7 @@ def test_unpack(cuda, dtype, D, Hkv, page):
                 want[0], want[1] = (t[0][:, lp * page:(lp + 1) * page] for t in (c.keys, c.vals))
             assert torch.equal(out[i], want.to(dtype))
     err = err_flag()
-    ops.unpack_cache(c.plane, c.plane.stride(0), page, table, torch.tensor([[0, 7], [0, 90], [0, -1]], dtype=torch.int32, device="cuda"),
+    ops.unpack_cache(c.plane, c.plane.stride(0), page, table, torch.tensor([[0, 7], [0, 90], [7, 0]], dtype=torch.int32, device="cuda"),
                      torch.empty(3, 2, Hkv, page, D, dtype=dtype, device="cuda"), err)
     assert err.item() == 5
 
@@ -188,6 +188,74 @@ def test_scores_far_apart(cuda, dtype):
     s = H.Step(c, [1, 2], 8, 6)
     s.qkv *= 12
     s.check(s.attend(), "large scores")
+
+
+@pytest.mark.parametrize("dtype", H.DTYPES)
+@pytest.mark.parametrize("kind", ["zeros", "constant", "growing", "shrinking", "tiny", "far offset"])
+@pytest.mark.parametrize("new", [[1, 1], [4, 2]])
+def test_values_of_many_sizes(cuda, dtype, kind, new):
+    """Groups without a range (steps of 0), steps that grow or shrink by orders of magnitude along a context, very small ones, values far from 0."""
+    spread, offset = {"zeros": (0.0, 0.0), "constant": (0.0, 1.0), "tiny": (1e-5, 1e-5), "far offset": (0.1, 30.0)}.get(kind, (1.0, 1.0))
+    size = None
+    if kind in ("growing", "shrinking"):
+        size = lambda m: 10.0 ** torch.linspace(-4, 3, m, device="cuda").flip(0 if kind == "shrinking" else ())
+    c = H.Cache([900, 70], 2, 128, 16, dtype, 31, spread=spread, offset=offset, size=size)
+    s = H.Step(c, new, 8, 32)
+    s.check(s.attend(), kind)
+
+
+@pytest.mark.parametrize("dtype", H.DTYPES)
+@pytest.mark.parametrize("seen", ["never", "first"])
+def test_a_value_far_larger_than_the_others(cuda, dtype, seen):
+    """A value 10^4 (float16) or 10^7 times as large as the others under a key that no row attends to, or that was the best one seen before a far better
+    one came: the others' weights keep their precision."""
+    far = 1e4 if dtype == torch.float16 else 1e7
+    c = H.Cache([2100], 1, 128, 16, dtype, 41, spread=0.3, offset=0.0)
+    s = H.Step(c, [1], 4, 42)
+    # the key at 37 is the negative query, so that its score is far below all others; or (first) the query, and the last 500 keys are twice that
+    q = s.qkv[0, :128].float()
+    s.qkv[:, :512] = s.qkv[:, :128].repeat(1, 4)
+    kv = torch.stack([c.keys[0].float(), c.vals[0].float()])                       # [2, 1, 2100, 128]
+    kv[0, 0, 37] = -8 * q if seen == "never" else 4 * q
+    if seen == "first":
+        kv[0, 0, -500:] += 8 * q
+    kv[1, 0, 37] *= far
+    codes, step, mid = H.quantise(kv, dtype)
+    vals = H.values(codes, step, mid)
+    c.keys, c.vals, c.mids = [vals[0]], [vals[1]], [mid[1].double().repeat_interleave(64, -1)]
+    pad = lambda t: torch.cat([t, torch.zeros(2, 1, 12, t.shape[-1], dtype=t.dtype, device="cuda")], 2).unflatten(2, (132, 1, 16)).transpose(1, 2)
+    c.plane[c.table[0].long()] = H.block_bytes(*[[pad(t)[i] for t in (codes, step, mid)] for i in (0, 1)], dtype)
+    s.check(s.attend(), seen)
+
+
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-4, 3.0])
+def test_score_scales(cuda, scale):
+    for new in ([1, 1], [3, 2], [40, 1]):
+        s = H.Step(H.Cache([300, 77], 2, 64, 16, torch.float16, 33), new, 8, 34)
+        s.mixer.scale = scale
+        s.check(s.attend(), f"scale {scale}")
+
+
+@pytest.mark.parametrize("new,window", [([1, 2], 0), ([2, 4], 40)])
+def test_nan_in_hidden_places_stays_there(cuda, new, window):
+    """Keys and values that a row does not see (behind it in its own request, ahead of its window, on pages of nobody) may be NaN; a NaN that a
+    row sees spoils that row alone."""
+    c = H.Cache([200, 333], 2, 128, 16, torch.bfloat16, 35, fill=255)
+    s = H.Step(c, new, 8, 36, window)
+    want = s.attend()
+    s.check(want, "hidden")
+    pairs = c.plane.view(torch.bfloat16)                        # a block: 16 * D / 2 pairs' worth of codes first
+    at = lambda pos: (int(c.table[1, pos // 16].item()), slice(None), pos % 16 // 16, slice(8 * 128 + pos % 16 * 4, 8 * 128 + pos % 16 * 4 + 4))
+    if window:
+        pairs[at(333 - 4 - window - 1)] = float("nan")          # ahead of every row's window
+        assert torch.equal(s.attend(), want)
+        pairs[at(333 - 4 - window + 1)] = float("nan")          # the first row sees it, the others do not
+        out = s.attend()
+        assert torch.isnan(out[2]).all() and torch.equal(out[[0, 1, 3, 4, 5]], want[[0, 1, 3, 4, 5]])
+    else:
+        pairs[at(332)] = float("nan")                           # the last token's own key: hidden from the one before it
+        out = s.attend()
+        assert torch.equal(out[:2], want[:2]) and torch.isnan(out[2]).all()
 
 
 def test_rows_of_other_requests_and_wider_rows(cuda):
@@ -324,3 +392,22 @@ def test_engine_refuses_models_that_cannot(cuda, model_dirs):
         Engine(model_dirs["A"], dtype="float32", cache_bits=4, num_pages=16, max_model_len=64)
     with pytest.raises(ConfigError, match="multiple of 16"):
         Engine(model_dirs["D"], dtype="bfloat16", cache_bits=4, num_pages=16, max_model_len=64, page_size=8)
+
+
+def test_command_line(cuda, model_dirs):
+    """`ferrum generate` with a cache in 4 bits and filters: the tokens of the Python entry point; what it refuses."""
+    import json
+    import subprocess
+    import sys
+
+    from conftest import ROOT
+    run = lambda *args: subprocess.run([sys.executable, ROOT + "/bin/ferrum", "generate", "--model", *args], capture_output=True, text=True, cwd=ROOT, timeout=600)
+    common = ("--prompt-tokens", "5,17,3", "--max-new-tokens", "6", "--num-pages", "16", "--max-model-len", "64")
+    p = run(model_dirs["D"], *common, "--cache-bits", "4", "--temperature", "0.7", "--top-k", "30", "--top-p", "0.9", "--min-p", "0.01", "--seed", "5", "--profile")
+    assert p.returncode == 0, p.stderr
+    eng = engine(model_dirs, "D", 4)
+    assert json.loads(p.stdout)["tokens"] == eng.generate([[5, 17, 3]], 6, 0.7, 5, (), 30, 0.9, 0.01)[0]
+    assert "attention_packed" in p.stderr and "sample_filtered" in p.stderr
+    for args, word in ((("--top-p", "1.5", "--temperature", "1"), "top_p"), (("--cache-bits", "8"), "8 bits"), (("--page-size", "8", "--cache-bits", "4"), "multiple of 16")):
+        p = run(model_dirs["D"], *common, *args)
+        assert p.returncode == 1 and word in p.stderr, p.stderr

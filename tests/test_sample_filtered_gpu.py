@@ -163,6 +163,8 @@ def test_picked_rows_strides_and_a_second_place(cuda):
     want = {4: P.draw(host[4], 1.0, 0, 0.7, 0.0, 0.3)[0], 1: P.draw(host[1], 0.5, 7, 1.0, 0.0, 0.8)[0]}
     assert err == 0 and ids == [want.get(r, -7) for r in range(6)] and also.tolist() == [want.get(r, -9) for r in range(9)]
     assert sample(x, [1.0], None, None, None, [0.5], n=0)[0] == [-7] * 6
+    ids, err = sample(x, [1.0, 1.0, 1.0], None, None, None, [0.3, 0.3, 0.3], rows=[6, 2, -1])       # rows that are not there
+    assert err == 7 and ids[2] >= 0 and ids[:2] + ids[3:] == [-7] * 5
 
 
 def test_replayed_graph_and_another_stream(cuda):

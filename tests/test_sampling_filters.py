@@ -47,7 +47,7 @@ def test_wrapper_refuses():
     x, f, i = torch.zeros(2, 10), torch.zeros(2), torch.zeros(2, dtype=torch.int32)
     with pytest.raises(KernelError, match="CUDA tensor"):
         ops.sample_filtered(x, 2, i, i, f, i, f, f, f.double())
-    assert ops.lib().ferrum_sample_filtered(None, 5, 2, 10, None, None, None, None, None, None, None, None, None, None) == 1
+    assert ops.lib().ferrum_sample_filtered(None, 5, 2, 2, 10, None, None, None, None, None, None, None, None, None, None) == 1
     assert b"bad sizes" in ops.lib().ferrum_last_error()
-    assert ops.lib().ferrum_sample_filtered(None, 10, 2, 10, None, None, None, None, None, None, None, None, None, None) == 1
+    assert ops.lib().ferrum_sample_filtered(None, 10, 2, 2, 10, None, None, None, None, None, None, None, None, None, None) == 1
     assert b"required" in ops.lib().ferrum_last_error()
