@@ -25,7 +25,7 @@ typedef unsigned long long u64;
 constexpr int BINS = 2048;
 constexpr int MAX_CLUSTER = 16;
 constexpr int MAX_WARPS = 32;
-constexpr int SEGMENTS = 4;         // parts of a warp's run whose masses are kept for the draw
+constexpr int SEGMENTS = 2;         // parts of a warp's run whose masses are kept for the draw
 constexpr int LIST = 1024;          // listed tokens of a CTA, LIST / warps of a warp
 constexpr int MOST_BINS = 4;        // bins of a thread's share: BINS / 512
 constexpr int FEW = 1024;           // tokens that one CTA sorts
@@ -119,19 +119,59 @@ struct Row {
 
   // w * 2^shift of a key, not rounded.  exp by 2^(n / 64) from a table and the series of the rest (below 2^-7 in size: the sixth term is
   // 3e-17 of the sum); what is below 2^-1 after the scaling rounds to 0 whatever its value.
+  // Without a branch, so that several weights are on their way at a time.
   __device__ __forceinline__ double scaled_weight(uint32_t k) const {
-    if (k == best) return (double)(1ull << p.shift);
-    const double y = ((double)key_value(k) - (double)top) * inv_t * 92.332482616893656877;      // 64 log2(e)
-    if (!(y > -3000.0)) return 0.0;
+    const double exact = ((double)key_value(k) - (double)top) * inv_t * 92.332482616893656877;      // 64 log2(e)
+    const double y = fmax(exact, -3000.0);                        // (-infinity, and the NaN of two infinities)
     const double t = y + 6755399441055744.0;                       // 1.5 * 2^52: the nearest whole number in the low bits
     const int n = __double2loint(t);
     const double q = (y - (t - 6755399441055744.0)) * 0.010830424696249145347;               // ln(2) / 64
     const double s = fma(q, fma(q, fma(q, fma(q, fma(q, 1.0 / 120.0, 1.0 / 24.0), 1.0 / 6.0), 0.5), 1.0), 1.0);
     const double v = sh.powers[n & 63] * s;
-    return __hiloint2double(__double2hiint(v) + (((n >> 6) + p.shift) << 20), __double2loint(v));
+    const double w = __hiloint2double(__double2hiint(v) + (((n >> 6) + p.shift) << 20), __double2loint(v));
+    return k == best ? (double)(1ull << p.shift) : exact > -3000.0 ? w : 0.0;
   }
   static __device__ __forceinline__ u64 whole(double v) { return (u64)__double_as_longlong(v + 4503599627370496.0) & 0xfffffffffffffull; }      // (v below 2^51)
   __device__ __forceinline__ u64 mass(uint32_t k) const { return whole(scaled_weight(k)); }
+
+  // hist[bin_of(k)] += 1 or (MASS) the mass of k, for the tokens of the warp's run that wanted(key, entry) names.
+  template <bool MASS, typename Wanted, typename Bin>
+  __device__ __forceinline__ void fill_histogram(Wanted wanted, Bin bin_of) {
+    const int lane = threadIdx.x & 31;
+    for (int i = threadIdx.x; i < BINS; i += blockDim.x) sh.hist[i] = 0;
+    __syncthreads();
+    constexpr int AT_ONCE = 4;
+    for (int e = e0 + lane; e - lane < e1; e += 32 * AT_ONCE) {
+      uint32_t k[AT_ONCE];
+      u64 v[AT_ONCE];
+      bool any = false;
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) {
+        const int at = e + 32 * i;
+        k[i] = at < e1 ? key(at) : 0;
+        if (k[i] && !wanted(k[i], at)) k[i] = 0;
+        any |= k[i] != 0;
+      }
+      if (!__any_sync(0xffffffffu, any)) continue;
+      if (MASS) {
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) v[i] = mass(k[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) {
+        if (k[i] == 0) continue;
+        unsigned* half = reinterpret_cast<unsigned*>(&sh.hist[bin_of(k[i])]);      // (a 64-bit addition by two of 32 bits, the second hardly ever made)
+        if (MASS) {
+          const unsigned low = (unsigned)v[i];
+          if (v[i] == 0) continue;
+          const unsigned old = atomicAdd(half, low), high = (unsigned)(v[i] >> 32) + (old + low < old ? 1 : 0);
+          if (high) atomicAdd(half + 1, high);
+        } else {
+          atomicAdd(half, 1u);
+        }
+      }
+    }
+  }
 
   // Sums (or maxima of) two numbers over the block, then hands them to every CTA; afterwards exchange[..][0 or 1][c] holds CTA c's.
   template <bool MAXIMA>
@@ -229,23 +269,7 @@ struct Row {
     if (!(isfinite(top) && isfinite(range))) return false;
     const float scale = (float)BINS / range;
     auto bin_of = [&](uint32_t k) { return min(BINS - 1, (int)((top - key_value(k)) * scale)); };
-    for (int i = tid; i < BINS; i += blockDim.x) sh.hist[i] = 0;
-    __syncthreads();
-#pragma unroll 4
-    for (int e = e0 + lane; e < e1; e += 32) {
-      const uint32_t k = key(e);
-      if (k == 0) continue;
-      unsigned* half = reinterpret_cast<unsigned*>(&sh.hist[bin_of(k)]);
-      if (BY_MASS) {
-        const u64 v = mass(k);
-        const unsigned low = (unsigned)v;
-        if (v == 0) continue;
-        const unsigned old = atomicAdd(half, low), high = (unsigned)(v >> 32) + (old + low < old ? 1 : 0);
-        if (high) atomicAdd(half + 1, high);
-      } else {
-        atomicAdd(half, 1u);
-      }
-    }
+    fill_histogram<BY_MASS>([](uint32_t, int) { return true; }, bin_of);
     cluster_sync();
     u64 mine[MOST_BINS], own, all, at;
     int b0, each;
@@ -398,23 +422,7 @@ struct Row {
         whole_known = true;
         known.bin = -1;
       } else {
-        for (int i = tid; i < BINS; i += blockDim.x) sh.hist[i] = 0;
-        __syncthreads();
-#pragma unroll 4
-        for (int e = e0 + lane; e < e1; e += 32) {
-          const uint32_t k = key(e);
-          if (k < lo_key || k > hi_key || !cut.stays(k, index(e))) continue;
-          unsigned* half = reinterpret_cast<unsigned*>(&sh.hist[bin_of(k)]);      // (a 64-bit addition by two of 32 bits, the second hardly ever made)
-          if (MASS) {
-            const u64 v = mass(k);
-            const unsigned low = (unsigned)v;
-            if (v == 0) continue;
-            const unsigned old = atomicAdd(half, low), high = (unsigned)(v >> 32) + (old + low < old ? 1 : 0);
-            if (high) atomicAdd(half + 1, high);
-          } else {
-            atomicAdd(half, 1u);
-          }
-        }
+        fill_histogram<MASS>([&](uint32_t k, int e) { return k >= lo_key && k <= hi_key && cut.stays(k, index(e)); }, bin_of);
         cluster_sync();
         u64 mine[MOST_BINS], own, all, at;
         int b0, each;
@@ -536,18 +544,32 @@ struct Row {
   __device__ __forceinline__ void draw(const Cut cut, double min_w, double u, int out) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int rows = (e1 - e0 + 31) / 32;
-    auto mass_at = [&](int r) -> u64 {
-      const int e = e0 + r * 32 + lane;
-      const uint32_t k = e < e1 ? key(e) : 0;
-      if (k == 0 || !cut.stays(k, index(e))) return 0;
-      const double v = scaled_weight(k);
-      return v >= min_w ? whole(v) : 0;
+    // the masses of entries of the lines r .. r + AT_ONCE - 1 (of 32) before `end`; false: none has any
+    constexpr int AT_ONCE = 4;
+    auto masses = [&](int r, int end, u64 (&m)[AT_ONCE]) {
+      uint32_t k[AT_ONCE];
+      bool any = false;
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) {
+        const int e = e0 + (r + i) * 32 + lane;
+        k[i] = r + i < end && e < e1 ? key(e) : 0;
+        if (k[i] && !cut.stays(k[i], index(e))) k[i] = 0;
+        any |= k[i] != 0;
+      }
+      if (!__any_sync(0xffffffffu, any)) return false;
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) {
+        const double v = scaled_weight(k[i]);
+        m[i] = k[i] && v >= min_w ? whole(v) : 0;
+      }
+      return true;
     };
     u64 sum = 0;
     for (int s = 0; s < SEGMENTS; ++s) {
-      u64 part = 0;
-#pragma unroll 4
-      for (int r = rows * s / SEGMENTS; r < rows * (s + 1) / SEGMENTS; ++r) part += mass_at(r);
+      u64 part = 0, m[AT_ONCE];
+      const int end = rows * (s + 1) / SEGMENTS;
+      for (int r = rows * s / SEGMENTS; r < end; r += AT_ONCE)
+        if (masses(r, end, m)) part += m[0] + m[1] + m[2] + m[3];
       sum += part;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
@@ -567,20 +589,25 @@ struct Row {
     for (int s = 0; s < SEGMENTS; ++s) {
       const u64 part = sh.segment[warp][s];
       if (threshold >= at && threshold < at + part) {
-        for (int r = rows * s / SEGMENTS; r < rows * (s + 1) / SEGMENTS; ++r) {
-          const u64 own = mass_at(r);
-          u64 run = own;
+        const int end = rows * (s + 1) / SEGMENTS;
+        u64 m[AT_ONCE];
+        for (int r = rows * s / SEGMENTS; r < end; r += AT_ONCE) {
+          if (!masses(r, end, m)) continue;
 #pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const u64 v = __shfl_up_sync(0xffffffffu, run, o);
-            if (lane >= o) run += v;
+          for (int i = 0; i < AT_ONCE; ++i) {
+            u64 run = m[i];
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+              const u64 v = __shfl_up_sync(0xffffffffu, run, o);
+              if (lane >= o) run += v;
+            }
+            if (threshold >= at + run - m[i] && threshold < at + run) {
+              const int id = index(e0 + (r + i) * 32 + lane);
+              p.out_ids[out] = id;
+              if (p.also_to) p.also_to[out] = id;
+            }
+            at += __shfl_sync(0xffffffffu, run, 31);
           }
-          if (threshold >= at + run - own && threshold < at + run) {
-            const int id = index(e0 + r * 32 + lane);
-            p.out_ids[out] = id;
-            if (p.also_to) p.also_to[out] = id;
-          }
-          at += __shfl_sync(0xffffffffu, run, 31);
         }
         return;
       }
@@ -622,12 +649,23 @@ sample_filtered_kernel(const FilterParams p) {
   }
   // ---- the slice, its largest key and its smallest of a finite logit
   uint32_t most = 0, least_finite = ~0u;
-#pragma unroll 8
-  for (int i = tid; i < n; i += blockDim.x) {
-    const uint32_t k = order_key(row[lo + i]);
-    if (RESIDENT) slice[i] = k;
+  auto take = [&](float x) {
+    const uint32_t k = order_key(x);
     most = max(most, k);
     if (k > 0x007fffffu) least_finite = min(least_finite, k);      // (0x007fffff: minus infinity)
+    return k;
+  };
+  const int quads = ((uintptr_t)(row + lo) & 15) == 0 ? n / 4 : 0;
+#pragma unroll 4
+  for (int i = tid; i < quads; i += blockDim.x) {
+    const float4 x = reinterpret_cast<const float4*>(row + lo)[i];
+    const uint4 k = make_uint4(take(x.x), take(x.y), take(x.z), take(x.w));
+    if (RESIDENT) reinterpret_cast<uint4*>(slice)[i] = k;
+  }
+#pragma unroll 8
+  for (int i = quads * 4 + tid; i < n; i += blockDim.x) {
+    const uint32_t k = take(row[lo + i]);
+    if (RESIDENT) slice[i] = k;
   }
   const int warps = blockDim.x >> 5, lines = (n + 31) / 32;
   Row<RESIDENT> w{p, sh, slice, row, rank, (int)gridDim.y, lo, (int)((long long)(tid >> 5) * lines / warps) * 32,
@@ -709,8 +747,9 @@ FERRUM_API int ferrum_sample_filtered(const float* logits, int ld, int held, int
   if (n_rows == 0) return 0;
   int bits = 0;
   while (bits < 31 && (1ll << bits) < V) ++bits;
-  // A few rows: clusters of 16 CTAs of 1,024 threads, so that the whole GPU reads them; more: 8 CTAs of 512.  Small vocabularies: one CTA.
-  const int sms = ferrum_sm_count(), ctas = V < 16384 ? 1 : n_rows * MAX_CLUSTER <= sms && V >= 65536 ? MAX_CLUSTER : 8;
+  // Small vocabularies: one CTA a row.  Else 8, of 1,024 threads while every CTA has an SM to itself (8 rows of 128,256 logits, top-k: 25 us, in clusters of 16 37), then of 512.
+  // 16 for up to four rows: more clusters of 16 do not find room at a time.
+  const int sms = ferrum_sm_count(), ctas = V < 16384 ? 1 : n_rows <= 4 && V >= 65536 ? MAX_CLUSTER : 8;
   const int threads = n_rows * ctas <= sms && V >= 8192 ? 1024 : 512;
   FilterParams p{logits, rows, temperature, top_k, top_p, min_p, uniform, out_ids, also_to, err_flag, ld, V, (V + ctas - 1) / ctas, bits > 17 ? 62 - bits : 45, held};
   if (p.per <= MOST_RESIDENT) return launch_sample<true>(p, n_rows, ctas, threads, stream);
