@@ -122,6 +122,10 @@ __device__ __forceinline__ Span span_of(const PackedParams& p, int r) {
   const int n = p.q_start[r + 1] - p.q_start[r], rows = n * p.G;
   if (rows <= 0 || rows > PACKED_FEW_ROWS) return Span{0, 0, 0};
   const int pos = p.pos0[r];
+  if (pos < 0 || pos > (long long)p.table_width * p.page_size - n) {      // keys that no page of the table could hold
+    atomicExch(p.err, 5);
+    return Span{0, 0, 0};
+  }
   const int lo = (p.window > 0 ? max(0, pos - p.window + 1) : 0) / PACKED_POS * PACKED_POS;
   return Span{lo, (pos + n - lo + TILE - 1) / TILE, (rows + 8 * NT - 1) / (8 * NT)};
 }
@@ -435,7 +439,24 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, const Item it
       }
     if (__any_sync(0xffffffffu, most > most_allowed)) {
       const unsigned top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
-      const int e = min(127, (int)(top >> 23) - 126);              // top < 2^e
+      // top < 2^e; no further down than float32 holds 2^-e with HEAD; a product beyond float32: a weight of 2^SLACK takes it there
+      int e = top < 0x7f800000u ? max(-100, (int)(top >> 23) - 126) : 132;
+      const int was = 127 + HEAD - (int)(__float_as_uint(v_up) >> 23);
+      if (e < was - 40) {            // much smaller products than before: what the sums hold still needs its room
+        float held = 0.f;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int g = 0; g < GN; ++g)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              held = fmaxf(held, fabsf(eights[nt][g][c]));
+#pragma unroll
+              for (int j = 0; j < 4; ++j) held = fmaxf(held, fabsf(o[nt][g][j][c]));
+            }
+        const int held_e = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(held)) >> 23) - 126;      // held < 2^held_e, at most 2^80 afterwards
+        e = max(e, max(was - 126, min(was, was + held_e - 80)));
+      }
       const float up = __uint_as_float((unsigned)(127 + HEAD - e) << 23), ratio = up / v_up;
       most_allowed = __uint_as_float(min((unsigned)(127 + e + 15 - HEAD), 254u) << 23);
       v_up = up;

@@ -885,6 +885,8 @@ def attention_packed(q, out, n_tokens, block_table, q_start, pos0, plane, page_s
     n_reqs, (held, width) = pos0.shape[0], block_table.shape
     if q_start.shape[0] != n_reqs + 1 or held < n_reqs or min(q.shape[0], out.shape[0]) < n_tokens:
         raise KernelError("attention_packed: q_start, pos0, block_table and the rows do not agree")
+    if q_at == out_at:
+        raise KernelError("attention_packed: out must not be q, whose rows several CTAs read")
     _check(lib().ferrum_attention_packed(q_at, ldq, out_at, ldo, dt, plane_at, page_stride, n_pages, page_size, table_at, width, start_at, pos_at, n_reqs,
                                          n_tokens, part_at, part.shape[0], counters_at, counters.shape[0], Hq, Hkv, D, float(scale), window, _at(err),
                                          _stream_at()), "attention_packed")
@@ -917,7 +919,7 @@ def sample_filtered(logits, n_rows, out_ids, err, temperature, top_k, top_p, min
     top_p of their mass before them; of these, those with at least min_p times the largest one's probability.  The draw is the first
     of them in index order at which their running mass exceeds uniform times their whole mass.  NaN logits are never drawn.  A row of NaN
     raises error 6, a temperature, top_p or min_p out of range error 7 (id -1 each), as does a row that the logits or the ids do not
-    have (left out).  `also_to` (int32) receives the ids as well."""
+    have (left out).  A row named twice gets the draw of one of its two.  `also_to` (int32) receives the ids as well."""
     at, ld = _rows(logits, torch.float32, "logits")
     _need(err, torch.int32, "err")
     t_at, u_at = _dense(temperature, torch.float32, "temperature", 1), _dense(uniform, torch.float64, "uniform", 1)

@@ -228,6 +228,55 @@ def test_a_value_far_larger_than_the_others(cuda, dtype, seen):
     s.check(s.attend(), seen)
 
 
+@pytest.mark.parametrize("small", [1e-20, 1e-31, 1e-34])
+@pytest.mark.parametrize("kind", ["all", "the best keys'", "the best keys', of large ones"])
+def test_values_near_the_smallest(cuda, kind, small):
+    """bfloat16 values down to the smallest normal steps: all of them, or those of the last 500 keys, whose scores are ten above the others' (so that the
+    others' values make the result all the same).  Compared after a factor that makes the result about one."""
+    c = H.Cache([2100], 1, 128, 16, torch.bfloat16, 43, spread=0.3, offset=0.0)
+    s = H.Step(c, [1], 4, 44)
+    q = s.qkv[0, :128].float()
+    s.qkv[:, :512] = s.qkv[:, :128].repeat(1, 4)
+    kv = torch.stack([c.keys[0].float(), c.vals[0].float()])
+    kv[0, 0, -500:] += 10 / (s.mixer.scale * q.square().sum()) * q
+    large = 1e15 if kind.endswith("large ones") else 1.0
+    kv[1, 0, :1600] *= small if kind == "all" else large
+    kv[1, 0, 1600:] *= small
+    codes, step, mid = H.quantise(kv, torch.bfloat16)
+    assert bool((step[1].float() >= torch.finfo(torch.bfloat16).smallest_normal).all())
+    pad = lambda t: torch.cat([t, torch.zeros(2, 1, 12, t.shape[-1], dtype=t.dtype, device="cuda")], 2).unflatten(2, (132, 1, 16)).transpose(1, 2)
+    c.plane[c.table[0].long()] = H.block_bytes(*[[pad(t)[i] for t in (codes, step, mid)] for i in (0, 1)], torch.bfloat16)
+    up = 1 / small if kind == "all" else 1e5 / large
+    vals = H.values(codes, step, mid)
+    want, bound = H.attention(s.qkv[:1, :512].view(1, 4, 128), vals[0], vals[1] * up, mid[1].double().repeat_interleave(64, -1) * up, 2099, s.mixer.scale, 0, torch.bfloat16)
+    got = s.attend().view(1, 4, 128).double() * up
+    assert bool(((got - want).abs() <= bound).all()), ((got - want).abs() / bound).max().item()
+
+
+@pytest.mark.parametrize("where", [-1, -1000, 16 * 13 - 1, 10 ** 6, 2 ** 31 - 1])
+@pytest.mark.parametrize("n_reqs", [2, 40])
+def test_positions_beyond_the_table_raise_the_flag(cuda, where, n_reqs):
+    """A request whose keys no page of the table could hold raises error 5; the other requests' rows stay right."""
+    c = H.Cache([100, 200] + [30] * (n_reqs - 2), 2, 128, 16, torch.float16, 4)
+    assert c.width == 13
+    s = H.Step(c, [1, 2] + [1] * (n_reqs - 2), 8, 5)
+    s.ctx.pos0[1] = where
+    out = s.attend()
+    assert s.ctx.err.item() == 5
+    keep = [0] + list(range(3, n_reqs + 1))
+    s.new[1], s.qkv = 0, s.qkv[keep]
+    s.check(out[keep])
+
+
+def test_out_in_the_place_of_q_is_refused(cuda):
+    from ferrum_b200.ops import lib as ops
+    c = H.Cache([100], 2, 64, 16, torch.bfloat16, 8)
+    s = H.Step(c, [1], 8, 9)
+    part, counters = torch.empty(ops.attention_packed_workspace(64), device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda")
+    with pytest.raises(ops.KernelError, match="out must not be q"):
+        ops.attention_packed(s.qkv, s.qkv, 1, s.ctx.block_tables[0], s.ctx.q_start, s.ctx.pos0, c.plane, c.plane.stride(0), 16, 8, 2, 64, 0.125, 0, s.ctx.err, part, counters)
+
+
 @pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-4, 3.0])
 def test_score_scales(cuda, scale):
     for new in ([1, 1], [3, 2], [40, 1]):
