@@ -54,7 +54,7 @@ struct PackedParams {
   int* counters;        // [requests * Hkv * 2], zeros before and after: the parts of a (request, head, row tile) that are there
   int* err;
   long long page_stride;
-  int ldq, ldo, n_pages, page_size, table_width, Hq, Hkv, G, window, n_reqs;
+  int ldq, ldo, n_pages, page_size, table_width, table_keys, Hq, Hkv, G, window, n_reqs;
   float scale_log2;
 };
 
@@ -115,17 +115,14 @@ constexpr int MAX_RESIDENT = 4;
 
 // A request's part of the line.
 struct Span {
-  int lo, tiles, row_tiles;      // first key (a block's first), tiles of TILE keys, tiles of rows; none of either: not a request of few rows
+  int lo, tiles, row_tiles;      // first key (a block's first), tiles of TILE keys (none: not a request of few rows, or a bad one, which has rows), tiles of rows
 };
 template <int NT>
 __device__ __forceinline__ Span span_of(const PackedParams& p, int r) {
   const int n = p.q_start[r + 1] - p.q_start[r], rows = n * p.G;
   if (rows <= 0 || rows > PACKED_FEW_ROWS) return Span{0, 0, 0};
   const int pos = p.pos0[r];
-  if (pos < 0 || pos > (long long)p.table_width * p.page_size - n) {      // keys that no page of the table could hold
-    atomicExch(p.err, 5);
-    return Span{0, 0, 0};
-  }
+  if ((unsigned)pos > (unsigned)(p.table_keys - n)) return Span{0, 0, rows};      // keys that no page of the table could hold (n <= 16 <= table_keys)
   const int lo = (p.window > 0 ? max(0, pos - p.window + 1) : 0) / PACKED_POS * PACKED_POS;
   return Span{lo, (pos + n - lo + TILE - 1) / TILE, (rows + 8 * NT - 1) / (8 * NT)};
 }
@@ -205,7 +202,7 @@ struct Flow {
 
 // One item, whose first copies are on their way; next() sends the next item's.
 template <typename T, int D, int NT, typename Next>
-__device__ __forceinline__ void packed_item(const PackedParams& p, const Item it, Flow<D>& flow, uint8_t* ring, uint32_t bars, uint32_t& turn, float* merge,
+__device__ __forceinline__ void packed_item(const PackedParams& p, const Item it, Flow<D>& flow, uint8_t* ring, uint32_t bars, uint32_t& turn, float* merge, volatile int* far_e,
                                             bool& failed, Next next) {
   using B = PackedBlock<D>;
   constexpr int GN = B::GROUPS;
@@ -291,6 +288,7 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, const Item it
         for (int j = 0; j < 4; ++j) o[nt][g][j][c] = o[nt][g][j][2 + c] = 0.f;
       }
     }
+  *far_e = -100;                       // the largest e of the part, below
   float most_allowed = 0x1p-100f, v_up = __uint_as_float((unsigned)(127 + 100 + 15) << 23);      // p step is at most most_allowed = 2^15 / v_up
 
   // (m_run: the maximum in use, a score times f_row.)
@@ -441,22 +439,8 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, const Item it
       const unsigned top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
       // top < 2^e; no further down than float32 holds 2^-e with HEAD; a product beyond float32: a weight of 2^SLACK takes it there
       int e = top < 0x7f800000u ? max(-100, (int)(top >> 23) - 126) : 132;
-      const int was = 127 + HEAD - (int)(__float_as_uint(v_up) >> 23);
-      if (e < was - 40) {            // much smaller products than before: what the sums hold still needs its room
-        float held = 0.f;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int g = 0; g < GN; ++g)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              held = fmaxf(held, fabsf(eights[nt][g][c]));
-#pragma unroll
-              for (int j = 0; j < 4; ++j) held = fmaxf(held, fabsf(o[nt][g][j][c]));
-            }
-        const int held_e = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(held)) >> 23) - 126;      // held < 2^held_e, at most 2^80 afterwards
-        e = max(e, max(was - 126, min(was, was + held_e - 80)));
-      }
+      e = max(e, *far_e - 60);       // (the sums so far keep their room: products 2^60 below the largest one that the part has met lose bits)
+      *far_e = max(e, *far_e);       // (every lane writes the same)
       const float up = __uint_as_float((unsigned)(127 + HEAD - e) << 23), ratio = up / v_up;
       most_allowed = __uint_as_float(min((unsigned)(127 + e + 15 - HEAD), 254u) << 23);
       v_up = up;
@@ -703,7 +687,7 @@ attention_packed_kernel(const PackedParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) unsigned long long bars_mem[WARPS * HALVES];
   __shared__ long long s_scan[WARPS];
-  __shared__ int s_req, s_begin;
+  __shared__ int s_req, s_begin, s_far[WARPS];
   __shared__ Way way;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint8_t* ring = smem + warp * HALVES * NB * B::BYTES;
@@ -720,7 +704,10 @@ attention_packed_kernel(const PackedParams p) {
   auto ctas_of = [&](const Span sp) { return sp.tiles ? (int)min((long long)sp.tiles, 1 + (long long)sp.tiles * max(0ll, way.P - way.N) / way.U) : 0; };
   auto pairs_of = [&](const Span sp) { return sp.row_tiles * p.Hkv; };
   // units in the low 40 bits, pairs above
-  auto load_of = [&](const Span sp) { return sp.tiles ? (long long)sp.tiles * pairs_of(sp) + ((long long)pairs_of(sp) << 40) : 0ll; };
+  auto load_of = [&](const Span sp) {
+    if (sp.tiles == 0 && sp.row_tiles) atomicExch(p.err, 5);
+    return sp.tiles ? (long long)sp.tiles * pairs_of(sp) + ((long long)pairs_of(sp) << 40) : 0ll;
+  };
   auto length_of = [&](const Span sp) { return way.own ? ctas_of(sp) : sp.tiles ? sp.tiles + EXTRA : 0; };
   auto line_of = [&](const Span sp) { return (long long)length_of(sp) * pairs_of(sp); };
   auto decide = [&](long long load) {      // the same in every thread
@@ -833,7 +820,7 @@ attention_packed_kernel(const PackedParams p) {
   bool more = next_item(it);
   if (more) flow.begin(p, it, turn, ring, bars);
   while (more) {
-    packed_item<T, D, NT>(p, it, flow, ring, bars, turn, merge, failed, [&]() {
+    packed_item<T, D, NT>(p, it, flow, ring, bars, turn, merge, s_far + warp, failed, [&]() {
       more = next_item(following);
       if (more) flow.begin(p, following, turn, ring, bars);
     });
@@ -887,7 +874,8 @@ FERRUM_API int ferrum_attention_packed(const void* q, int ldq, void* out, int ld
   const int G = Hq / Hkv;
   float* part_ml = part + (size_t)most_ctas() * 2 * PART_ROWS * D;
   PackedParams p{q, out, (const uint8_t*)plane, block_table, q_start, pos0, part, part_ml, counters,
-                 err_flag, page_stride, ldq, ldo, n_pages, page_size, table_width, Hq, Hkv, G, window, n_reqs, scale * 1.4426950408889634f};
+                 err_flag, page_stride, ldq, ldo, n_pages, page_size, table_width, (int)std::min<long long>((long long)table_width * page_size, 0x7fffff00), Hq, Hkv, G, window,
+                 n_reqs, scale * 1.4426950408889634f};
   // One row tile of 8 where every request brings a token of at most 8 rows (a longer one takes two passes over its keys), else 16 rows
   // in one pass.
   const bool narrow = G <= 8 && n_tokens <= n_reqs;
