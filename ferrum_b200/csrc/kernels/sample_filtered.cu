@@ -15,6 +15,10 @@
 // above it is listed on the way, in index order, and all that follows reads the lists (where a warp's share outgrows its list,
 // the slice again).  Where the first histogram leaves no more than 1,024 tokens, the usual case, one CTA sorts those and does the rest alone.  Of equal keys at the cut the first in index order stay: a threshold is a key and an index.
 //
+// What bounds it is neither bytes (64 rows of 128,256 logits are read once: 5 us at 6.5 TB/s) nor arithmetic but the chain of passes over shared memory and
+// of cluster barriers between them, and for many rows that their clusters do not all find room at a time.  B200, 128,256 logits, in a CUDA graph: one row
+// with top-k 50 19.5 us, with top-p alone 29, unfiltered 11; 8 rows with top-k 23; 64 rows with top-k 59, unfiltered 52, each with filters of its own 83 (0.4 TB/s).
+//
 // The reference samples greedily only (crates/core-types/src/model.rs:44-62).
 #include "common.cuh"
 
@@ -24,10 +28,11 @@ typedef unsigned long long u64;
 
 constexpr int BINS = 2048;
 constexpr int MAX_CLUSTER = 16;
-constexpr int MAX_WARPS = 32;
+constexpr int THREADS = 512;         // two CTAs an SM
+constexpr int WARPS = THREADS / 32;
 constexpr int SEGMENTS = 2;         // parts of a warp's run whose masses are kept for the draw
 constexpr int LIST = 1024;          // listed tokens of a CTA, LIST / warps of a warp
-constexpr int MOST_BINS = 4;        // bins of a thread's share: BINS / 512
+constexpr int MOST_BINS = BINS / THREADS;      // bins of a thread's share
 constexpr int FEW = 1024;           // tokens that one CTA sorts
 
 // Order-preserving integer of a logit; 0 stands for NaN, which comes after everything and is never kept.
@@ -84,8 +89,8 @@ struct Shared {
   };
   unsigned few;                     // how many there are
   u64 exchange[4][2][MAX_CLUSTER];
-  u64 warp[MAX_WARPS][2];
-  u64 segment[MAX_WARPS][SEGMENTS];
+  u64 warp[32][2];
+  u64 segment[WARPS][SEGMENTS];
   u64 found[2];
   uint32_t list_key[LIST];
   int list_index[LIST];
@@ -138,7 +143,7 @@ struct Row {
   template <bool MASS, typename Wanted, typename Bin>
   __device__ __forceinline__ void fill_histogram(Wanted wanted, Bin bin_of) {
     const int lane = threadIdx.x & 31;
-    for (int i = threadIdx.x; i < BINS; i += blockDim.x) sh.hist[i] = 0;
+    for (int i = threadIdx.x; i < BINS; i += THREADS) sh.hist[i] = 0;
     __syncthreads();
     constexpr int AT_ONCE = 4;
     for (int e = e0 + lane; e - lane < e1; e += 32 * AT_ONCE) {
@@ -188,8 +193,8 @@ struct Row {
     __syncthreads();
     u64(&ex)[2][MAX_CLUSTER] = sh.exchange[turn++ & 3];
     if (warp == 0) {
-      a = lane < (int)(blockDim.x >> 5) ? sh.warp[lane][0] : 0;
-      b = lane < (int)(blockDim.x >> 5) ? sh.warp[lane][1] : 0;
+      a = lane < WARPS ? sh.warp[lane][0] : 0;
+      b = lane < WARPS ? sh.warp[lane][1] : 0;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
         const u64 x = __shfl_xor_sync(0xffffffffu, a, o), y = __shfl_xor_sync(0xffffffffu, b, o);
@@ -222,7 +227,7 @@ struct Row {
   __device__ __forceinline__ void run_sums(int size) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, chunks = size / 32;
     __syncthreads();
-    for (int w = warp; w < chunks; w += blockDim.x >> 5) {
+    for (int w = warp; w < chunks; w += WARPS) {
       u64 v = sh.mass[w * 32 + lane];
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -243,7 +248,7 @@ struct Row {
       sh.warp[lane][0] = v - own;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < size; i += blockDim.x) sh.mass[i] += sh.warp[i >> 5][0];
+    for (int i = threadIdx.x; i < size; i += THREADS) sh.mass[i] += sh.warp[i >> 5][0];
     __syncthreads();
   }
   // order[0 .. size - 1], the largest first.
@@ -251,7 +256,7 @@ struct Row {
     for (int k = 2; k <= size; k <<= 1)
       for (int j = k >> 1; j > 0; j >>= 1) {
         __syncthreads();
-        for (int t = threadIdx.x; t < size / 2; t += blockDim.x) {
+        for (int t = threadIdx.x; t < size / 2; t += THREADS) {
           const int i = 2 * t - (t & (j - 1));      // the lower of the pair (i, i + j)
           const u64 a = sh.order[i], b = sh.order[i + j];
           if ((a < b) == ((i & k) == 0)) sh.order[i] = b, sh.order[i + j] = a;
@@ -318,37 +323,37 @@ struct Row {
     if (rank != 0) return true;
     int size = 32;
     while (size < (int)n) size <<= 1;
-    for (int i = tid; i < size; i += blockDim.x)
+    for (int i = tid; i < size; i += THREADS)
       if (i >= (int)n) sh.order[i] = 0;
     sort_down(size);
     auto weigh = [&](int i) { return i < (int)n ? scaled_weight((uint32_t)(sh.order[i] >> 32)) : 0.0; };
-    for (int i = tid; i < size; i += blockDim.x) sh.mass[i] = whole(weigh(i));
+    for (int i = tid; i < size; i += THREADS) sh.mass[i] = whole(weigh(i));
     run_sums(size);
     const int n_k = BY_MASS ? (int)n : min((int)n, top_k);
     const double part = BY_MASS ? limit : top_p < 1.f ? (double)top_p * (double)sh.mass[n_k - 1] : INFINITY;
     // what stays are the first so many
     int stays = 0;
-    for (int i = tid; i < n_k; i += blockDim.x)
+    for (int i = tid; i < n_k; i += THREADS)
       if ((i == 0 || (double)sh.mass[i - 1] < part) && weigh(i) >= min_w) stays = i + 1;
     stays = __reduce_max_sync(0xffffffffu, stays);
     __syncthreads();
     if (lane == 0) sh.warp[warp][1] = stays;
     __syncthreads();
-    for (int w = 0; w < (int)(blockDim.x >> 5); ++w) stays = max(stays, (int)sh.warp[w][1]);
+    for (int w = 0; w < WARPS; ++w) stays = max(stays, (int)sh.warp[w][1]);
     const u64 sum = sh.mass[stays - 1];
     const double x = u > 0.0 ? u * (double)sum : 0.0;
     const u64 threshold = x >= (double)sum ? sum - 1 : min((u64)x, sum - 1);
     // in index order: (~index, key) from the largest down
     size = 32;
     while (size < stays) size <<= 1;
-    for (int i = tid; i < size; i += blockDim.x) {
+    for (int i = tid; i < size; i += THREADS) {
       const u64 v = sh.order[i];
       sh.order[i] = i < stays ? v << 32 | v >> 32 : 0;
     }
     sort_down(size);
-    for (int i = tid; i < size; i += blockDim.x) sh.mass[i] = i < stays ? mass((uint32_t)sh.order[i]) : 0;
+    for (int i = tid; i < size; i += THREADS) sh.mass[i] = i < stays ? mass((uint32_t)sh.order[i]) : 0;
     run_sums(size);
-    for (int i = tid; i < stays; i += blockDim.x)
+    for (int i = tid; i < stays; i += THREADS)
       if (threshold < sh.mass[i] && (i == 0 || threshold >= sh.mass[i - 1])) {
         const int id = (int)~(uint32_t)(sh.order[i] >> 32);
         p.out_ids[out] = id;
@@ -361,7 +366,7 @@ struct Row {
   // bins before them (at) and in all (all).  All threads of the cluster call it behind the barrier that ends the counting.
   __device__ __forceinline__ void bins_of_cluster(u64 (&mine)[MOST_BINS], u64& own, u64& all, u64& at, int& b0, int& each) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, share = BINS / n_ctas;
-    each = max(1, share / (int)blockDim.x);
+    each = max(1, share / THREADS);
     b0 = rank * share + tid * each;
     const bool has = tid * each < share;
     u64 run = 0;
@@ -446,7 +451,7 @@ struct Row {
       }
       // the range of the keys in that bin, for the next histogram; and the lists of what lies in it or above
       uint32_t a = 0, b = 0;        // maximum of ~key and of key
-      const int most = LIST / (int)(blockDim.x >> 5);
+      const int most = LIST / WARPS;
       int count = 0;
 #pragma unroll 4
       for (int e = e0 + lane; e - lane < e1; e += 32) {
@@ -617,7 +622,7 @@ struct Row {
 };
 
 template <bool RESIDENT>
-__global__ void __launch_bounds__(32 * MAX_WARPS)
+__global__ void __launch_bounds__(THREADS, 2)
 sample_filtered_kernel(const FilterParams p) {
   extern __shared__ __align__(16) uint32_t slice[];
   __shared__ Shared sh;
@@ -657,19 +662,19 @@ sample_filtered_kernel(const FilterParams p) {
   };
   const int quads = ((uintptr_t)(row + lo) & 15) == 0 ? n / 4 : 0;
 #pragma unroll 4
-  for (int i = tid; i < quads; i += blockDim.x) {
+  for (int i = tid; i < quads; i += THREADS) {
     const float4 x = reinterpret_cast<const float4*>(row + lo)[i];
     const uint4 k = make_uint4(take(x.x), take(x.y), take(x.z), take(x.w));
     if (RESIDENT) reinterpret_cast<uint4*>(slice)[i] = k;
   }
 #pragma unroll 8
-  for (int i = quads * 4 + tid; i < n; i += blockDim.x) {
+  for (int i = quads * 4 + tid; i < n; i += THREADS) {
     const uint32_t k = take(row[lo + i]);
     if (RESIDENT) slice[i] = k;
   }
-  const int warps = blockDim.x >> 5, lines = (n + 31) / 32;
-  Row<RESIDENT> w{p, sh, slice, row, rank, (int)gridDim.y, lo, (int)((long long)(tid >> 5) * lines / warps) * 32,
-                  min(n, (int)((long long)((tid >> 5) + 1) * lines / warps) * 32), false, 0, 0, 0.f, 0.0};
+  const int lines = (n + 31) / 32;
+  Row<RESIDENT> w{p, sh, slice, row, rank, (int)gridDim.y, lo, (int)((long long)(tid >> 5) * lines / WARPS) * 32,
+                  min(n, (int)((long long)((tid >> 5) + 1) * lines / WARPS) * 32), false, 0, 0, 0.f, 0.0};
   const u64(&ex)[2][MAX_CLUSTER] = w.template gather<true>(most, (uint32_t)~least_finite);
   for (int c = 0; c < w.n_ctas; ++c) {
     w.best = max(w.best, (uint32_t)ex[0][c]);
@@ -704,7 +709,7 @@ sample_filtered_kernel(const FilterParams p) {
 }
 
 template <bool RESIDENT>
-int launch_sample(const FilterParams& p, int n_rows, int ctas, int threads, cudaStream_t stream) {
+int launch_sample(const FilterParams& p, int n_rows, int ctas, cudaStream_t stream) {
   const int smem = RESIDENT ? p.per * 4 : 0;
   static int reserved = 0;
   if (smem > reserved || reserved == 0) {
@@ -715,7 +720,7 @@ int launch_sample(const FilterParams& p, int n_rows, int ctas, int threads, cuda
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(n_rows, ctas);
-  cfg.blockDim = dim3(threads);
+  cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -736,6 +741,20 @@ int launch_sample(const FilterParams& p, int n_rows, int ctas, int threads, cuda
 // The most logits that a CTA keeps in its shared memory; a row of more than MAX_CLUSTER times that is read from global memory every time.
 constexpr int MOST_RESIDENT = 45 * 1024;
 
+// CTAs of a row.  What does not find room waits for a whole row: an SM holds two CTAs whose slices are of up to 16,384 logits or so, and clusters of 16 go
+// onto few SMs at a time.  B200, top-k 50 and top-p 0.9, us with 1 / 4 / 8 / 16 CTAs (-: not measured):
+//   8,192 logits, 8 rows 18 / - / 19 / -, 64 rows 18 / - / 34 / -
+//   16,384: 8 rows 23 / - / 15 / 19, 32 rows 22 / 17 / 23 / -, 64 rows 23 / 20 / 36 / -
+//   65,536: 4 rows - / - / 18.0 / 17.4, 8 rows - / - / 18 / 21, 16 rows - / 23 / 21 / 30, 32 rows - / 25 / 28 / -, 64 rows - / 29 / 46 / -
+//   128,256: 4 rows - / - / 23 / 20, 8 rows - / - / 23 / 24, 16 rows - / 32 / 28 / 35, 64 rows - / 63 / 60 / -; top-p alone at a temperature of 1.3,
+//   where the bins above the cut hold too many to list, 1 row - / - / 59 / 41, 64 rows - / 203 / 163 / -
+// (CTAs of 1,024 threads, one an SM: 1 row of 128,256 23 instead of 20, 16 rows 40 instead of 28.)
+int ctas_of(int n_rows, int V) {
+  if (V < 16384) return 1;
+  if (n_rows <= 4 && V >= 65536) return MAX_CLUSTER;
+  return n_rows > 16 && V <= 65536 ? 4 : 8;
+}
+
 }  // namespace
 
 // held: rows of the logits, of out_ids and of also_to; a row named in `rows` beyond them is left out and raises error 7.
@@ -747,11 +766,8 @@ FERRUM_API int ferrum_sample_filtered(const float* logits, int ld, int held, int
   if (n_rows == 0) return 0;
   int bits = 0;
   while (bits < 31 && (1ll << bits) < V) ++bits;
-  // Small vocabularies: one CTA a row.  Else 8, of 1,024 threads while every CTA has an SM to itself (8 rows of 128,256 logits, top-k: 25 us, in clusters of 16 37), then of 512.
-  // 16 for up to four rows: more clusters of 16 do not find room at a time.
-  const int sms = ferrum_sm_count(), ctas = V < 16384 ? 1 : n_rows <= 4 && V >= 65536 ? MAX_CLUSTER : 8;
-  const int threads = n_rows * ctas <= sms && V >= 8192 ? 1024 : 512;
+  const int ctas = ctas_of(n_rows, V);
   FilterParams p{logits, rows, temperature, top_k, top_p, min_p, uniform, out_ids, also_to, err_flag, ld, V, (V + ctas - 1) / ctas, bits > 17 ? 62 - bits : 45, held};
-  if (p.per <= MOST_RESIDENT) return launch_sample<true>(p, n_rows, ctas, threads, stream);
-  return launch_sample<false>(p, n_rows, ctas, threads, stream);
+  if (p.per <= MOST_RESIDENT) return launch_sample<true>(p, n_rows, ctas, stream);
+  return launch_sample<false>(p, n_rows, ctas, stream);
 }
