@@ -16,12 +16,21 @@
 // step of 2^-12, and the result's own.  All sums are float32.
 //
 // The work is handed out on the device, so that the launch does not depend on the lengths and a captured one serves any.  A (request, KV head,
-// rows of 8 NT) is a pair.  Few pairs (at most half the CTAs): each gets a number of CTAs of its own by its length, one part a CTA, as a
-// part costs some 4 us beside its keys.  Many: they form one line, a pair as long as its units of 64 keys and EXTRA for that cost, and CTA c of
-// P takes the stretch [c L / P, (c + 1) L / P); pairs of up to WHOLE units (and of no more than a stretch) are not cut but belong to the CTA in whose
-// stretch they begin.
+// rows of 8 NT) is a pair.  Few pairs (OWN CTAs or more for each): each gets a number of CTAs of its own by its length, one part a CTA, of NB units at
+// least (a step takes as long with one), as a part costs some 4 us beside its keys.  Many: they form one line, a pair as long as its units of 64 keys and EXTRA for
+// that cost, and CTA c of P takes the stretch [c L / P, (c + 1) L / P); pairs of up to WHOLE units (and of no more than a stretch) are not cut but belong
+// to the CTA in whose stretch they begin.  B200, bfloat16, us (D 128, 8 KV heads, where nothing else is said):
+//   OWN 2 / 3: 17 requests of up to 6,000 keys, 4 tokens each 45 / 41; a line always: the same in a window of 2,000, D 64, 20.4 -> 21.6; parts of one unit: 100 keys 7.1 -> 8.6
+//   EXTRA 0 / 6 / 12: 40 requests of 30 to 900 keys, 32 KV heads 102 / 45.6 / 48, 64 x 8,192 keys 138 / 135 / 135, 40 x 30 to 900 keys 31 / 20 / 19
+//   WHOLE 0 / 16 / 64: 64 x 200 keys 20.8 / 17.9 / 17.9, 40 x 465 keys, 32 KV heads 47 / 36 / 36, 64 x 400 to 2,000 keys 35.8 / 36.1 / 39.6
 // A CTA's four warps take every fourth block of 16 positions; a block is one bulk copy into the warp's own ring of stages, and no
 // warp waits for another until its part is done; the first copies of the next part are on their way by then.  Of the CTAs that share a (request, head) the one that comes last adds up the parts, in a fixed order.
+//
+// Measured (B200, bfloat16, D 128, 32 heads on 8 KV heads, in a CUDA graph): 64 requests of 8,192 keys 135 us, 4.5 TB/s of cache where a copy runs at 6.6; one of
+// 131,000 keys 43 us, 3.5 TB/s; 64 of 200 keys 17.9 us; one of 700 keys 9.3 us.  What bounds the long ones is the chain of instructions from a block's codes to its
+// sums, which the 11 warps that an SM's registers hold do not hide: 54 % of the issue slots and of the ALU, 27 % of the matrix pipe, 52 % of the
+// DRAM are busy, and with the copies alone the same kernel takes 107 us.  Two CTAs an SM take 147 us; longer rings or steps of four blocks, for
+// which the third CTA goes, were no faster.
 #include "packed_cache.cuh"
 #include "ptx_sm100.cuh"
 
@@ -38,6 +47,7 @@ constexpr int HEAD = 12;                     // the largest p step so far is bro
 constexpr int SETTLE = 16;                   // steps after which the sums of codes are centred
 constexpr int HALVES = 2;                    // steps in a warp's ring: one is read while the next arrives
 static_assert(32 % NB == 0, "the blocks of a step lie in one window of 32 blocks, one a lane");
+constexpr int OWN = 3;                       // pairs get CTAs of their own where there are this many CTAs for each
 constexpr int EXTRA = 6;                     // what a part costs beside its keys, in units
 constexpr int WHOLE = 16;                    // units up to which a pair is not cut
 constexpr int PART_ROWS = 16;                // rows of a partial's slot
@@ -701,7 +711,7 @@ attention_packed_kernel(const PackedParams p) {
   pdl_launch();
   // ---- the CTA's first item
   // CTAs that a pair of its own gets: their sum over all pairs is at most N + (P - N)
-  auto ctas_of = [&](const Span sp) { return sp.tiles ? (int)min((long long)sp.tiles, 1 + (long long)sp.tiles * max(0ll, way.P - way.N) / way.U) : 0; };
+  auto ctas_of = [&](const Span sp) { return sp.tiles ? (int)min((long long)(sp.tiles + NB - 1) / NB, 1 + (long long)sp.tiles * max(0ll, way.P - way.N) / way.U) : 0; };
   auto pairs_of = [&](const Span sp) { return sp.row_tiles * p.Hkv; };
   // units in the low 40 bits, pairs above
   auto load_of = [&](const Span sp) {
@@ -712,7 +722,7 @@ attention_packed_kernel(const PackedParams p) {
   auto line_of = [&](const Span sp) { return (long long)length_of(sp) * pairs_of(sp); };
   auto decide = [&](long long load) {      // the same in every thread
     const long long c = blockIdx.x, U = load & ((1ll << 40) - 1), N = load >> 40, L = U + EXTRA * N;
-    const bool own = 2 * N <= gridDim.x;
+    const bool own = OWN * N <= gridDim.x;
     const long long P = min((long long)gridDim.x, own ? U : L);
     if (tid == 0 && U) way = Way{L, U, P, N, own ? c : c * L / P, own ? c + 1 : (c + 1) * L / P, (int)min((long long)WHOLE, L / P), own};
     return U > 0 && (own || c < P);
@@ -877,7 +887,7 @@ FERRUM_API int ferrum_attention_packed(const void* q, int ldq, void* out, int ld
                  err_flag, page_stride, ldq, ldo, n_pages, page_size, table_width, (int)std::min<long long>((long long)table_width * page_size, 0x7fffff00), Hq, Hkv, G, window,
                  n_reqs, scale * 1.4426950408889634f};
   // One row tile of 8 where every request brings a token of at most 8 rows (a longer one takes two passes over its keys), else 16 rows
-  // in one pass.
+  // in one pass.  (64 x 8,192 keys, 4 rows each: 135 us, with 16 rows 202; 700 keys 9.3 and 11.4.)
   const bool narrow = G <= 8 && n_tokens <= n_reqs;
   FERRUM_DISPATCH_16BIT(dtype, T, {
     if (D == 64) return narrow ? launch_packed<T, 64, 1>(p, stream) : launch_packed<T, 64, 2>(p, stream);
