@@ -9,8 +9,8 @@
 // for the largest bfloat16 values it is beyond float32.)
 //
 // Both kernels move bytes: the write reads a token's row and writes 9 D / 8 bytes a KV head (2,048 tokens of 48 head slots of 128 and their cosines, 45 MB: 21 us,
-// 2.2 TB/s; a few tokens take the 4 us of a launch and of one chain of loads, shuffles and divisions); the unpacking writes 3.6 times what it reads (64 pages
-// of 32 positions, 8 KV heads of 128, 10 MB: 5.7 us; 319 of them, 53 MB: 14 us, 3.8 TB/s).
+// 2.2 TB/s; a few tokens take the 4 us of a launch and of one chain of loads, shuffles and divisions); the unpacking writes 3.6 times what it reads (2,048
+// positions, 8 KV heads of 128, 10.7 MB: 5.7 us; 10,208 of them, 53 MB: 14 us, 3.8 TB/s).
 //
 // The reference keeps F32 and F16 caches only (crates/core-types/src/cache.rs); this format is this framework's own.
 #include "packed_cache.cuh"
