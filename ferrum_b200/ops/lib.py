@@ -711,11 +711,11 @@ def attention_flash_supported(dtype, D, page_stride=0):
     return dtype in SIXTEEN_BIT and bool(lib().ferrum_attention_flash_supported(c_int(D), c_int(16)))
 
 
-def attention_work(ctx, Hq, Hkv, D, window, esize):
+def attention_work(ctx, Hq, Hkv, D, window, esize, cached=None):
     """(bytes, flops) of causal attention for the step in `ctx`, for the profile: every visible key
-    and value row once, the queries and outputs; two products per (query, visible key) pair."""
+    and value row once (`cached` bytes an element; None: esize), the queries and outputs; two products per (query, visible key) pair."""
     keys, pairs = visible_keys(ctx, window)
-    return (keys * 2 * Hkv * D * esize + 2 * ctx.n_tokens * Hq * D * esize, 4.0 * pairs * Hq * D)
+    return (keys * 2 * Hkv * D * (esize if cached is None else cached) + 2 * ctx.n_tokens * Hq * D * esize, 4.0 * pairs * Hq * D)
 
 
 def visible_keys(ctx, window):

@@ -125,7 +125,7 @@ class PagedAttention(Mixer):
         if kinds[0]:
             part = ctx.buf("attn_packed_part", (ops.attention_packed_workspace(D),), torch.float32)
             if ops.profiling():      # (a step with prompt portions counts the whole step's work for each kernel)
-                ops.set_work(ops.attention_work(ctx, Hq, Hkv, D, self.window, 9 / 16))
+                ops.set_work(ops.attention_work(ctx, Hq, Hkv, D, self.window, qkv.element_size(), 9 / 16))
             ops.attention_packed(qkv, out, ctx.n_tokens, table, ctx.q_start, ctx.pos0, cache.plane, cache.page_stride, cache.page_size,
                                  Hq, Hkv, D, self.scale, self.window, ctx.err, part, ctx.zeros("attn_packed_counters", 2 * ctx.n_reqs * Hkv))
         if not kinds[1]:
