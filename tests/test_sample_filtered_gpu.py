@@ -84,6 +84,23 @@ def test_launch_shapes(cuda, n, V):
               some(rng.uniform(0, 0.05, n), 0.0), rng.random(n))
 
 
+@pytest.mark.parametrize("V", [9000, 16384, 40000, 70001])
+def test_a_draw_does_not_depend_on_the_rows_beside_it(cuda, V):
+    """Rows drawn alone, a few and all at a time (by clusters of other sizes) get the same ids."""
+    g = torch.Generator(device="cuda").manual_seed(V)
+    rng = np.random.default_rng(V)
+    n = 34
+    x = rows_of("ties", n, V, g)
+    t, u = rng.uniform(0.7, 1.5, n), rng.random(n)
+    k, p, m = rng.choice([0, 1, 40, 3000], n), rng.choice([1.0, 0.9, 0.4], n), rng.choice([0.0, 0.02], n)
+    want, err = sample(x, t, k, p, m, u)
+    assert err == 0
+    for size in (1, 3, 7, 16):
+        for a in range(0, n, 5 * size):
+            part = slice(a, a + size)
+            assert sample(x[part].contiguous(), t[part], k[part], p[part], m[part], u[part])[0] == want[part]
+
+
 @pytest.mark.parametrize("V", [700, 50000])
 def test_edges_of_the_filters(cuda, V):
     """k of 1, V and beyond; p next to 0 and 1; min_p of 1; random numbers 0 and next to 1; a temperature next to 0 and a large one."""
