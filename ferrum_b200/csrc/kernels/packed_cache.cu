@@ -8,8 +8,8 @@
 // float32 one, rounded on its own: the codes of a key follow from the definition alone.  (lo + 8 step is one fused operation: 8 step is exact, but
 // for the largest bfloat16 values it is beyond float32.)
 //
-// Both kernels move bytes: the write reads a token's row and writes 9 D / 8 bytes a KV head (2,048 tokens of 48 head slots of 128 and their cosines, 45 MB: 21 us,
-// 2.2 TB/s; a few tokens take the 4 us of a launch and of one chain of loads, shuffles and divisions); the unpacking writes 3.6 times what it reads (2,048
+// Both kernels move bytes: the write reads a token's row and writes 9 D / 8 bytes a KV head (2,048 tokens of 48 head slots of 128 and their cosines, 45 MB: 21 us
+// from DRAM, 2.2 TB/s, 15 from the L2; a few tokens take the 4 us of a launch and of one chain of loads, shuffles and divisions); the unpacking writes 3.6 times what it reads (2,048
 // positions, 8 KV heads of 128, 10.7 MB: 5.7 us; 10,208 of them, 53 MB: 14 us, 3.8 TB/s).
 //
 // The reference keeps F32 and F16 caches only (crates/core-types/src/cache.rs); this format is this framework's own.
@@ -24,7 +24,8 @@ __device__ __forceinline__ float r16(float v) { return to_f32<T>(from_f32<T>(v))
 // heads, Hkv value heads.  Lane l owns elements l*E .. l*E + E - 1 of a head and keeps their cosines and sines for all of its heads.  WIDE:
 // rows and halves are aligned to E elements, so that a lane reads its own in one piece and has those they are turned with from another lane.
 // Few tokens: a slot a warp, so that a token's heads are written at once.  Many: six, since the cosines and sines are four times a
-// head's bytes (B200, 2,048 tokens of 48 slots of 128: 29 us with one, 21 with six; from two tokens an SM on: with fewer the blocks of six would not fill the SMs).
+// head's bytes (B200, 48 slots of 128, one / six: 2,048 tokens 29 / 21 us; 290 tokens,
+// with the pages brought back, 7.9 / 6.1, 150 tokens 5.7 / 5.8).
 template <typename T, int D, bool WIDE, int SLOTS>
 __global__ void __launch_bounds__(256)
 packed_write_kernel(const T* __restrict__ qkv, int ld, T* __restrict__ q_out, int ldq, const int* __restrict__ positions,
@@ -161,10 +162,16 @@ packed_write_kernel(const T* __restrict__ qkv, int ld, T* __restrict__ q_out, in
     float step = r16<T>(__fsub_rn(__fmul_rn(hi, 1.f / 15.f), __fmul_rn(lo, 1.f / 15.f)));
     float middle = r16<T>(fmaf(8.f, step, lo));
     if (bad & of_group) step = middle = __int_as_float(0x7fc00000);
+    // the quotient by a reciprocal is off by three roundings: it names the same whole number as the quotient itself unless it is next to a half, and
+    // there, or where the reciprocal is no number, the division decides
     unsigned codes = 0;
+    const float inverse = __frcp_rn(step);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const float c = step > 0.f ? fminf(fmaxf(__fadd_rn(rintf(__fdiv_rn(__fsub_rn(x[e], middle), step)), 8.f), 0.f), 15.f) : 8.f;
+      const float d = __fsub_rn(x[e], middle), q = __fmul_rn(d, inverse);
+      float c = rintf(q);
+      if (!(fabsf(q - c) < 0.4999f)) c = rintf(__fdiv_rn(d, step));
+      c = step > 0.f ? fminf(fmaxf(__fadd_rn(c, 8.f), 0.f), 15.f) : 8.f;
       codes |= (unsigned)c << (4 * e);
     }
     uint8_t* block = page_at + (size_t)h * (page_size / PACKED_POS) * B::BYTES;
@@ -249,7 +256,7 @@ FERRUM_API int ferrum_rope_cache_write_packed(const void* qkv, int dtype, int n_
   if (n_tokens == 0) return 0;
   const int slots = Hq + (write_kv ? 2 * Hkv : 0), E = D / 32;
   const bool wide = ld % E == 0 && ldq % E == 0 && (((uintptr_t)qkv | (uintptr_t)q_out) & (2 * E - 1)) == 0 && (pairing == 0 || R / 2 % E == 0);
-  const int a_warp = wide && n_tokens >= 2 * ferrum_sm_count() ? 6 : 1;
+  const int a_warp = wide && 2 * n_tokens >= 3 * ferrum_sm_count() ? 6 : 1;
   const dim3 grid(n_tokens, (slots + 8 * a_warp - 1) / (8 * a_warp));
   FERRUM_CHECK_ARG(grid.y <= 65535, "rope_packed: too many heads");
   auto launch = [&](auto kernel, auto* x, auto* q) {

@@ -82,6 +82,37 @@ def test_write_is_the_definition(cuda, dtype, T, Hq, Hkv, D, page, R, pairing):
     assert torch.equal(plane, before)
 
 
+@pytest.mark.parametrize("T,Hq,Hkv,D,R,pairing", [(221, 6, 3, 128, 128, 1), (223, 6, 3, 128, 128, 1), (700, 30, 5, 64, 32, 0)])
+def test_write_of_many_tokens_is_the_definition(cuda, T, Hq, Hkv, D, R, pairing):
+    """As above on both sides of where a warp starts to take several heads of a token."""
+    for dtype in H.DTYPES:
+        test_write_is_the_definition(cuda, dtype, T, Hq, Hkv, D, 32, R, pairing)
+
+
+@pytest.mark.parametrize("dtype", H.DTYPES)
+@pytest.mark.parametrize("kind", ["halves", "next to halves", "subnormal steps", "all sizes"])
+def test_codes_next_to_halves(cuda, dtype, kind):
+    """Values half way between two levels go to the even one, values next to that to theirs; steps below the smallest normal number and of all sizes."""
+    D, page, T = 128, 16, 800
+    g = torch.Generator(device="cuda").manual_seed(5)
+    v = torch.randint(0, 31, (T, D), device="cuda", generator=g).float()         # range 30: a step of 2, every odd value half way
+    v[:, ::64], v[:, 1::64] = 0.0, 30.0
+    if kind == "next to halves":                                                 # (the type's next number up or down)
+        v = v.to(dtype)
+        v = (v.view(torch.int16) + torch.randint(-1, 2, (T, D), device="cuda", generator=g).to(torch.int16) * (v > 0)).view(dtype).float()
+    elif kind == "subnormal steps":
+        v = v * (2.0 ** -131 if dtype == torch.bfloat16 else 2.0 ** -19)
+    elif kind == "all sizes":
+        e = torch.randint(-100 if dtype == torch.bfloat16 else -12, 100 if dtype == torch.bfloat16 else 12, (T, 1), device="cuda", generator=g)
+        v = torch.randn(T, D, device="cuda", generator=g) * 2.0 ** e
+    x = torch.cat([torch.zeros(T, D, device="cuda"), v, v.flip(0)], 1).to(dtype)
+    table, plane = torch.arange(T // page, dtype=torch.int32, device="cuda")[None], torch.zeros(T // page, 1, 1, 18 * D, dtype=torch.uint8, device="cuda")
+    assert write(x, 1, 1, D, page, list(range(T)), [0] * T, table, None, 0, 0, plane) == 0
+    cut = lambda t: t.unflatten(0, (T // page, 1, 1, 16))
+    want = H.block_bytes(*[[cut(t) for t in H.quantise(x[:, part * D:(part + 1) * D].float(), dtype)] for part in (1, 2)], dtype)
+    assert torch.equal(plane, want)
+
+
 @pytest.mark.parametrize("dtype", H.DTYPES)
 def test_write_of_special_values(cuda, dtype):
     """Constant groups come back exactly, as does a group of zeros; a NaN or an infinity spoils its own group alone; the type's largest
