@@ -44,7 +44,11 @@ class Filters:
     min_p: float = 0.0
 
     def __post_init__(self):
-        if isinstance(self.top_k, bool) or int(self.top_k) != self.top_k or not 0 <= self.top_k < 1 << 31:
+        try:
+            whole = not isinstance(self.top_k, bool) and int(self.top_k) == self.top_k
+        except (TypeError, ValueError, OverflowError):      # (what is no number, a NaN, an infinity)
+            whole = False
+        if not whole or not 0 <= self.top_k < 1 << 31:
             raise InvalidRequest("top_k must be a whole number, 0 (off) or more")
         # what the kernel gets are float32 numbers: one below 2^-149 would be 0 there
         if not 0 < float(np.float32(self.top_p)) <= 1:

@@ -18,6 +18,13 @@ def test_filters_out_of_range(kw, name):
         Filters(**kw)
 
 
+@pytest.mark.parametrize("top_k", [math.inf, -math.inf, math.nan, None, "a"])
+def test_top_k_that_is_no_whole_number(top_k):
+    from ferrum_b200.sampling import Filters
+    with pytest.raises(InvalidRequest, match="top_k"):
+        Filters(top_k=top_k)
+
+
 def test_filters_on():
     from ferrum_b200.sampling import Filters
     assert not Filters().on and Filters(3).on and Filters(0, 0.5).on and Filters(0, 1.0, 0.1).on
