@@ -190,6 +190,9 @@ template <> __device__ __forceinline__ float largest<__half>() { return 65504.f;
 
 // One block per (item, KV head); a thread brings eight elements back at a time: a word of codes in, 16 bytes out, both of its rows of a block of
 // 16 positions (and of keys and values) on their way together.
+// middle + (code - 8) step is rounded to the 16-bit type, since that is what the kernels of prompt portions read: an output's error against 64 bits
+// becomes that of a 16-bit cache, 0.003 to 0.004 in bfloat16 and 0.0004 in float16 (0.0017 and 0.0002 for rounding the result alone).
+// 32-bit pages would want kernels of their own and twice the bytes written.
 template <typename T, int D>
 __global__ void __launch_bounds__(256)
 unpack_kernel(const uint8_t* __restrict__ plane, long long page_stride, int n_pages, int page_size, const int* __restrict__ block_table,
