@@ -227,6 +227,7 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, const Item it
   // ---- the rows' queries as float16 operands, their sums per group and their scale
   unsigned qf[NT][GN][4][2];
   float q_sum[NT][GN][2], f_row[NT][2];
+  int e_row[NT], e_least = 126;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int row = row0 + nt * 8 + gid;
@@ -249,8 +250,11 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, const Item it
     }
     big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
     big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-    // 2^e brings the largest element to [2^14, 2^15); a row of zeros (or of subnormals) keeps e within a float's exponents
-    const int e = max(-100, min(100, 14 + 127 - (int)(__float_as_uint(big) >> 23)));
+    // 2^e brings the largest element to [2^14, 2^15); bfloat16's largest numbers to 65,280 at most, which a float16 still holds; its smallest to
+    // what a float's exponents allow
+    const int e = max(-112, min(126, 14 + 127 - (int)(__float_as_uint(big) >> 23)));
+    e_least = min(e_least, e);
+    e_row[nt] = e;
     const float up = copysignf(__uint_as_float((unsigned)(127 + e) << 23), p.scale_log2);      // (f_row is not negative: it orders the scores)
     float sum[GN];
 #pragma unroll
@@ -272,14 +276,21 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, const Item it
         }
     }
     // the scores' columns: this thread meets rows 2 tig and 2 tig + 1
-    const float f = fabsf(p.scale_log2) * __uint_as_float((unsigned)(127 - e) << 23) * 16777216.f;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int from = (2 * tig + c) * 4;
-      f_row[nt][c] = __shfl_sync(0xffffffffu, f, from);
+    for (int c = 0; c < 2; ++c)
 #pragma unroll
-      for (int g = 0; g < GN; ++g) q_sum[nt][g][c] = __shfl_sync(0xffffffffu, sum[g], from) * 0x1p-24f;
-    }
+      for (int g = 0; g < GN; ++g) q_sum[nt][g][c] = __shfl_sync(0xffffffffu, sum[g], (2 * tig + c) * 4) * 0x1p-24f;
+  }
+  // A score is f_row, 2^24 scale 2^-e, times a sum that the keys' steps and middles make.  Under queries of 2^90 and more the one would leave float32 and the other
+  // its normal numbers: 2^shift moves from the factor to the keys then (whose own elements are far below 2^90 where the scores are to be finite).
+  constexpr bool WIDE_Q = std::is_same<T, __nv_bfloat16>::value;
+  const int shift = WIDE_Q ? max(0, -76 - __reduce_min_sync(0xffffffffu, e_least)) : 0;
+  const float k_up = __uint_as_float((unsigned)(127 + shift) << 23);
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const float f = fabsf(p.scale_log2) * __uint_as_float((unsigned)(127 + 24 - shift) << 23) * __uint_as_float((unsigned)(127 - e_row[nt]) << 23);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) f_row[nt][c] = __shfl_sync(0xffffffffu, f, (2 * tig + c) * 4);
   }
   // keys that every row sees: from the last row's window on, up to the first row's position
   const int all_hi = pos0 + row0 / p.G, all_lo = p.window > 0 ? max(0, pos0 + (min(n_rows, row0 + 8 * NT) - 1) / p.G - p.window + 1) : 0;
@@ -302,7 +313,7 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, const Item it
   float most_allowed = 0x1p-100f, v_up = __uint_as_float((unsigned)(127 + 100 + 15) << 23);      // p step is at most most_allowed = 2^15 / v_up
 
   // (m_run: the maximum in use, a score times f_row.)
-  // The step's blocks, the first at key0.  MASKED: some key of theirs is hidden from some row or lies behind the last key.
+  // The step's blocks, the first at key0.  MASKED: some key of theirs is hidden from some row or lies behind the last key, or the queries want k_up.
   auto step_of = [&](auto masked, const uint8_t* const first, const int key0, const int n) {
     constexpr bool MASKED = decltype(masked)::value;
     // ---- scores, still to be multiplied by f_row
@@ -333,7 +344,8 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, const Item it
         load_words<GN>(pairs, first + b * B::BYTES + B::K_PAIRS + (gid + 8 * k) * GN * 4);
 #pragma unroll
         for (int g = 0; g < GN; ++g) {
-          const float2 v = pair_values<T>(pairs[g]);
+          float2 v = pair_values<T>(pairs[g]);
+          if (MASKED && WIDE_Q) v.x *= k_up, v.y *= k_up;
           const float mid = fmaf(-8.f, v.x, v.y);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
@@ -540,7 +552,7 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, const Item it
     const uint32_t half = (turn + j) % HALVES;
     failed |= !arrived(bars + 8 * half, (turn + j) / HALVES & 1, failed);
     const uint8_t* first = ring + half * NB * B::BYTES;
-    if (NB * j >= k_lo && NB * j + NB <= min(k_hi, n_blocks)) step_of(std::false_type{}, first, 0, NB);
+    if (shift == 0 && NB * j >= k_lo && NB * j + NB <= min(k_hi, n_blocks)) step_of(std::false_type{}, first, 0, NB);
     else step_of(std::true_type{}, first, base + NB * j * TILE, n_blocks - NB * j);
     if (j % SETTLE == SETTLE - 1) settle();
     __syncwarp();                      // the half is free
