@@ -43,6 +43,7 @@ constexpr int WARPS = 4;
 constexpr int TILE = WARPS * PACKED_POS;     // keys of a unit
 constexpr int NB = 2;                        // blocks of a step: one running maximum for 32 keys
 constexpr float SLACK = 6.f;                 // a weight is at most 2^SLACK times that of the maximum in use
+constexpr float FAR = 0x1p24f;               // scores of which float32 holds whole numbers at best
 constexpr int HEAD = 12;                     // the largest p step so far is brought to 2^(HEAD - 1) to 2^HEAD: room for one of up to 2^15, within float16
 constexpr int SETTLE = 16;                   // steps after which the sums of codes are centred
 constexpr int HALVES = 2;                    // steps in a warp's ring: one is read while the next arrives
@@ -312,8 +313,15 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, const Item it
   *far_e = -100;                       // the largest e of the part, below
   float most_allowed = 0x1p-100f, v_up = __uint_as_float((unsigned)(127 + 100 + 15) << 23);      // p step is at most most_allowed = 2^15 / v_up
 
-  // (m_run: the maximum in use, a score times f_row.)
-  // The step's blocks, the first at key0.  MASKED: some key of theirs is hidden from some row or lies behind the last key, or the queries want k_up.
+  // whole blocks, by their number in the warp: [k_lo, k_hi) hide no key from any row
+  const int base = flow.key_lo + flow.b0 * PACKED_POS;
+  const int k_lo = all_lo > base ? (all_lo - base + TILE - 1) / TILE : 0;
+  int k_hi = shift == 0 && all_hi - PACKED_POS + 1 >= base ? (all_hi - PACKED_POS + 1 - base) / TILE + 1 : 0;
+
+  // (m_run: the maximum in use, a score times f_row.  Its own rounding is a part of a fused exponent, which from scores of FAR on is no longer small: the steps
+  // that follow take the masked form, whose exponents are not fused.)
+  // The step's blocks, the first at key0.  MASKED: some key of theirs is hidden from some row or lies behind the last key, or queries or scores are
+  // so large that they want its ways.
   auto step_of = [&](auto masked, const uint8_t* const first, const int key0, const int n) {
     constexpr bool MASKED = decltype(masked)::value;
     // ---- scores, still to be multiplied by f_row
@@ -385,7 +393,7 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, const Item it
       }
     // ---- exponents against the maximum in use, which moves only when a score leaves it 2^SLACK behind: a vote in its place otherwise
     float x[NB][NT][4], far = -INFINITY;
-    auto exponents = [&]() {
+    if (!MASKED) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -395,9 +403,9 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, const Item it
             x[b][nt][e] = fmaf(s[b][nt][e], f_row[nt][e & 1], -m_run[nt][e & 1]);
             far = fmaxf(far, x[b][nt][e]);
           }
-    };
-    if (!MASKED) exponents();
+    }
     if (MASKED || __any_sync(0xffffffffu, far > SLACK)) {
+      bool large = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -412,6 +420,7 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, const Item it
           // (nothing seen so far: the sums are zeros)
           const float corr = m_run[nt][c] == -INFINITY ? 0.f : exp2_fast(m_run[nt][c] - m_new);
           m_run[nt][c] = m_new;
+          large |= fabsf(m_new) >= FAR && m_new != -INFINITY;
           l_run[nt][c] *= corr;
 #pragma unroll
           for (int g = 0; g < GN; ++g) {
@@ -424,18 +433,15 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, const Item it
             }
           }
         }
+      if (__any_sync(0xffffffffu, large)) k_hi = 0;
       most_allowed = 0.f;            // (what was the largest product may have shrunk to nothing: found anew below)
-      if (MASKED) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
+        for (int e = 0; e < 4; ++e)
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
-              x[b][nt][e] = s[b][nt][e] == -INFINITY ? -INFINITY : fmaf(s[b][nt][e], f_row[nt][e & 1], -m_run[nt][e & 1]);
-      } else {
-        exponents();
-      }
+          for (int b = 0; b < NB; ++b)      // (the product rounded as the maximum was: its own exponent is 0 whatever its size)
+            x[b][nt][e] = MASKED && s[b][nt][e] == -INFINITY ? -INFINITY : __fsub_rn(__fmul_rn(s[b][nt][e], f_row[nt][e & 1]), m_run[nt][e & 1]);
     }
     // ---- weights; times a step they are float16 operands, whose power of two follows the largest product (and not the largest step: a key that
     // nobody looks at must not push the others' weights into the subnormals)
@@ -545,14 +551,11 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, const Item it
           eights[nt][g][c] = 0.f;
         }
   };
-  // whole blocks, by their number in the warp: [k_lo, k_hi) hide no key from any row
-  const int base = flow.key_lo + flow.b0 * PACKED_POS;
-  const int k_lo = all_lo > base ? (all_lo - base + TILE - 1) / TILE : 0, k_hi = all_hi - PACKED_POS + 1 >= base ? (all_hi - PACKED_POS + 1 - base) / TILE + 1 : 0;
   for (int j = 0; j < n_steps; ++j) {
     const uint32_t half = (turn + j) % HALVES;
     failed |= !arrived(bars + 8 * half, (turn + j) / HALVES & 1, failed);
     const uint8_t* first = ring + half * NB * B::BYTES;
-    if (shift == 0 && NB * j >= k_lo && NB * j + NB <= min(k_hi, n_blocks)) step_of(std::false_type{}, first, 0, NB);
+    if (NB * j >= k_lo && NB * j + NB <= min(k_hi, n_blocks)) step_of(std::false_type{}, first, 0, NB);
     else step_of(std::true_type{}, first, base + NB * j * TILE, n_blocks - NB * j);
     if (j % SETTLE == SETTLE - 1) settle();
     __syncwarp();                      // the half is free
