@@ -12,8 +12,10 @@
 //                weights comes from a product with a constant and goes off every 512 keys, so that the sums do not outgrow what they
 //                stand for; the middles' sum on the CUDA cores in float32.
 // Roundings: q, a power of two times itself that puts a row's largest element at 2^14 to 2^15, is a float16 (exactly, from bfloat16 also, but for what is
-// 2^-30 below the largest); p step, times a power of two that follows the largest one seen, is rounded to float16: a weight's half
-// step of 2^-12, and the result's own.  All sums are float32.
+// 2^-30 below the largest); p step, times a power of two that follows the largest one seen by the row in the group, is rounded to float16: a weight's half
+// step of 2^-12, and the result's own.  All sums are float32: an element's weighted sum, values times keys times 2^SLACK at most, has to stay in it.
+// (A power of two of the warp's own instead of each row's and group's took the bits of values that are 2^26 times smaller than what another row, or the other half of
+// a head, looks at; B200, us, it / each its own: 64 x 8,192 keys 135 / 134, one of 700 9.6 / 9.9, 17 x up to 6,000, 4 tokens each, 42 / 44.)
 //
 // The work is handed out on the device, so that the launch does not depend on the lengths and a captured one serves any.  A (request, KV head,
 // rows of 8 NT) is a pair.  Few pairs (OWN CTAs or more for each): each gets a number of CTAs of its own by its length, one part a CTA, of NB units at
@@ -44,7 +46,9 @@ constexpr int TILE = WARPS * PACKED_POS;     // keys of a unit
 constexpr int NB = 2;                        // blocks of a step: one running maximum for 32 keys
 constexpr float SLACK = 6.f;                 // a weight is at most 2^SLACK times that of the maximum in use
 constexpr float FAR = 0x1p24f;               // scores of which float32 holds whole numbers at best
-constexpr int HEAD = 12;                     // the largest p step so far is brought to 2^(HEAD - 1) to 2^HEAD: room for one of up to 2^15, within float16
+constexpr int HEAD = 10;                     // a row's largest p step, when v_up is set by it, comes to 2^(HEAD - 1) to 2^HEAD: 2^6 of room
+constexpr float BEHIND = 6.f;               // the maximum may rise by so much until v_up follows
+constexpr int V_UP_MOST = 115;               // (its exponent: bfloat16's smallest normal steps come to 2^-11 with it)
 constexpr int SETTLE = 16;                   // steps after which the sums of codes are centred
 constexpr int HALVES = 2;                    // steps in a warp's ring: one is read while the next arrives
 static_assert(32 % NB == 0, "the blocks of a step lie in one window of 32 blocks, one a lane");
@@ -213,8 +217,8 @@ struct Flow {
 
 // One item, whose first copies are on their way; next() sends the next item's.
 template <typename T, int D, int NT, typename Next>
-__device__ __forceinline__ void packed_item(const PackedParams& p, const Item it, Flow<D>& flow, uint8_t* ring, uint32_t bars, uint32_t& turn, float* merge, volatile int* far_e,
-                                            bool& failed, Next next) {
+__device__ __forceinline__ void packed_item(const PackedParams& p, const Item it, Flow<D>& flow, uint8_t* ring, uint32_t bars, uint32_t& turn, float* merge, bool& failed,
+                                            Next next) {
   using B = PackedBlock<D>;
   constexpr int GN = B::GROUPS;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tig = lane & 3;
@@ -310,14 +314,29 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, const Item it
         for (int j = 0; j < 4; ++j) o[nt][g][j][c] = o[nt][g][j][2 + c] = 0.f;
       }
     }
-  *far_e = -100;                       // the largest e of the part, below
-  float most_allowed = 0x1p-100f, v_up = __uint_as_float((unsigned)(127 + 100 + 15) << 23);      // p step is at most most_allowed = 2^15 / v_up
+  // what p step is multiplied by before it becomes a float16 operand: of each row and group its own, so that no row, and no half of a head, loses bits to another
+  float v_up[NT][GN][2], m_up[NT][2];      // (m_up: the maximum that v_up goes by)
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int g = 0; g < GN; ++g) v_up[nt][g][0] = v_up[nt][g][1] = __uint_as_float((unsigned)(127 + V_UP_MOST) << 23);
 
   // whole blocks, by their number in the warp: [k_lo, k_hi) hide no key from any row
   const int base = flow.key_lo + flow.b0 * PACKED_POS;
   const int k_lo = all_lo > base ? (all_lo - base + TILE - 1) / TILE : 0;
   int k_hi = shift == 0 && all_hi - PACKED_POS + 1 >= base ? (all_hi - PACKED_POS + 1 - base) / TILE + 1 : 0;
 
+  // v_up and the sums that hold it, times 2^by
+  auto scale_up = [&](int nt, int g, int c, int by) {
+    const float ratio = by < -126 ? 0.f : __uint_as_float((unsigned)(127 + min(by, 127)) << 23);      // (by 2^127 and more: what float32's weights had shrunk to nothing)
+    v_up[nt][g][c] = __uint_as_float(__float_as_uint(v_up[nt][g][c]) + ((unsigned)by << 23));
+    eights[nt][g][c] *= ratio;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      o[nt][g][j][c] *= ratio;
+      o[nt][g][j][2 + c] *= ratio;
+    }
+  };
   // (m_run: the maximum in use, a score times f_row.  Its own rounding is a part of a fused exponent, which from scores of FAR on is no longer small: the steps
   // that follow take the masked form, whose exponents are not fused.)
   // The step's blocks, the first at key0.  MASKED: some key of theirs is hidden from some row or lies behind the last key, or queries or scores are
@@ -405,7 +424,7 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, const Item it
           }
     }
     if (MASKED || __any_sync(0xffffffffu, far > SLACK)) {
-      bool large = false;
+      bool large = false, behind = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -419,7 +438,9 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, const Item it
           const float m_new = fmaxf(m_run[nt][c], mx == -INFINITY ? mx : mx * f_row[nt][c]);
           // (nothing seen so far: the sums are zeros)
           const float corr = m_run[nt][c] == -INFINITY ? 0.f : exp2_fast(m_run[nt][c] - m_new);
+          if (m_run[nt][c] == -INFINITY) m_up[nt][c] = m_new;
           m_run[nt][c] = m_new;
+          behind |= m_new - m_up[nt][c] > BEHIND;
           large |= fabsf(m_new) >= FAR && m_new != -INFINITY;
           l_run[nt][c] *= corr;
 #pragma unroll
@@ -434,7 +455,19 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, const Item it
           }
         }
       if (__any_sync(0xffffffffu, large)) k_hi = 0;
-      most_allowed = 0.f;            // (what was the largest product may have shrunk to nothing: found anew below)
+      // The largest product so far has shrunk with the sums, by 2^BEHIND and more: v_up and the sums rise by what it was, so that what is left of it is where it was, and
+      // products of smaller steps keep their bits.
+      if (__any_sync(0xffffffffu, behind)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int most = (int)fminf(m_run[nt][c] - m_up[nt][c], 300.f);
+            m_up[nt][c] = m_run[nt][c];
+#pragma unroll
+            for (int g = 0; g < GN; ++g) scale_up(nt, g, c, min(most, V_UP_MOST + 127 - (int)(__float_as_uint(v_up[nt][g][c]) >> 23)));
+          }
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -443,75 +476,84 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, const Item it
           for (int b = 0; b < NB; ++b)      // (the product rounded as the maximum was: its own exponent is 0 whatever its size)
             x[b][nt][e] = MASKED && s[b][nt][e] == -INFINITY ? -INFINITY : __fsub_rn(__fmul_rn(s[b][nt][e], f_row[nt][e & 1]), m_run[nt][e & 1]);
     }
-    // ---- weights; times a step they are float16 operands, whose power of two follows the largest product (and not the largest step: a key that
-    // nobody looks at must not push the others' weights into the subnormals)
-    float w[NB][NT][4], most = 0.f;
+    // ---- weights; times a step and v_up they are float16 operands
+    float w[NB][NT][4];
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        float of_key = 0.f;
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const float y = exp2_fast(x[b][nt][2 * k + c]);
-            w[b][nt][2 * k + c] = y;
-            l_run[nt][c] += y;
-            of_key = fmaxf(of_key, y);
-          }
-#pragma unroll
-        for (int g = 0; g < GN; ++g) most = fmaxf(most, of_key * step[b][g][k]);
-      }
-    if (__any_sync(0xffffffffu, most > most_allowed)) {
-      const unsigned top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
-      // top < 2^e; no further down than float32 holds 2^-e with HEAD; a product beyond float32: a weight of 2^SLACK takes it there
-      int e = top < 0x7f800000u ? max(-100, (int)(top >> 23) - 126) : 132;
-      e = max(e, *far_e - 60);       // (the sums so far keep their room: products 2^60 below the largest one that the part has met lose bits)
-      *far_e = max(e, *far_e);       // (every lane writes the same)
-      const float up = __uint_as_float((unsigned)(127 + HEAD - e) << 23), ratio = up / v_up;
-      most_allowed = __uint_as_float(min((unsigned)(127 + e + 15 - HEAD), 254u) << 23);
-      v_up = up;
+        for (int e = 0; e < 4; ++e) {
+          w[b][nt][e] = exp2_fast(x[b][nt][e]);
+          l_run[nt][e & 1] += w[b][nt][e];
+        }
+    // Where a product has left float16: v_up of each row and group whose largest one in the step is beyond 2^HEAD goes down to where it is 2^(HEAD - 1) to 2^HEAD.
+    auto lower = [&]() {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int g = 0; g < GN; ++g)
+        for (int g = 0; g < GN; ++g) {
+          unsigned both = 0;           // the exponents of two columns' largest products
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            eights[nt][g][c] *= ratio;
+          for (int c = 0; c < 2; ++c) {
+            float top = 0.f;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) o[nt][g][j][c] *= ratio;
+            for (int b = 0; b < NB; ++b) top = fmaxf(top, fmaxf(w[b][nt][c] * step[b][g][0], w[b][nt][2 + c] * step[b][g][1]));      // (hidden keys' NaN are passed over)
+            both |= __float_as_uint(top) >> 23 << (16 * c);
           }
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, d));
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            // top < 2^(top - 126); a product beyond float32: a weight of 2^SLACK takes it to 2^132 at most
+            const int top = both >> (16 * c) & 255, now = (int)(__float_as_uint(v_up[nt][g][c]) >> 23) - 127;
+            scale_up(nt, g, c, min(0, HEAD - (top == 255 ? 132 : top - 126) - now));
+          }
+        }
+    };
+    unsigned pf[NB][NT][GN][2];
+    auto operands = [&]() {      // returns whether one is beyond a float16
+      __half2 most = __float2half2_rn(0.f);
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int g = 0; g < GN; ++g)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              // (the weight first: what a row looks away from is 0 whatever its step is)
+              float y0 = w[b][nt][2 * k] * v_up[nt][g][0] * step[b][g][k], y1 = w[b][nt][2 * k + 1] * v_up[nt][g][1] * step[b][g][k];
+              if (MASKED) {            // a key that a row does not see counts for nothing, whatever it holds
+                if (w[b][nt][2 * k] == 0.f) y0 = 0.f;
+                if (w[b][nt][2 * k + 1] == 0.f) y1 = 0.f;
+              }
+              pf[b][nt][g][k] = pack2<__half>(y0, y1);
+              most = __hmax2(most, *reinterpret_cast<__half2*>(&pf[b][nt][g][k]));
+            }
+      const unsigned bits = *reinterpret_cast<unsigned*>(&most);
+      return (bits & 0xffffu) >= 0x7c00u || bits >= 0x7c000000u;
+    };
+    if (__any_sync(0xffffffffu, operands())) {
+      lower();
+      operands();
     }
     // ---- values
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      unsigned pf[NT][GN][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int g = 0; g < GN; ++g) {
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            const float up = step[b][g][k] * v_up;
-            float y0 = w[b][nt][2 * k] * up, y1 = w[b][nt][2 * k + 1] * up;
-            if (MASKED) {              // a key that a row does not see counts for nothing, whatever it holds
-              if (w[b][nt][2 * k] == 0.f) y0 = 0.f;
-              if (w[b][nt][2 * k + 1] == 0.f) y1 = 0.f;
-              if (w[b][nt][2 * k] != 0.f) mid_acc[nt][g][0] = fmaf(w[b][nt][2 * k], mid[b][g][k], mid_acc[nt][g][0]);
-              if (w[b][nt][2 * k + 1] != 0.f) mid_acc[nt][g][1] = fmaf(w[b][nt][2 * k + 1], mid[b][g][k], mid_acc[nt][g][1]);
-            } else {
-              mid_acc[nt][g][0] = fmaf(w[b][nt][2 * k], mid[b][g][k], mid_acc[nt][g][0]);
-              mid_acc[nt][g][1] = fmaf(w[b][nt][2 * k + 1], mid[b][g][k], mid_acc[nt][g][1]);
-            }
-            pf[nt][g][k] = transpose8(pack2<__half>(y0, y1));
+            if (!MASKED || w[b][nt][2 * k] != 0.f) mid_acc[nt][g][0] = fmaf(w[b][nt][2 * k], mid[b][g][k], mid_acc[nt][g][0]);
+            if (!MASKED || w[b][nt][2 * k + 1] != 0.f) mid_acc[nt][g][1] = fmaf(w[b][nt][2 * k + 1], mid[b][g][k], mid_acc[nt][g][1]);
+            pf[b][nt][g][k] = transpose8(pf[b][nt][g][k]);
           }
+          mma_f16(eights[nt][g], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, pf[b][nt][g][0], pf[b][nt][g][1]);
         }
       }
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int g = 0; g < GN; ++g) mma_f16(eights[nt][g], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, pf[nt][g][0], pf[nt][g][1]);
       // keys of the contraction: index 2 tig + i of the first half is row tig * 2 + i of the block, of the second half 8 more
 #pragma unroll
       for (int g = 0; g < GN; ++g) {
@@ -526,7 +568,7 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, const Item it
           for (int h = 0; h < 2; ++h) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-              mma_f16(o[nt][g][2 * half + h], x & 0x000F000Fu, x & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u, pf[nt][g][0], pf[nt][g][1]);
+              mma_f16(o[nt][g][2 * half + h], x & 0x000F000Fu, x & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u, pf[b][nt][g][0], pf[b][nt][g][1]);
             x >>= 8;
             y >>= 8;
           }
@@ -567,7 +609,6 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, const Item it
   next();
 
   // ---- the warps' parts meet, eight rows at a time
-  const float down = 1.f / v_up;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -592,6 +633,7 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, const Item it
       for (int g = 0; g < GN; ++g)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {      // tile j of the group: elements 8 gid + 2 j and, 16 times as large, 8 gid + 2 j + 1
+          const float down = __uint_as_float((254u << 23) - __float_as_uint(v_up[nt][g][c]));      // its reciprocal
           float2 v = make_float2(fmaf(o[nt][g][j][c] * 0x1p24f, down, mid_acc[nt][g][c]), fmaf(o[nt][g][j][2 + c] * 0x1p20f, down, mid_acc[nt][g][c]));
           *reinterpret_cast<float2*>(merge + (warp * 8 + row) * D + g * PACKED_GROUP + 8 * gid + 2 * j) = v;
         }
@@ -712,7 +754,7 @@ attention_packed_kernel(const PackedParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) unsigned long long bars_mem[WARPS * HALVES];
   __shared__ long long s_scan[WARPS];
-  __shared__ int s_req, s_begin, s_far[WARPS];
+  __shared__ int s_req, s_begin;
   __shared__ Way way;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint8_t* ring = smem + warp * HALVES * NB * B::BYTES;
@@ -845,7 +887,7 @@ attention_packed_kernel(const PackedParams p) {
   bool more = next_item(it);
   if (more) flow.begin(p, it, turn, ring, bars);
   while (more) {
-    packed_item<T, D, NT>(p, it, flow, ring, bars, turn, merge, s_far + warp, failed, [&]() {
+    packed_item<T, D, NT>(p, it, flow, ring, bars, turn, merge, failed, [&]() {
       more = next_item(following);
       if (more) flow.begin(p, following, turn, ring, bars);
     });

@@ -85,3 +85,88 @@ def test_equal_scores_far_from_zero(cuda, dtype, up, n):
     part = ((picked - s.cache.mids[0][0, at]).abs() + s.cache.mids[0][0, at].abs()).mean(0)
     out = s.attend().view(n * 4, 128).double()
     assert bool(((out - picked.mean(0)).abs() <= 2.0 ** -11 * part + H.HALF_STEP[dtype] * picked.mean(0).abs() * 1.01 + 1e-6).all())
+
+
+FACTORS = [(torch.bfloat16, 2.0 ** 20, 2.0 ** -20), (torch.bfloat16, 2.0 ** 60, 2.0 ** -60), (torch.bfloat16, 1.0, 2.0 ** -32), (torch.bfloat16, 2.0 ** 30, 1.0),
+           (torch.float16, 2.0 ** 13, 2.0 ** -11)]
+
+
+@pytest.mark.parametrize("dtype,large,small", FACTORS)
+@pytest.mark.parametrize("n", [1, 4])
+@pytest.mark.parametrize("kind", ["heads", "halves", "both"])
+def test_values_far_apart(cuda, dtype, large, small, n, kind):
+    """Query heads of a KV head that look at keys with large and with small values, and heads whose halves are large and small: each row and half keeps
+    its own precision.  Compared after a factor that makes the smallest values about one, so that the bound's absolute part is nothing."""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    rand = lambda *s: torch.randn(*s, device="cuda", generator=g)
+    L, D = 1100, 128
+    side = torch.where(torch.arange(L, device="cuda") % 7 < 3, 1.0, -1.0)
+    keys = 0.2 * rand(1, L, D)
+    keys[0, :, 0] = 60 * side                                          # (a group of its own range in keys: the other elements of that half are lost in its steps)
+    vals = rand(1, L, D)
+    if kind != "halves":
+        vals *= torch.where(side > 0, large, small)[None, :, None]
+    if kind != "heads":
+        vals[..., 64:] *= small if kind == "halves" else 2.0 ** -6
+    q = 0.5 * rand(n, 4, D)
+    q[..., 0] = torch.tensor([30.0, -30.0, 30.0, -30.0], device="cuda")       # scores of +-159: what a head looks away from weighs e^-300
+    s = step_over(keys, vals, q, dtype)
+    out = s.attend().view(n, 4, D).double()
+    assert s.ctx.err.item() == 0
+    up = 2.0 ** 6 / small
+    want, bound = H.attention(s.qkv[:, :4 * D].view(n, 4, D), s.cache.keys[0], s.cache.vals[0] * up, s.cache.mids[0] * up, L - n, s.mixer.scale, 0, dtype)
+    if dtype == torch.float16:
+        bound = bound + 2.0 ** -25 * up             # (half a step of float16's subnormal numbers)
+    over = ((out * up - want).abs() / bound).amax((0, 2)).tolist()
+    assert max(over) <= 1, over
+
+
+@pytest.mark.parametrize("far", [1e9, 1e12, 1e25])
+@pytest.mark.parametrize("heads", [1, 4, 7])
+def test_a_value_that_no_row_attends_to(cuda, far, heads):
+    """However large a value is that no row attends to, in tiles that the rows fill and in tiles that they do not."""
+    g = torch.Generator(device="cuda").manual_seed(heads)
+    rand = lambda *s: torch.randn(*s, device="cuda", generator=g)
+    L = 2100
+    q = rand(1, 1, 128).repeat(1, heads, 1)
+    keys, vals = 0.3 * rand(1, L, 128), rand(1, L, 128)
+    keys[0, 37] = -60 * q[0, 0]
+    vals[0, 37] *= far
+    s = step_over(keys, vals, q, torch.bfloat16)
+    s.check(s.attend(), f"{far}")
+
+
+@pytest.mark.parametrize("large,small", [(1e15, 1e-20), (1e25, 1e-20), (1e10, 1e-25)])
+def test_small_values_behind_large_ones(cuda, large, small):
+    """Keys with large values, then keys that outweigh them by far with small ones: the sums so far shrink to nothing, the small values keep their bits."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    rand = lambda *s: torch.randn(*s, device="cuda", generator=g)
+    L = 2100
+    q = rand(1, 1, 128).repeat(1, 4, 1)
+    keys, vals = 0.3 * rand(1, L, 128), rand(1, L, 128)
+    keys[0, -500:] += 160 * math.sqrt(128) / q[0, 0].square().sum() * q[0, 0]
+    vals[:, :-500] *= large
+    vals[:, -500:] *= small
+    s = step_over(keys, vals, q, torch.bfloat16)
+    out = s.attend().view(1, 4, 128).double()
+    want, bound = H.attention(s.qkv[:, :512].view(1, 4, 128), s.cache.keys[0], s.cache.vals[0] / small, s.cache.mids[0] / small, L - 1, s.mixer.scale, 0, torch.bfloat16)
+    assert bool(((out / small - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("dtype", H.DTYPES)
+@pytest.mark.parametrize("ahead", [False, True])
+def test_many_equal_keys_of_small_weight(cuda, dtype, ahead):
+    """60,000 equal keys, each of 2^-15 of one key's weight, whose weights times a step all round the same way; ahead: behind a key of larger values that
+    the heavy one then outweighs by 2^10."""
+    g = torch.Generator(device="cuda").manual_seed(9)
+    rand = lambda *s: torch.randn(*s, device="cuda", generator=g)
+    L = 60000
+    q = rand(1, 1, 128).repeat(1, 4, 1).to(dtype).float()
+    keys, vals = torch.zeros(1, L, 128, device="cuda"), rand(1, 1, 128).repeat(1, L, 1)
+    one = math.sqrt(128) * math.log(2) / q[0, 0].square().sum() * q[0, 0]            # a score of one power of two
+    keys[0, 40] = 15 * one
+    vals[0, 40] = rand(128)
+    if ahead:
+        keys[0, 2], vals[0, 2] = 5 * one, 1000 * rand(128)
+    s = step_over(keys, vals, q, dtype)
+    s.check(s.attend(), "light keys")
