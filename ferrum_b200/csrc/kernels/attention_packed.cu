@@ -97,6 +97,20 @@ template <typename T> __device__ __forceinline__ float2 pair_values(unsigned v);
 template <> __device__ __forceinline__ float2 pair_values<__nv_bfloat16>(unsigned v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)); }
 template <> __device__ __forceinline__ float2 pair_values<__half>(unsigned v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
 
+// Two results, rounded.  The rounding of a step may carry a group's outermost levels beyond the type, which what they stand for is not: the type's largest number then,
+// as for an infinity (a sum that has left float32); a NaN stays one.
+template <typename T> __device__ __forceinline__ unsigned pack2_within(float lo, float hi);
+template <> __device__ __forceinline__ unsigned pack2_within<__nv_bfloat16>(float lo, float hi) {
+  unsigned r;
+  asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+template <> __device__ __forceinline__ unsigned pack2_within<__half>(float lo, float hi) {
+  unsigned r;
+  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
 template <int N>
 __device__ __forceinline__ void load_words(unsigned (&w)[N], const uint8_t* p) {
   if (N == 2) {
@@ -153,8 +167,8 @@ template <typename T>
 __device__ __forceinline__ void write_row4(const PackedParams& p, int token, int head, int D, int d, float4 acc, float L) {
   const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
   uint2 r;
-  r.x = pack2<T>(acc.x * inv, acc.y * inv);
-  r.y = pack2<T>(acc.z * inv, acc.w * inv);
+  r.x = pack2_within<T>(acc.x * inv, acc.y * inv);
+  r.y = pack2_within<T>(acc.z * inv, acc.w * inv);
   *reinterpret_cast<uint2*>((T*)p.out + (size_t)token * p.ldo + (size_t)head * D + d) = r;
 }
 

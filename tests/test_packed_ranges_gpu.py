@@ -170,3 +170,22 @@ def test_many_equal_keys_of_small_weight(cuda, dtype, ahead):
         keys[0, 2], vals[0, 2] = 5 * one, 1000 * rand(128)
     s = step_over(keys, vals, q, dtype)
     s.check(s.attend(), "light keys")
+
+
+@pytest.mark.parametrize("dtype", H.DTYPES)
+@pytest.mark.parametrize("n,L", [(1, 1), (1, 200), (3, 70)])
+def test_the_largest_values(cuda, dtype, n, L):
+    """Groups that reach the type's largest values, whose outermost levels lie beyond it: results are what the values would be, brought back into the type, as
+    pages brought back to 16 bits are.  (bfloat16: one key, as float32 sums of more leave float32.)"""
+    if dtype == torch.bfloat16 and L > 1:
+        L, n = 1, 1
+    top = torch.finfo(dtype).max
+    vals = torch.zeros(1, L, 128, device="cuda")
+    vals[..., :32], vals[..., 32:64] = top, -top
+    vals[..., 64:96] = top
+    keys = torch.zeros(1, L, 128, device="cuda")
+    s = step_over(keys, vals, torch.ones(n, 2, 128, device="cuda"), dtype)
+    assert float(s.cache.vals[0].max()) > top
+    out = s.attend().view(n, 2, 128).double()
+    want = s.cache.vals[0][0, 0].clamp(-top, top)
+    assert bool(torch.isfinite(out).all()) and bool(((out - want).abs() <= 2 * H.HALF_STEP[dtype] * top).all())
