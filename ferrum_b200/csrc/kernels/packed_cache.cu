@@ -256,6 +256,7 @@ FERRUM_API int ferrum_rope_cache_write_packed(const void* qkv, int dtype, int n_
   FERRUM_CHECK_ARG(!write_kv || (packed_page_ok(page_size) && table_width > 0 && plane && n_pages > 0),
                    "rope_packed: page size %d must be a multiple of %d, and the cache given", page_size, PACKED_POS);
   FERRUM_CHECK_ARG(((uintptr_t)plane & 15) == 0 && page_stride % 16 == 0, "rope_packed: pages must be 16-byte aligned");
+  FERRUM_CHECK_ARG(err_flag != nullptr, "rope_packed: the error flag is required");
   if (n_tokens == 0) return 0;
   const int slots = Hq + (write_kv ? 2 * Hkv : 0), E = D / 32;
   const bool wide = ld % E == 0 && ldq % E == 0 && (((uintptr_t)qkv | (uintptr_t)q_out) & (2 * E - 1)) == 0 && (pairing == 0 || R / 2 % E == 0);
@@ -290,6 +291,7 @@ FERRUM_API int ferrum_unpack_cache(const void* plane, long long page_stride, int
   FERRUM_CHECK_ARG(packed_page_ok(page_size) && table_width > 0 && n_pages > 0 && Hkv > 0 && Hkv <= 65535 && n_items >= 0,
                    "unpack_cache: bad sizes (page size %d must be a multiple of %d)", page_size, PACKED_POS);
   FERRUM_CHECK_ARG((((uintptr_t)plane | (uintptr_t)out) & 15) == 0 && page_stride % 16 == 0, "unpack_cache: operands must be 16-byte aligned");
+  FERRUM_CHECK_ARG(err_flag != nullptr, "unpack_cache: the error flag is required");
   if (n_items == 0) return 0;
   const dim3 grid(n_items, Hkv);
   FERRUM_DISPATCH_16BIT(dtype, T, {

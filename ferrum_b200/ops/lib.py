@@ -226,11 +226,6 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _device_index = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-def _at(t):
-    """A tensor's address for an entry point of `_ARGUMENTS`."""
-    return t.data_ptr() if t is not None else None
-
-
 def _dense(t, dtype, name, ndim):
     """The address of a contiguous CUDA tensor of this type (for the wrappers whose share of a short call counts)."""
     if type(t) is torch.Tensor and t.is_cuda and t.dtype is dtype and t.ndim == ndim and t.is_contiguous():
@@ -245,6 +240,14 @@ def _rows(t, dtype, name):
         _need(t, dtype, name, 2)
         return t.data_ptr(), t.stride(0)
     return t.data_ptr(), t.shape[1]
+
+
+def _flag(err):
+    """The address of an error flag, which kernels write when something is wrong only: an int32 on the GPU."""
+    _need(err, torch.int32, "err")
+    if err.numel() == 0:
+        raise KernelError("err must have an element")
+    return err.data_ptr()
 
 
 def _stream_at():
@@ -821,7 +824,7 @@ def rope_cache_write_packed(qkv, n_tokens, positions, req_of_token, block_table,
     """Rotate q and k and store k and v in the pages of a cache held in 4 bits, quantised by groups of 64 elements.  The turned
     q goes to `q_out` ([>= n_tokens, >= Hq * D]; None: in place).  plane: uint8 [pages, Hkv, page_size / 16, `packed_block_bytes(D)`]."""
     dt = dtype_code(qkv.dtype) if isinstance(qkv, torch.Tensor) and qkv.dtype in SIXTEEN_BIT else _need16(qkv, "qkv", 2)
-    at, ld = _rows(qkv, qkv.dtype, "qkv")
+    (at, ld), err_at = _rows(qkv, qkv.dtype, "qkv"), _flag(err)
     q_at, ldq = (at, ld) if q_out is None else _rows(q_out, qkv.dtype, "q_out")
     cs_at = n_pos = 0
     if R:
@@ -837,7 +840,7 @@ def rope_cache_write_packed(qkv, n_tokens, positions, req_of_token, block_table,
     if _profile is not None:
         _work = (n_tokens * (2 * (2 * Hq + (2 * Hkv if write_kv else 0)) * D + (Hkv * 9 * D // 8 if write_kv else 0)), 0.0)
     _check(lib().ferrum_rope_cache_write_packed(at, dt, n_tokens, ld, q_at, ldq, pos_at, req_at, table_at, block_table.shape[1], cs_at or None, n_pos,
-                                                plane_at, page_stride, n_pages, page_size, Hq, Hkv, D, R, pairing, 1 if write_kv else 0, _at(err),
+                                                plane_at, page_stride, n_pages, page_size, Hq, Hkv, D, R, pairing, 1 if write_kv else 0, err_at,
                                                 _stream_at()), "rope_cache_write_packed")
 
 
@@ -847,6 +850,7 @@ def unpack_cache(plane, page_stride, page_size, block_table, items, out, err):
     raises the error flag."""
     dt = dtype_code(out.dtype) if isinstance(out, torch.Tensor) and out.dtype in SIXTEEN_BIT else _need16(out, "out", 5)
     out_at, items_at, table_at = _dense(out, out.dtype, "out", 5), _dense(items, torch.int32, "items", 2), _dense(block_table, torch.int32, "block_table", 2)
+    err_at = _flag(err)
     held, two, Hkv, page, D = out.shape
     plane_at, n_pages = _need_packed(plane, page_stride, page_size, Hkv, D, "unpack_cache")
     n, pair = items.shape
@@ -855,7 +859,7 @@ def unpack_cache(plane, page_stride, page_size, block_table, items, out, err):
     global _work
     if _profile is not None:
         _work = (n * Hkv * page_size * D * (9 / 8 + 4), 0.0)
-    _check(lib().ferrum_unpack_cache(plane_at, page_stride, n_pages, page_size, table_at, *block_table.shape, items_at, n, out_at, dt, Hkv, D, _at(err),
+    _check(lib().ferrum_unpack_cache(plane_at, page_stride, n_pages, page_size, table_at, *block_table.shape, items_at, n, out_at, dt, Hkv, D, err_at,
                                      _stream_at()), "unpack_cache")
 
 
@@ -881,14 +885,14 @@ def attention_packed(q, out, n_tokens, block_table, q_start, pos0, plane, page_s
     (q_at, ldq), (out_at, ldo) = _rows(q, q.dtype, "q"), _rows(out, q.dtype, "out")
     start_at, pos_at, table_at = _dense(q_start, torch.int32, "q_start", 1), _dense(pos0, torch.int32, "pos0", 1), _dense(block_table, torch.int32, "block_table", 2)
     plane_at, n_pages = _need_packed(plane, page_stride, page_size, Hkv, D, "attention_packed")
-    part_at, counters_at = _dense(part, torch.float32, "part", 1), _dense(counters, torch.int32, "counters", 1)
+    part_at, counters_at, err_at = _dense(part, torch.float32, "part", 1), _dense(counters, torch.int32, "counters", 1), _flag(err)
     n_reqs, (held, width) = pos0.shape[0], block_table.shape
     if q_start.shape[0] != n_reqs + 1 or held < n_reqs or min(q.shape[0], out.shape[0]) < n_tokens:
         raise KernelError("attention_packed: q_start, pos0, block_table and the rows do not agree")
     if q_at == out_at:
         raise KernelError("attention_packed: out must not be q, whose rows several CTAs read")
     _check(lib().ferrum_attention_packed(q_at, ldq, out_at, ldo, dt, plane_at, page_stride, n_pages, page_size, table_at, width, start_at, pos_at, n_reqs,
-                                         n_tokens, part_at, part.shape[0], counters_at, counters.shape[0], Hq, Hkv, D, float(scale), window, _at(err),
+                                         n_tokens, part_at, part.shape[0], counters_at, counters.shape[0], Hq, Hkv, D, float(scale), window, err_at,
                                          _stream_at()), "attention_packed")
 
 
@@ -920,8 +924,7 @@ def sample_filtered(logits, n_rows, out_ids, err, temperature, top_k, top_p, min
     of them in index order at which their running mass exceeds uniform times their whole mass.  NaN logits are never drawn.  A row of NaN
     raises error 6, a temperature, top_p or min_p out of range error 7 (id -1 each), as does a row that the logits or the ids do not
     have (left out).  A row named twice gets the draw of one of its two.  `also_to` (int32) receives the ids as well."""
-    at, ld = _rows(logits, torch.float32, "logits")
-    _need(err, torch.int32, "err")
+    (at, ld), err_at = _rows(logits, torch.float32, "logits"), _flag(err)
     t_at, u_at = _dense(temperature, torch.float32, "temperature", 1), _dense(uniform, torch.float64, "uniform", 1)
     k_at = _dense(top_k, torch.int32, "top_k", 1) if top_k is not None else None
     p_at = _dense(top_p, torch.float32, "top_p", 1) if top_p is not None else None
@@ -938,7 +941,7 @@ def sample_filtered(logits, n_rows, out_ids, err, temperature, top_k, top_p, min
     global _work
     if _profile is not None:
         _work = (n_rows * V * 4, 0.0)
-    _check(lib().ferrum_sample_filtered(at, ld, held, n_rows, V, r_at, t_at, k_at, p_at, m_at, u_at, ids_at, also_at, _at(err), _stream_at()), "sample_filtered")
+    _check(lib().ferrum_sample_filtered(at, ld, held, n_rows, V, r_at, t_at, k_at, p_at, m_at, u_at, ids_at, also_at, err_at, _stream_at()), "sample_filtered")
 
 
 # ----------------------------------------------------------------------------- parallel gated block
