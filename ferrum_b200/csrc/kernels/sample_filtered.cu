@@ -648,7 +648,7 @@ sample_filtered_kernel(const FilterParams p) {
       atomicExch(p.err, code);
     }
   };
-  if (!(T >= 0.f) || T == INFINITY || !(top_p > 0.f) || !(min_p <= 1.f)) {      // (the same for the whole cluster)
+  if (!(T >= 0.f) || T == INFINITY || !(top_p > 0.f && top_p <= 1.f) || !(min_p <= 1.f)) {      // (the same for the whole cluster)
     refuse(7);
     return;
   }
