@@ -708,15 +708,19 @@ sample_filtered_kernel(const FilterParams p) {
   cluster_sync();                   // (no CTA leaves while a peer may still reach into its shared memory)
 }
 
+// The most logits that a CTA keeps in its shared memory; a row of more than MAX_CLUSTER times that is read from global memory every time.
+constexpr int MOST_RESIDENT = 45 * 1024;
+
 template <bool RESIDENT>
 int launch_sample(const FilterParams& p, int n_rows, int ctas, cudaStream_t stream) {
   const int smem = RESIDENT ? p.per * 4 : 0;
-  static int reserved = 0;
-  if (smem > reserved || reserved == 0) {
+  static bool configured = false;
+  if (!configured) {                  // (for the largest slice there is: calls of other threads ask for the same)
+    constexpr int most = RESIDENT ? MOST_RESIDENT * 4 : 0;
     cudaError_t e = cudaFuncSetAttribute(sample_filtered_kernel<RESIDENT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(sample_filtered_kernel<RESIDENT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    FERRUM_CHECK_ARG(e == cudaSuccess, "sample_filtered: cannot reserve %d bytes of shared memory: %s", smem, cudaGetErrorString(e));
-    reserved = max(smem, 1);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(sample_filtered_kernel<RESIDENT>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    FERRUM_CHECK_ARG(e == cudaSuccess, "sample_filtered: cannot reserve %d bytes of shared memory: %s", most, cudaGetErrorString(e));
+    configured = true;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(n_rows, ctas);
@@ -737,9 +741,6 @@ int launch_sample(const FilterParams& p, int n_rows, int ctas, cudaStream_t stre
   FERRUM_CHECK_LAUNCH("sample_filtered");
   return 0;
 }
-
-// The most logits that a CTA keeps in its shared memory; a row of more than MAX_CLUSTER times that is read from global memory every time.
-constexpr int MOST_RESIDENT = 45 * 1024;
 
 // CTAs of a row.  What does not find room waits for a whole row: an SM holds two CTAs whose slices are of up to 16,384 logits or so, and clusters of 16 go
 // onto few SMs at a time.  B200, top-k 50 and top-p 0.9, us with 1 / 4 / 8 / 16 CTAs (-: not measured):

@@ -18,3 +18,30 @@ def test_top_p_out_of_range(cuda, top_p, V):
     ids, err = sample(x, [1.0] * 3, [5, 0, 5], [0.9, top_p, 1.0], [0.0] * 3, [0.5] * 3)
     good, code = sample(x, [1.0] * 3, [5, 0, 5], [0.9, 1.0, 1.0], [0.0] * 3, [0.5] * 3)
     assert code == 0 and err == 7 and ids == [good[0], -1, good[2]]
+
+
+def test_calls_from_several_threads(cuda):
+    """Rows of different lengths, whose CTAs hold slices of different sizes, drawn by threads at a time, each on a stream of its own."""
+    import threading
+    g = torch.Generator(device="cuda").manual_seed(3)
+    sizes = [900, 15000, 40000, 128256, 200001, 300000]
+    logits = [torch.randn(2, V, device="cuda", generator=g) for V in sizes]
+    draw = lambda x: sample(x, [0.8, 1.1], [50, 0], [0.9, 0.8], [0.0, 0.01], [0.3, 0.7])
+    got, together = [None] * len(sizes), threading.Barrier(len(sizes))
+    torch.cuda.synchronize()
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            together.wait(60)
+            try:
+                got[i] = [draw(logits[i]) for _ in range(20)]
+            except Exception as e:      # noqa: BLE001 (the thread's own failure is the test's)
+                got[i] = e
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(sizes))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(300)
+    for x, all_of in zip(logits, got):
+        want = draw(x)
+        assert want[1] == 0 and all_of == [want] * 20
