@@ -937,29 +937,29 @@ FERRUM_API int ferrum_attention_packed_rows() { return PACKED_FEW_ROWS; }
 FERRUM_API long long ferrum_attention_packed_workspace(int D) { return (long long)most_ctas() * 2 * PART_ROWS * (D + 2); }
 
 // part: workspace of ferrum_attention_packed_workspace(D) floats; counters: n_reqs * Hkv * 2 int32 zeros, which the call leaves zeros.
-// Calls that may run at the same time need one of each for themselves.
+// Calls that may run at the same time need one of each for themselves.  row_tiles: rows that a pass over a request's keys takes, in tiles of eight (a request of
+// more than eight takes two passes with one).
 FERRUM_API int ferrum_attention_packed(const void* q, int ldq, void* out, int ldo, int dtype, const void* plane, long long page_stride, int n_pages,
                                        int page_size, const int* block_table, int table_width, const int* q_start, const int* pos0, int n_reqs,
-                                       int n_tokens, float* part, long long part_floats, int* counters, int n_counters, int Hq, int Hkv, int D, float scale, int window,
+                                       int row_tiles, float* part, long long part_floats, int* counters, int n_counters, int Hq, int Hkv, int D, float scale, int window,
                                        int* err_flag, cudaStream_t stream) {
   FERRUM_CHECK_ARG(Hq > 0 && Hkv > 0 && Hq % Hkv == 0, "attention_packed: bad head counts Hq=%d Hkv=%d", Hq, Hkv);
   FERRUM_CHECK_ARG(D == 64 || D == 128, "attention_packed: a cache in 4 bits has heads of 64 or 128 elements, found %d", D);
-  FERRUM_CHECK_ARG(packed_page_ok(page_size) && table_width > 0 && n_pages > 0 && window >= 0 && n_reqs >= 0 && n_tokens >= 0,
+  FERRUM_CHECK_ARG(packed_page_ok(page_size) && table_width > 0 && n_pages > 0 && window >= 0 && n_reqs >= 0,
                    "attention_packed: bad sizes (page size %d must be a multiple of %d)", page_size, PACKED_POS);
+  FERRUM_CHECK_ARG(row_tiles == 1 || row_tiles == 2, "attention_packed: a pass takes one or two tiles of eight rows, found %d", row_tiles);
   FERRUM_CHECK_ARG(err_flag != nullptr, "attention_packed: the error flag is required");
   FERRUM_CHECK_ARG((((uintptr_t)q | (uintptr_t)out | (uintptr_t)plane | (uintptr_t)part) & 15) == 0 && ldq % 8 == 0 && ldo % 8 == 0 && page_stride % 16 == 0,
                    "attention_packed: operands must be 16-byte aligned");
   FERRUM_CHECK_ARG(ldq >= Hq * D && ldo >= Hq * D, "attention_packed: rows of %d and %d elements are too short", ldq, ldo);
   FERRUM_CHECK_ARG(part_floats >= ferrum_attention_packed_workspace(D) && n_counters >= (long long)n_reqs * Hkv * 2, "attention_packed: the workspace is too small");
-  if (n_reqs == 0 || n_tokens == 0) return 0;
+  if (n_reqs == 0) return 0;
   const int G = Hq / Hkv;
   float* part_ml = part + (size_t)most_ctas() * 2 * PART_ROWS * D;
   PackedParams p{q, out, (const uint8_t*)plane, block_table, q_start, pos0, part, part_ml, counters,
                  err_flag, page_stride, ldq, ldo, n_pages, page_size, table_width, (int)std::min<long long>((long long)table_width * page_size, 0x7fffff00), Hq, Hkv, G, window,
                  n_reqs, scale * 1.4426950408889634f};
-  // One row tile of 8 where every request brings a token of at most 8 rows (a longer one takes two passes over its keys), else 16 rows
-  // in one pass.  (64 x 8,192 keys, 4 rows each: 135 us, with 16 rows 202; 700 keys 9.3 and 11.4.)
-  const bool narrow = G <= 8 && n_tokens <= n_reqs;
+  const bool narrow = row_tiles == 1;
   FERRUM_DISPATCH_16BIT(dtype, T, {
     if (D == 64) return narrow ? launch_packed<T, 64, 1>(p, stream) : launch_packed<T, 64, 2>(p, stream);
     return narrow ? launch_packed<T, 128, 1>(p, stream) : launch_packed<T, 128, 2>(p, stream);

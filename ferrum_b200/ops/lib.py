@@ -875,12 +875,21 @@ def attention_packed_workspace(D):
     return int(lib().ferrum_attention_packed_workspace(D))
 
 
-def attention_packed(q, out, n_tokens, block_table, q_start, pos0, plane, page_stride, page_size, Hq, Hkv, D, scale, window, err, part, counters):
+def attention_packed_tiles(tiles, requests):
+    """Tiles of eight rows that a pass of `attention_packed` over a request's keys takes, 1 or 2, for requests that have so many of them in all.  With one, a request
+    of two reads its keys twice; with two, a request of one pays for both, and fewer blocks fit a multiprocessor.  So: one, up to one and a half tiles a request.
+    (B200, bfloat16, 8 KV heads of 128, us, one / two: 64 requests of 8,192 keys, all of one tile 134 / 203, a quarter of two 164 / 206, half of them 193 / 208, all
+    253 / 210; 16 of 700 keys, half of two tiles 18 / 24, all 24 / 25.)"""
+    return 1 if 2 * tiles <= 3 * requests else 2
+
+
+def attention_packed(q, out, n_tokens, block_table, q_start, pos0, plane, page_stride, page_size, Hq, Hkv, D, scale, window, err, part, counters, few=None):
     """Causal grouped-query attention over a cache held in 4 bits, for the requests of the step that bring few rows (decoded tokens, see
     `attention_packed_rows`); the rows of other requests stay as they are.  q_start (int32 [requests + 1]): first token of
     each request; pos0 (int32 [requests]): positions cached before the step, whose own keys must be in the pages already.  part:
     float32 workspace of `attention_packed_workspace(D)` elements; counters: int32, requests x Hkv x 2 zeros, which the call leaves
-    zeros.  Calls that may run at the same time need one of each for themselves."""
+    zeros.  Calls that may run at the same time need one of each for themselves.  few: (tiles of eight rows, requests) of the requests that the call
+    reads, by which it chooses its kernel (`attention_packed_tiles`); None: as if they brought all of the n_tokens."""
     dt = dtype_code(q.dtype) if isinstance(q, torch.Tensor) and q.dtype in SIXTEEN_BIT else _need16(q, "q", 2)
     (q_at, ldq), (out_at, ldo) = _rows(q, q.dtype, "q"), _rows(out, q.dtype, "out")
     start_at, pos_at, table_at = _dense(q_start, torch.int32, "q_start", 1), _dense(pos0, torch.int32, "pos0", 1), _dense(block_table, torch.int32, "block_table", 2)
@@ -891,8 +900,12 @@ def attention_packed(q, out, n_tokens, block_table, q_start, pos0, plane, page_s
         raise KernelError("attention_packed: q_start, pos0, block_table and the rows do not agree")
     if q_at == out_at:
         raise KernelError("attention_packed: out must not be q, whose rows several CTAs read")
+    if few is None:
+        few = (max(n_tokens, n_reqs) * -(-Hq // (8 * Hkv)), n_reqs)
+    if n_tokens == 0 or few[1] == 0:
+        return
     _check(lib().ferrum_attention_packed(q_at, ldq, out_at, ldo, dt, plane_at, page_stride, n_pages, page_size, table_at, width, start_at, pos_at, n_reqs,
-                                         n_tokens, part_at, part.shape[0], counters_at, counters.shape[0], Hq, Hkv, D, float(scale), window, err_at,
+                                         attention_packed_tiles(*few), part_at, part.shape[0], counters_at, counters.shape[0], Hq, Hkv, D, float(scale), window, err_at,
                                          _stream_at()), "attention_packed")
 
 

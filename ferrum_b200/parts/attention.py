@@ -120,14 +120,15 @@ class PagedAttention(Mixer):
         Hq, Hkv, D = self.Hq, self.Hkv, self.D
         few, G = ops.attention_packed_rows(), Hq // Hkv
         kinds = ctx.step_cache.get(("packed", G))
-        if kinds is None:            # whether the step brings decoded tokens, and portions of prompts
-            kinds = ctx.step_cache[("packed", G)] = (any(0 < n * G <= few for n in ctx.h_q_len), ctx.max_q_len * G > few)
-        if kinds[0]:
+        if kinds is None:            # (tiles of eight rows, requests) of the step's decoded tokens; whether it brings portions of prompts
+            rows = [n * G for n in ctx.h_q_len if 0 < n * G <= few]
+            kinds = ctx.step_cache[("packed", G)] = ((sum(-(-n // 8) for n in rows), len(rows)), ctx.max_q_len * G > few)
+        if kinds[0][1]:
             part = ctx.buf("attn_packed_part", (ops.attention_packed_workspace(D),), torch.float32)
             if ops.profiling():      # (a step with prompt portions counts the whole step's work for each kernel)
                 ops.set_work(ops.attention_work(ctx, Hq, Hkv, D, self.window, qkv.element_size(), 9 / 16))
             ops.attention_packed(qkv, out, ctx.n_tokens, table, ctx.q_start, ctx.pos0, cache.plane, cache.page_stride, cache.page_size,
-                                 Hq, Hkv, D, self.scale, self.window, ctx.err, part, ctx.zeros("attn_packed_counters", 2 * ctx.n_reqs * Hkv))
+                                 Hq, Hkv, D, self.scale, self.window, ctx.err, part, ctx.zeros("attn_packed_counters", 2 * ctx.n_reqs * Hkv), few=kinds[0])
         if not kinds[1]:
             return
         items, pages = attention_plan.unpack_plan(ctx, cache.group, G, self.window, cache.page_size, few)

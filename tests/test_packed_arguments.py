@@ -58,3 +58,43 @@ def test_the_error_flag_is_looked_at(calls, name):
         with pytest.raises(KernelError, match="err"):
             call(err)
     assert len(calls) == 1
+
+
+def test_tiles_follow_the_rows_of_the_requests_that_are_read(calls):
+    """The kernel is chosen by the rows of the requests that it reads, not by a step's other tokens."""
+    from ferrum_b200.ops import lib as ops
+    assert [ops.attention_packed_tiles(*f) for f in ((1, 1), (64, 64), (65, 64), (96, 64), (97, 64), (128, 64), (2, 1))] == [1, 1, 1, 1, 2, 2, 2]
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32)
+    x, plane = torch.zeros(40, 256, dtype=torch.bfloat16), torch.zeros(2, 1, 1, 1152, dtype=torch.uint8)
+    call = lambda tokens, requests, Hq, few=None: ops.attention_packed(x, torch.zeros_like(x), tokens, i32(requests, 2), i32(requests + 1), i32(requests), plane, 1152, 16, Hq, 1, 64,
+                                                                       1.0, 0, i32(1), torch.zeros(1), i32(2 * requests), few=few)
+    for tokens, requests, Hq, few, tiles in ((4, 4, 2, None, 1), (8, 4, 2, None, 2), (4, 4, 16, None, 2), (3, 4, 2, None, 1), (40, 4, 2, (3, 3), 1), (40, 4, 2, (6, 3), 2)):
+        calls.clear()
+        call(tokens, requests, Hq, few)
+        assert len(calls) == 1 and calls[0][1][14] == tiles
+    calls.clear()
+    call(0, 4, 2), call(40, 1, 2, (0, 0))
+    assert not calls
+
+
+@pytest.mark.parametrize("G,new,few", [(4, [1] * 64 + [512], (64, 64)), (4, [1] * 63 + [3, 70, 90], (65, 64)), (8, [1, 2, 0, 3], (3, 2)), (4, [1, 2, 2], (3, 3)), (16, [1, 40], (2, 1))])
+def test_a_step_with_portions_of_prompts_names_its_decoded_tokens(monkeypatch, G, new, few):
+    from ferrum_b200.ops import lib as ops
+    from ferrum_b200.parts.attention import PagedAttention
+    seen = []
+
+    class Enough(Exception):
+        pass
+
+    def attention(*a, few=None):
+        seen.append(few)
+        raise Enough
+    monkeypatch.setattr(ops, "attention_packed", attention)
+    mixer = PagedAttention(G * 64, G, 1, 64, None, torch.bfloat16)
+    mixer.set_cache_bits(4)
+    ctx = types.SimpleNamespace(step_cache={}, h_q_len=new, max_q_len=max(new), n_reqs=len(new), n_tokens=sum(new), q_start=None, pos0=None, err=None, block_tables=[None],
+                                buf=lambda *a: None, zeros=lambda *a: None)
+    cache = types.SimpleNamespace(group=0, plane=None, page_stride=1152, page_size=16)
+    with pytest.raises(Enough):
+        mixer.attend(torch.zeros(1, 1, dtype=torch.bfloat16), None, ctx, cache)
+    assert seen == [few]

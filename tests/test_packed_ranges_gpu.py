@@ -189,3 +189,19 @@ def test_the_largest_values(cuda, dtype, n, L):
     out = s.attend().view(n, 2, 128).double()
     want = s.cache.vals[0][0, 0].clamp(-top, top)
     assert bool(torch.isfinite(out).all()) and bool(((out - want).abs() <= 2 * H.HALF_STEP[dtype] * top).all())
+
+
+@pytest.mark.parametrize("dtype", H.DTYPES)
+@pytest.mark.parametrize("tiles", [1, 2])
+@pytest.mark.parametrize("total,new,Hq,Hkv,D,window", [([700], [1], 32, 8, 128, 0), ([300, 5, 2049], [1] * 3, 16, 1, 64, 0), ([90, 200, 31], [2, 1, 2], 14, 2, 128, 0),
+                                                       ([500, 20, 77, 600], [4] * 4, 8, 4, 64, 1), ([900, 3, 128], [3, 3, 1], 5, 1, 128, 100),
+                                                       ([1 + 13 * i % 200 for i in range(300)], [1 + i % 4 for i in range(300)], 12, 3, 128, 0), ([700, 90, 33], [1, 90, 4], 8, 2, 128, 0)])
+def test_either_number_of_tiles(cuda, monkeypatch, dtype, tiles, total, new, Hq, Hkv, D, window):
+    """The rule that picks a pass's rows is one of speed: with either number every request's rows are right."""
+    from ferrum_b200.ops import lib as ops
+    monkeypatch.setattr(ops, "attention_packed_tiles", lambda *few: tiles)
+    total = [max(t, n) for t, n in zip(total, new)]
+    s = H.Step(H.Cache(total, Hkv, D, 16, dtype, 5), new, Hq, 6, window)
+    out = s.attend()
+    assert s.ctx.err.item() == 0
+    s.check(out, f"{tiles} tiles")
