@@ -105,6 +105,11 @@ class CacheLayout:
         return sum((h * ops.packed_block_bytes(d) // 16 if packed else parts * h * d * size) * planes
                    for (h, d, _, parts), planes, packed in zip(self.group_keys, self.group_planes, self.group_packed))
 
+    def scratch_bytes_per_token(self, dtype) -> int:
+        """What a position of the cache may take beside it while a step runs: the pages of one layer that prompt portions see, brought back from 4 bits."""
+        size = torch.empty((), dtype=dtype).element_size()
+        return max([parts * h * d * size for (h, d, _, parts), packed in zip(self.group_keys, self.group_packed) if packed], default=0)
+
 
 class CacheStorage:
     def __init__(self, model, dtype, device, page_size=16, num_pages=None, max_requests=64, max_model_len=None,
@@ -156,6 +161,10 @@ class CacheStorage:
     @staticmethod
     def bytes_per_token_of(model, dtype) -> int:
         return CacheLayout(model).bytes_per_token(dtype)
+
+    @staticmethod
+    def scratch_bytes_per_token_of(model, dtype) -> int:
+        return CacheLayout(model).scratch_bytes_per_token(dtype)
 
     def layer_cache(self, k) -> LayerCache:
         return self._views[k]

@@ -102,7 +102,7 @@ class Engine:
         cfg = model.config
         self.max_model_len = int(max_model_len or getattr(cfg, "n_ctx_train", 4096))
         if num_pages is None:
-            layout_bytes = CacheStorage.bytes_per_token_of(model, td)
+            layout_bytes = CacheStorage.bytes_per_token_of(model, td) + CacheStorage.scratch_bytes_per_token_of(model, td)
             free, _total = torch.cuda.mem_get_info()
             budget = int(free * gpu_memory_fraction) - 2 * (1 << 30)
             num_pages = max(16, min(budget // max(layout_bytes * page_size, 1),

@@ -77,6 +77,10 @@ class Scratch:
             return t[:n].view(*shape)
         if t is None or t.dtype != dtype or t.numel() < n:
             spare = min(2 * t.numel(), limit) if t is not None and t.dtype == dtype else 0
+            if not captured:         # (nothing reads the old one any more: its memory may serve the new one)
+                t = None
+                self._bufs.pop(name, None)
+                self._views.pop(name, None)
             t = torch.empty(max(n, spare, 1), dtype=dtype, device=self.device)
             self._bufs[name] = t
             self.generation += captured
