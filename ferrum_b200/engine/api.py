@@ -9,6 +9,7 @@ temperature (0 = greedy), top_p, seed, stop_tokens; top_k and min_p are this eng
 from __future__ import annotations
 
 import os
+import weakref
 from dataclasses import dataclass, field, replace
 from typing import Dict, List, Optional, Sequence
 
@@ -16,7 +17,7 @@ import numpy as np
 import torch
 
 from .. import host
-from ..cache import CacheStorage
+from ..cache import CacheLayout, CacheStorage
 from ..config import registry
 from ..errors import ConfigError, InvalidRequest
 from ..ops import lib as ops
@@ -97,6 +98,9 @@ class Engine:
         else:
             td = model.dtype
             if cache_bits is not None:
+                packed = any(CacheLayout(model).group_packed)
+                if len(getattr(model, "engine_caches", ())) and (int(cache_bits) == 4) != packed:
+                    raise ConfigError(f"another engine runs this model over a cache in {4 if packed else 8 * td.itemsize} bits; its own model is wanted for one in {cache_bits}")
                 model.set_cache_bits(int(cache_bits))
         self.model, self.dtype, self.device = model, td, device
         cfg = model.config
@@ -109,6 +113,9 @@ class Engine:
                                     (self.max_model_len * max_batch_seqs + page_size - 1) // page_size))
         self.cache = CacheStorage(model, td, device, page_size=page_size, num_pages=num_pages,
                                   max_requests=max_batch_seqs, max_model_len=self.max_model_len)
+        if not hasattr(model, "engine_caches"):
+            model.engine_caches = weakref.WeakSet()
+        model.engine_caches.add(self.cache)
         self.sampler = DeviceSampler(max_batch_seqs, device)
         self.runner = ModelRunner(model, self.cache, max_batch_tokens=max_batch_tokens,
                                   max_batch_requests=max_batch_seqs, err=self.sampler.err)

@@ -52,3 +52,25 @@ def test_pages_fit_the_memory_with_what_they_take_beside_them(cuda, model_dirs, 
     eng = Engine(model_dirs["E"], dtype="bfloat16", cache_bits=bits, max_model_len=2048)
     pages = eng.cache.pools[0].shape[1]
     assert pages * 16 * a_token <= room < (pages + 1) * 16 * a_token
+
+
+@pytest.mark.gpu
+def test_engines_that_share_a_model_share_its_cache_bits(cuda, model_dirs):
+    """A second engine on a model does not change the cache under the first; one that wants other bits is refused as long as the first lives."""
+    import gc
+
+    from ferrum_b200 import Engine
+    from ferrum_b200.engine.api import load_model
+    from ferrum_b200.errors import ConfigError
+    model, _ = load_model(model_dirs["E"], "bfloat16", max_positions=256)
+    make = lambda bits: Engine(model=model, cache_bits=bits, num_pages=16, max_model_len=256)
+    for mine, other in ((16, 4), (4, 16)):
+        first = make(mine)
+        want = first.generate([[5, 17, 3]], 6)
+        with pytest.raises(ConfigError, match="another engine"):
+            make(other)
+        second = make(mine)
+        assert second.generate([[5, 17, 3]], 6) == want and make(None).generate([[5, 17, 3]], 6) == want
+        assert first.generate([[5, 17, 3, 9]], 6) == second.generate([[5, 17, 3, 9]], 6)
+        del first, second
+        gc.collect()
