@@ -35,6 +35,15 @@ def uniform(seed, counter):
     return (_mix64(_mix64(int(seed) & _MASK) ^ int(counter)) >> 11) * 2.0 ** -53
 
 
+def _float32(v):
+    """A filter's value as the kernel gets it, where one below 2^-149 is 0; NaN for what is no number."""
+    try:
+        with np.errstate(over="ignore"):
+            return float("nan") if isinstance(v, (str, bytes, list, tuple)) else float(np.float32(v))
+    except (TypeError, ValueError, OverflowError):
+        return float("nan")
+
+
 @dataclass(frozen=True)
 class Filters:
     """What a draw leaves out (in this order; `ops.sample_filtered` has the definition): all but the top_k largest logits (0:
@@ -50,10 +59,9 @@ class Filters:
             whole = False
         if not whole or not 0 <= self.top_k < 1 << 31:
             raise InvalidRequest("top_k must be a whole number, 0 (off) or more")
-        # what the kernel gets are float32 numbers: one below 2^-149 would be 0 there
-        if not 0 < float(np.float32(self.top_p)) <= 1:
+        if not 0 < _float32(self.top_p) <= 1:
             raise InvalidRequest("top_p must be in (0, 1]")
-        if not 0 <= float(np.float32(self.min_p)) <= 1:
+        if not 0 <= _float32(self.min_p) <= 1:
             raise InvalidRequest("min_p must be in [0, 1]")
 
     @property
