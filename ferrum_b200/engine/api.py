@@ -146,7 +146,7 @@ class Engine:
             sp = replace(sp, temperature=float(temperature))
         if seed is not None:
             sp = replace(sp, seed=int(seed))
-        filters = Filters(sp.top_k, sp.top_p, sp.min_p)
+        filters = Filters(sp.top_k, sp.top_p if sp.temperature > 0 else 1.0, sp.min_p)      # (a greedy request's top_p is not looked at)
         rid = self._next_id if request_id is None else int(request_id)
         self._next_id = max(self._next_id, rid) + 1
         self.scheduler.submit(rid, [int(t) for t in prompt_tokens], int(max_new_tokens), float(sp.temperature),

@@ -45,3 +45,27 @@ def test_calls_from_several_threads(cuda):
     for x, all_of in zip(logits, got):
         want = draw(x)
         assert want[1] == 0 and all_of == [want] * 20
+
+
+def test_greedy_requests_do_not_look_at_top_p(cuda, model_dirs):
+    """Without a temperature top_p stands for nothing, as it did before there were filters, whatever it is; with one it has to be in its range."""
+    from ferrum_b200 import Engine, SamplingParams
+    from ferrum_b200.errors import InvalidRequest
+    eng = Engine(model_dirs["D"], dtype="bfloat16", num_pages=16, max_model_len=64)
+
+    def run(sp):
+        out = []
+        rid = eng.submit([5, 17, 3], 5, sp)
+        while True:
+            for ev in eng.step():
+                assert ev.id == rid
+                if ev.kind != "token":
+                    return out
+                out.append(ev.token)
+    want = run(SamplingParams())
+    for top_p in (0.0, -1.0, 2.0, math.nan, 0.5):
+        assert run(SamplingParams(0.0, top_p)) == want
+    for top_p in (0.0, 2.0, math.nan):
+        with pytest.raises(InvalidRequest, match="top_p"):
+            eng.submit([5, 17, 3], 5, SamplingParams(0.7, top_p))
+    assert not eng._filters
