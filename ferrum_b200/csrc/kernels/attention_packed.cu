@@ -15,22 +15,23 @@
 // 2^-30 below the largest); p step, times a power of two that follows the largest one seen by the row in the group, is rounded to float16: a weight's half
 // step of 2^-12, and the result's own.  All sums are float32: an element's weighted sum, values times keys times 2^SLACK at most, has to stay in it.
 // (A power of two of the warp's own instead of each row's and group's took the bits of values that are 2^26 times smaller than what another row, or the other half of
-// a head, looks at; B200, us, it / each its own: 64 x 8,192 keys 135 / 134, one of 700 9.6 / 9.9, 17 x up to 6,000, 4 tokens each, 42 / 44.)
+// a head, looks at; B200, us, it / each its own: 64 x 8,192 keys 134.8 / 134.0, one of 700 9.6 / 9.8, 17 x up to 6,000, 4 tokens each, 42 / 44, 8 x 8,192 with 16
+// heads a KV head 25.4 / 26.9.)
 //
 // The work is handed out on the device, so that the launch does not depend on the lengths and a captured one serves any.  A (request, KV head,
 // rows of 8 NT) is a pair.  Few pairs (OWN CTAs or more for each): each gets a number of CTAs of its own by its length, one part a CTA, of NB units at
 // least (a step takes as long with one), as a part costs some 4 us beside its keys.  Many: they form one line, a pair as long as its units of 64 keys and EXTRA for
 // that cost, and CTA c of P takes the stretch [c L / P, (c + 1) L / P); pairs of up to WHOLE units (and of no more than a stretch) are not cut but belong
 // to the CTA in whose stretch they begin.  B200, bfloat16, us (D 128, 8 KV heads, where nothing else is said):
-//   OWN 2 / 3: 17 requests of up to 6,000 keys, 4 tokens each 45 / 41; a line always: the same in a window of 2,000, D 64, 20.4 -> 21.6; parts of one unit: 100 keys 7.1 -> 8.6
-//   EXTRA 0 / 6 / 12: 40 requests of 30 to 900 keys, 32 KV heads 102 / 45.6 / 48, 64 x 8,192 keys 138 / 135 / 135, 40 x 30 to 900 keys 31 / 20 / 19
-//   WHOLE 0 / 16 / 64: 64 x 200 keys 20.8 / 17.9 / 17.9, 40 x 465 keys, 32 KV heads 47 / 36 / 36, 64 x 400 to 2,000 keys 35.8 / 36.1 / 39.6
+//   OWN 2 / 3: 17 requests of up to 6,000 keys, 4 tokens each 46 / 44; a line always: 17 in a window of 2,000, D 64, 14.9 -> 16.0; parts of one unit: 100 keys 7.6 -> 9.1
+//   EXTRA 0 / 6 / 12: 40 requests of 30 to 900 keys, 32 KV heads 113 / 47 / 50, 64 x 8,192 keys 139 / 135 / 134, 40 x 30 to 900 keys 33 / 21 / 20
+//   WHOLE 0 / 16 / 64: 64 x 200 keys 21.5 / 18.3 / 18.2, 40 x 465 keys, 32 KV heads 49 / 38 / 38, 64 x 400 to 2,000 keys 36.8 / 36.9 / 39.4
 // A CTA's four warps take every fourth block of 16 positions; a block is one bulk copy into the warp's own ring of stages, and no
 // warp waits for another until its part is done; the first copies of the next part are on their way by then.  Of the CTAs that share a (request, head) the one that comes last adds up the parts, in a fixed order.
 //
-// Measured (B200, bfloat16, D 128, 32 heads on 8 KV heads, in a CUDA graph): 64 requests of 8,192 keys 135 us, 4.5 TB/s of cache where a copy runs at 6.6; one of
-// 131,000 keys 43 us, 3.5 TB/s; 64 of 200 keys 17.9 us; one of 700 keys 9.3 us.  What bounds the long ones is the chain of instructions from a block's codes to its
-// sums, which the 11 warps that an SM's registers hold do not hide: 54 % of the issue slots and of the ALU, 27 % of the matrix pipe, 52 % of the
+// Measured (B200, bfloat16, D 128, 32 heads on 8 KV heads, in a CUDA graph): 64 requests of 8,192 keys 134 us, 4.5 TB/s of cache where a copy runs at 6.6; one of
+// 131,000 keys 43 us, 3.5 TB/s; 64 of 200 keys 18.2 us; one of 700 keys 9.8 us.  What bounds the long ones is the chain of instructions from a block's codes to its
+// sums, which the 11 warps that an SM's registers hold do not hide: 55 % of the issue slots, 54 % of the ALU, 27 % of the matrix pipe, 52 % of the
 // DRAM are busy, and with the copies alone the same kernel takes 107 us.  Two CTAs an SM take 147 us; longer rings or steps of four blocks, for
 // which the third CTA goes, were no faster.
 #include "packed_cache.cuh"
@@ -47,7 +48,7 @@ constexpr int NB = 2;                        // blocks of a step: one running ma
 constexpr float SLACK = 6.f;                 // a weight is at most 2^SLACK times that of the maximum in use
 constexpr float FAR = 0x1p24f;               // scores of which float32 holds whole numbers at best
 constexpr int HEAD = 10;                     // a row's largest p step, when v_up is set by it, comes to 2^(HEAD - 1) to 2^HEAD: 2^6 of room
-constexpr float BEHIND = 6.f;               // the maximum may rise by so much until v_up follows
+constexpr float BEHIND = 6.f;                // the maximum may rise by so much until v_up follows
 constexpr int V_UP_MOST = 115;               // (its exponent: bfloat16's smallest normal steps come to 2^-11 with it)
 constexpr int SETTLE = 16;                   // steps after which the sums of codes are centred
 constexpr int HALVES = 2;                    // steps in a warp's ring: one is read while the next arrives

@@ -7,9 +7,9 @@ h / (Hq/Hkv); the score scale is 1/sqrt(head_dim) unless given.  `window` > 0 ke
 `window` keys only; the reference has no window.
 
 The cache may be held in 4 bits (`set_cache_bits`): the rotary step quantises keys and values on their way into the pages, decoded
-tokens read the packed pages as they are, and the pages that a prompt portion sees are brought back to 16 bits in a scratch
-buffer for the kernels of prompt portions.  Every token reads quantised keys and values, its own portion's included, so a
-prompt's results do not depend on how it is cut.
+tokens (requests of up to 16 rows, tokens x query heads of a KV head, in the step) read the packed pages as they are, and the pages that a longer portion
+of a prompt sees are brought back to 16 bits in a scratch buffer for the kernels of prompt portions.  Every token reads quantised keys and values, its own
+portion's included, so that how a prompt is cut decides on roundings only: a longer portion's keys, values and weights are rounded to the compute type.
 """
 from __future__ import annotations
 
