@@ -84,6 +84,9 @@ class StepEvent:
 _NOTHING_SAMPLED = object()      # stands for the ticket of a batch without sampled rows
 
 
+_caches = weakref.WeakKeyDictionary()      # model -> the caches of the engines that run it
+
+
 class Engine:
     def __init__(self, model_path=None, dtype="bfloat16", random_weights=False, seed=0, page_size=16,
                  num_pages=None, max_batch_tokens=2048, max_batch_seqs=64, chunk_size=0, max_model_len=None,
@@ -105,7 +108,7 @@ class Engine:
             td = model.dtype
             if cache_bits is not None:
                 packed = any(CacheLayout(model).group_packed)
-                if len(getattr(model, "engine_caches", ())) and (int(cache_bits) == 4) != packed:
+                if len(_caches.get(model, ())) and (int(cache_bits) == 4) != packed:
                     raise ConfigError(f"another engine runs this model over a cache in {4 if packed else 8 * td.itemsize} bits; its own model is wanted for one in {cache_bits}")
                 model.set_cache_bits(int(cache_bits))
         self.model, self.dtype, self.device = model, td, device
@@ -119,9 +122,7 @@ class Engine:
                                     (self.max_model_len * max_batch_seqs + page_size - 1) // page_size))
         self.cache = CacheStorage(model, td, device, page_size=page_size, num_pages=num_pages,
                                   max_requests=max_batch_seqs, max_model_len=self.max_model_len)
-        if not hasattr(model, "engine_caches"):
-            model.engine_caches = weakref.WeakSet()
-        model.engine_caches.add(self.cache)
+        _caches.setdefault(model, weakref.WeakSet()).add(self.cache)
         self.sampler = DeviceSampler(max_batch_seqs, device)
         self.runner = ModelRunner(model, self.cache, max_batch_tokens=max_batch_tokens,
                                   max_batch_requests=max_batch_seqs, err=self.sampler.err)
