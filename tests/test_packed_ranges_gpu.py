@@ -205,3 +205,25 @@ def test_either_number_of_tiles(cuda, monkeypatch, dtype, tiles, total, new, Hq,
     out = s.attend()
     assert s.ctx.err.item() == 0
     s.check(out, f"{tiles} tiles")
+
+
+def test_calls_at_the_same_time(cuda):
+    """Calls on streams of their own, each with its own workspace and counters, do not disturb each other."""
+    from ferrum_b200.ops import lib as ops
+    steps, calls = [], []
+    for i, (total, new) in enumerate((([30000], [1]), ([700, 90, 2000], [1, 1, 1]), ([4000, 20], [4, 2]), ([300] * 20, [1] * 20))):
+        s = H.Step(H.Cache(total, 2, 128, 16, torch.bfloat16, i), new, 8, 10 + i)
+        out = torch.empty(s.qkv.shape[0], 8 * 128, dtype=torch.bfloat16, device="cuda")
+        part, counters = torch.empty(ops.attention_packed_workspace(128), device="cuda"), torch.zeros(4 * len(new), dtype=torch.int32, device="cuda")
+        steps.append((s, out, counters, torch.cuda.Stream()))
+        calls.append(lambda s=s, out=out, part=part, counters=counters: ops.attention_packed(
+            s.qkv, out, s.qkv.shape[0], s.ctx.block_tables[0], s.ctx.q_start, s.ctx.pos0, s.view.plane, s.view.page_stride, 16, 8, 2, 128, s.mixer.scale, 0, s.ctx.err, part, counters))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for (_, _, _, stream), call in zip(steps, calls):
+            with torch.cuda.stream(stream):
+                call()
+    torch.cuda.synchronize()
+    for i, (s, out, counters, _) in enumerate(steps):
+        assert s.ctx.err.item() == 0 and not counters.any()
+        s.check(out, f"call {i}")
