@@ -95,8 +95,8 @@ class Engine:
         of the compute type: up to 3.5 times the tokens fit and a decoded token reads that much less, for what 16
         levels cost in precision.  Beside the levels, decoded tokens lose next to nothing; portions of prompts read the levels rounded to the compute type, as they
         read a 16-bit cache (0.0034 off in bfloat16 where rounding the result alone is 0.0017 off).  It is faster where the cache is much of what a step reads:
-        an 8B model (B200, bfloat16, decoded tokens a second, 16 bits / 4) 8 requests of 8,192 tokens 1,776 / 2,017, 64 of them 10,363 / 13,585, 64 of 1,024
-        9,300 / 10,500, but one request of 1,024 310 / 297, one of 8,192 290 / 276, 8 of 1,024 2,190 / 2,120.  With more than 16 query heads on a KV head it
+        an 8B model (B200, bfloat16, ms a step of decoded tokens, 16 bits / 4): 64 requests of 8,192 tokens 15.5 / 8.3, 8 of them 4.64 / 4.05, 64 of 1,024 5.40 / 4.98,
+        8 of 1,024 3.55 / 3.55, but one of 1,024 3.28 / 3.43 and one of 8,192 3.52 / 3.66.  With more than 16 query heads on a KV head it
         saves memory only: every decoded token brings all its pages back to 16 bits.
         For 16-bit Llama models with heads of 64 or 128 elements; others are refused (`ConfigError`).  None: as the model says; a model that another engine
         runs keeps the bits it has."""
