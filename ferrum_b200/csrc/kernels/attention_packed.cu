@@ -10,7 +10,9 @@
 //                of the product (m16n8k16), the packed rows (tokens x query heads of the KV head) its columns;
 //   values       o = sum_j (p_j step_j) (c_j - 8) + p_j middle_j: elements are the rows, keys the contraction; 8 times the sum of the very
 //                weights comes from a product with a constant and goes off every 512 keys, so that the sums do not outgrow what they
-//                stand for; the middles' sum on the CUDA cores in float32.
+//                stand for; the middles' sum on the CUDA cores in float32.  (The matrix unit lines products up by their operands' exponents, 2^-14 for any
+//                subnormal, and cuts what lies 2^-24 or so below the largest: a sum of c * 2^-24 loses 2^-17 of 8 p step, less than a weight's rounding is worth at any
+//                code but 8, one of 16 c * 2^-24 2^-21.  The 8 takes either form, so that the rows of each are cut alike.)
 // Roundings: q, a power of two times itself that puts a row's largest element at 2^14 to 2^15, is a float16 (exactly, from bfloat16 also, but for what is
 // 2^-30 below the largest); p step, times a power of two that follows the largest one seen by the row in the group, is rounded to float16: a weight's half
 // step of 2^-12, and the result's own.  All sums are float32: an element's weighted sum, values times keys times 2^SLACK at most, has to stay in it.
@@ -346,6 +348,7 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, const Item it
     const float ratio = by < -126 ? 0.f : __uint_as_float((unsigned)(127 + min(by, 127)) << 23);      // (by 2^127 and more: what float32's weights had shrunk to nothing)
     v_up[nt][g][c] = __uint_as_float(__float_as_uint(v_up[nt][g][c]) + ((unsigned)by << 23));
     eights[nt][g][c] *= ratio;
+    eights[nt][g][2 + c] *= ratio;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       o[nt][g][j][c] *= ratio;
@@ -462,6 +465,7 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, const Item it
           for (int g = 0; g < GN; ++g) {
             mid_acc[nt][g][c] *= corr;
             eights[nt][g][c] *= corr;
+            eights[nt][g][2 + c] *= corr;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               o[nt][g][j][c] *= corr;
@@ -566,7 +570,7 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, const Item it
             if (!MASKED || w[b][nt][2 * k + 1] != 0.f) mid_acc[nt][g][1] = fmaf(w[b][nt][2 * k + 1], mid[b][g][k], mid_acc[nt][g][1]);
             pf[b][nt][g][k] = transpose8(pf[b][nt][g][k]);
           }
-          mma_f16(eights[nt][g], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, pf[b][nt][g][0], pf[b][nt][g][1]);
+          mma_f16(eights[nt][g], 0x00080008u, 0x00800080u, 0x00080008u, 0x00800080u, pf[b][nt][g][0], pf[b][nt][g][1]);
         }
       }
       // keys of the contraction: index 2 tig + i of the first half is row tig * 2 + i of the block, of the second half 8 more
@@ -603,9 +607,9 @@ __device__ __forceinline__ void packed_item(const PackedParams& p, const Item it
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             o[nt][g][j][c] -= eights[nt][g][c];
-            o[nt][g][j][2 + c] = fmaf(-16.f, eights[nt][g][c], o[nt][g][j][2 + c]);
+            o[nt][g][j][2 + c] -= eights[nt][g][2 + c];
           }
-          eights[nt][g][c] = 0.f;
+          eights[nt][g][c] = eights[nt][g][2 + c] = 0.f;
         }
   };
   for (int j = 0; j < n_steps; ++j) {

@@ -227,3 +227,23 @@ def test_calls_at_the_same_time(cuda):
     for i, (s, out, counters, _) in enumerate(steps):
         assert s.ctx.err.item() == 0 and not counters.any()
         s.check(out, f"call {i}")
+
+
+@pytest.mark.parametrize("dtype", H.DTYPES)
+@pytest.mark.parametrize("light", [3, 40, 400])
+@pytest.mark.parametrize("scale", [0.7, 1.0, 1.9])
+def test_middles_of_a_heavy_key(cuda, dtype, light, scale):
+    """A key of nearly all the weight whose values are their group's middle, 0, but for two: what the others' small values add up to is left, even elements and odd
+    ones.  Two sums, of the codes and of 8, are cut at 2^-17 of 8 steps of the heavy key each, beside the bound of float32 sums."""
+    g = torch.Generator(device="cuda").manual_seed(light)
+    rand = lambda *s: torch.randn(*s, device="cuda", generator=g)
+    L = light + 1
+    q = rand(1, 1, 128).repeat(1, 4, 1).to(dtype).float()
+    keys, vals = 0.02 * rand(1, L, 128), 0.02 * rand(1, L, 128)
+    keys[0, 5 % L] += 7 * math.sqrt(128) / q[0, 0].square().sum() * q[0, 0]
+    vals[0, 5 % L] = 0
+    vals[0, 5 % L, ::64], vals[0, 5 % L, 1::64] = -8 * scale, 7 * scale
+    s = step_over(keys, vals, q, dtype)
+    out = s.attend().view(1, 4, 128).double()
+    want, bound = H.attention(s.qkv[:, :512].view(1, 4, 128), s.cache.keys[0], s.cache.vals[0], s.cache.mids[0], L - 1, s.mixer.scale, 0, dtype)
+    assert bool(((out - want).abs() <= bound + 2 * 2.0 ** -17 * 8 * scale).all())
